@@ -18,7 +18,9 @@ LIB = os.path.join(LIBDIR, "libpgt_hip.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 ARCH = "gfx950"
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-I", INCLUDE, "-I", CSRC,
-         "-Wno-unused-result", "-ffp-contract=on"]
+         "-Wno-unused-result", "-ffp-contract=on",
+         # no v_pk_{add,mul,fma}_f32: some of their forms have given wrong results on MI355X now and then
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _hipcc():
