@@ -311,6 +311,65 @@ int pgt_mha(int32_t dtype, const void* q, int32_t ldq, const void* k, int32_t ld
             int32_t ldv, void* out, int32_t ldo, int32_t B, int32_t L, int32_t heads, int32_t hd,
             float scale, pgt_stream_t stream);
 
+/* ---- attention over a cache of earlier tokens (no reference counterpart: the reference's attention, codeformer_arch.py:105,129, sees
+ * one window at a time; these carry its keys and values from step to step) -------------------------------------------------------
+ * dtype PGT_F32, PGT_BF16 or PGT_F16 (type of q, k, v and outputs; statistics, sums and angles are fp32 or wider); rows 16-byte aligned
+ * with row strides (elements) that are multiples of 16 bytes; anything else: -22.
+ *
+ * pgt_qk_norm_rope: per head row x of hd elements (32, 64, 128 or 256), for the `heads` heads of q and the `kv_heads` of k (0 of one: skipped):
+ *   y = R(pos) (gain * x / sqrt(mean(x^2) + eps)),  one rounding at the store.  q_gain, k_gain: fp32 (hd), NULL = ones.
+ * R turns pair i of the first `rot` elements (a multiple of 8, <= hd; 0: no rotation, positions and freqs may be NULL) by 2 pi * positions[row]
+ * * freqs[i]: freqs (rot / 2) in REVOLUTIONS per position, fp64, the product reduced in fp64 (any int32 position).  Pairs are
+ * (i, i + rot / 2), or (2i, 2i + 1) with interleaved != 0.  An output may be its own input (same pointer and stride).
+ * pgt_qk_norm_rope_backward: dq, dk (gradients of the outputs) -> dq_in, dk_in (gradients of q, k; may be dq, dk themselves) and the fp32
+ * gain gradients (hd; NULL: not wanted), summed over rows and heads in a fixed order (bit-reproducible).  q, k are the forward's inputs.
+ * workspace: pgt_qk_norm_rope_backward_workspace_bytes(rows, hd) bytes. */
+int pgt_qk_norm_rope(int32_t dtype, const void* q, int32_t ldq, const void* k, int32_t ldk, int32_t rows, int32_t heads,
+                     int32_t kv_heads, int32_t hd, const int32_t* positions, const double* freqs, int32_t rot,
+                     int32_t interleaved, const float* q_gain, const float* k_gain, float eps, void* q_out, int32_t ldqo,
+                     void* k_out, int32_t ldko, pgt_stream_t stream);
+size_t pgt_qk_norm_rope_backward_workspace_bytes(int32_t rows, int32_t hd);
+int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const void* dk, int32_t lddk, const void* q, int32_t ldq,
+                              const void* k, int32_t ldk, int32_t rows, int32_t heads, int32_t kv_heads, int32_t hd,
+                              const int32_t* positions, const double* freqs, int32_t rot, int32_t interleaved, const float* q_gain,
+                              const float* k_gain, float eps, void* dq_in, int32_t lddqi, void* dk_in, int32_t lddki,
+                              float* dq_gain, float* dk_gain, void* workspace, size_t workspace_bytes, pgt_stream_t stream);
+
+/* The cache holds keys and values in 8 bits, in pages of `page` tokens (16, 32, 64 or 128) of all kv heads; hd 64 or 128:
+ *   k_pages (pages, kv_heads, hd / 16, page, 16), v_pages (pages, kv_heads, page / 16, hd, 16): e4m3 codes (OCP, no infinities);
+ *   k_scale, v_scale (pages, kv_heads) fp32: value = code * scale, scale = 2^e with the least e in [-32, 32] for which the largest |x| of the
+ *   page and head is <= 448 * 2^e.  Larger values and infinities saturate, NaN stays NaN and does not count for the scale.
+ * table (B, ld_table) int32: table[b][i] = page that holds tokens i * page .. of sequence b, `width` entries used; entries outside
+ * [0, pages) and tokens past width * page are not there: nothing is written to them, they read as zeros, attention does not see them.
+ * Sequence b owns rows cu[b] .. cu[b + 1] - 1 of the packed rows (cu: B + 1 int32 on the device, non-decreasing), at most max_new / max_rows
+ * of them; cu == NULL: rows b * max_new .. .  Rows that no sequence owns are neither read nor written.  lens, start: int32 (B),
+ * negative = 0.  All index tensors live on the device and are bounded there: no value of theirs reaches outside the buffers.
+ * pgt_kv_append: writes the rows k, v (kv_heads * hd) of sequence b to its tokens lens[b] .. (lens: tokens BEFORE the call).  A page that
+ * held tokens of the sequence keeps the larger of its scale and the new tokens' - its codes are re-expressed under it; a page that begins
+ * here is written whole, zeros behind the last token.  A page that is written to must belong to one sequence.
+ * pgt_kv_read: rows of sequence b <- its tokens start[b] .. , values rounded once to dtype.
+ * pgt_kv_attention: out = softmax(scale * q K^T) V; q, out rows of heads * hd, `heads` a multiple of kv_heads (head h reads kv head
+ * h / (heads / kv_heads)).  lens: tokens INCLUDING the rows' own: row i of n of sequence b is at position p = lens[b] - n + i.
+ *   causal == 0: sees tokens < lens[b].   causal = c >= 1: tokens < e = (p / c + 1) * c (and < lens[b]): c = 1 token by token, c = 1024 the whole
+ *   frames of 1024 tokens up to its own.  window = w > 0 (with causal): of these the tokens >= e - w.
+ * A row that sees no token is zero.  Deterministic.  workspace: pgt_kv_attention_workspace_bytes(...) bytes (0: may be NULL),
+ * scratch of one call - calls that may run concurrently need their own. */
+int pgt_kv_append(int32_t dtype, const void* k, int32_t ldk, const void* v, int32_t ldv, void* k_pages, void* v_pages,
+                  float* k_scale, float* v_scale, int32_t pages, int32_t page, int32_t kv_heads, int32_t hd, const int32_t* table,
+                  int32_t ld_table, int32_t width, const int32_t* lens, const int32_t* cu, int32_t B, int32_t rows,
+                  int32_t max_new, pgt_stream_t stream);
+int pgt_kv_read(int32_t dtype, void* k_out, int32_t ldk, void* v_out, int32_t ldv, const void* k_pages, const void* v_pages,
+                const float* k_scale, const float* v_scale, int32_t pages, int32_t page, int32_t kv_heads, int32_t hd,
+                const int32_t* table, int32_t ld_table, int32_t width, const int32_t* start, const int32_t* cu, int32_t B,
+                int32_t rows, int32_t max_rows, pgt_stream_t stream);
+size_t pgt_kv_attention_workspace_bytes(int32_t B, int32_t max_new, int32_t heads, int32_t kv_heads, int32_t hd, int32_t width,
+                                        int32_t page);
+int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const void* k_pages, const void* v_pages, const float* k_scale,
+                     const float* v_scale, int32_t pages, int32_t page, int32_t kv_heads, int32_t hd, const int32_t* table,
+                     int32_t ld_table, int32_t width, const int32_t* lens, const int32_t* cu, int32_t B, int32_t rows,
+                     int32_t max_new, int32_t heads, float scale, int32_t causal, int32_t window, void* out, int32_t ldo,
+                     void* workspace, size_t workspace_bytes, pgt_stream_t stream);
+
 /* ---- split-half (PGT_F16X3) forms of the normalisation / attention entry points ------------------------------
  * Same arithmetic as the functions above on tensors stored as [hi | lo] half planes; every tensor argument carries the
  * element offset of its lo plane (`*_lo`) next to its row stride.  Statistics, softmax and accumulation are fp32;

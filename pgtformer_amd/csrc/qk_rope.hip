@@ -1,0 +1,268 @@
+// Per-head RMS norm of queries and keys with the position rotation in the same pass, and its gradient.
+//
+//   y = R(pos) (g * x * r),   r = 1 / sqrt(mean(x^2) + eps)      per head row x of hd elements, fp32 inside, one rounding at the store
+//   R turns pair i of the first `rot` elements by the angle 2 pi * pos * freqs[i] (freqs in revolutions per position, fp64): pairs are
+//   (i, i + rot / 2), or (2i, 2i + 1) in the interleaved form; the elements behind `rot` are not turned.
+// gradient: z = R(-pos) dy, u = g * z, xh = x * r:   dx = r (u - xh * mean(xh * u)),   dg = sum over rows and heads of z * xh
+//
+// Memory bound: x is read once and y written once.  hd / 8 lanes hold a head row, 8 elements each, picked so that both halves of
+// every pair sit in one lane (a rotation needs no exchange; the mean is one shuffle reduction).  The angle is taken in fp64 and
+// reduced to a fraction of a turn before it is rounded to fp32 - exact for any int32 position - once per token and pair, into
+// LDS, for all heads of the token.
+#include "kv_common.h"
+#include "pgt_internal.h"
+
+namespace {
+
+// 8 elements of one head row: two runs of 4 (16-bit: 8 bytes each, fp32: 16 bytes each)
+template <typename T> __device__ __forceinline__ void ld4(const T* p, float* f) {
+    const uint2 w = *reinterpret_cast<const uint2*>(p);
+    if constexpr (__is_same(T, bf16_t)) {
+        f[0] = __uint_as_float(w.x << 16); f[1] = __uint_as_float(w.x & 0xffff0000u);
+        f[2] = __uint_as_float(w.y << 16); f[3] = __uint_as_float(w.y & 0xffff0000u);
+    } else {
+        const halfx2 a = __builtin_bit_cast(halfx2, w.x), b = __builtin_bit_cast(halfx2, w.y);
+        f[0] = (float)a.x; f[1] = (float)a.y; f[2] = (float)b.x; f[3] = (float)b.y;
+    }
+}
+template <> __device__ __forceinline__ void ld4<float>(const float* p, float* f) {
+    const float4 w = *reinterpret_cast<const float4*>(p);
+    f[0] = w.x; f[1] = w.y; f[2] = w.z; f[3] = w.w;
+}
+
+struct RopeP {
+    const void *q, *k, *dq, *dk;      // dq, dk: gradient form only
+    void *qo, *ko;
+    const int32_t* pos;
+    const double* freqs;
+    const float *qg, *kg;
+    float* part;                      // gradient form: (workgroups, 2, hd) partial sums of dg
+    int ldq, ldk, lddq, lddk, ldqo, ldko;
+    int rows, heads, kv_heads, rot, inter, tok;
+    float eps;
+};
+
+constexpr int MAXTOK = 4;
+
+template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void qk_rope_kernel(const RopeP p) {
+    constexpr int LPH = HD / 8, NG = 256 / LPH;      // lanes per head row, head rows in flight per workgroup
+    __shared__ float2 turn[MAXTOK][HD / 2];
+    const int tid = threadIdx.x, j = tid % LPH, grp = tid / LPH;
+    const int nh = p.heads + p.kv_heads, half = p.rot >> 1;
+    const bool turned = 8 * j < p.rot;
+    // the two runs of 4 elements this lane holds, and its first pair (pairs pr .. pr + 3)
+    const int lo = turned && !p.inter ? 4 * j : 8 * j;
+    const int hi = turned && !p.inter ? half + 4 * j : 8 * j + 4;
+    const int pr = 4 * j;
+    float gq[8], gk[8], sq[8], sk[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int d = (e < 4 ? lo : hi - 4) + e;
+        gq[e] = p.qg ? p.qg[d] : 1.f;
+        gk[e] = p.kg ? p.kg[d] : 1.f;
+        sq[e] = sk[e] = 0.f;
+    }
+    const int nblk = (p.rows + p.tok - 1) / p.tok;
+    for (int blk = blockIdx.x; blk < nblk; blk += gridDim.x) {
+        const int t0 = blk * p.tok, nt = min(p.tok, p.rows - t0);
+        for (int i = tid; i < nt * half; i += 256) {
+            const int t = i / half, c = i - t * half;
+            const double rev = (double)p.pos[t0 + t] * p.freqs[c];
+            float s, cs;
+            sincospif((float)(2.0 * (rev - rint(rev))), &s, &cs);
+            turn[t][c] = make_float2(cs, s);
+        }
+        __syncthreads();
+        for (int task = blockIdx.y * NG + grp; task < nt * nh; task += NG * gridDim.y) {
+            const int t = task / nh, h = task - t * nh;
+            const bool isq = h < p.heads;
+            const int hh = isq ? h : h - p.heads;
+            const size_t row = t0 + t;
+            const T* x = (const T*)(isq ? p.q : p.k) + row * (isq ? p.ldq : p.ldk) + hh * HD;
+            float f[8], z[8];
+            ld4(x + lo, f);
+            ld4(x + hi, f + 4);
+            if constexpr (BWD) {
+                const T* dy = (const T*)(isq ? p.dq : p.dk) + row * (isq ? p.lddq : p.lddk) + hh * HD;
+                ld4(dy + lo, z);
+                ld4(dy + hi, z + 4);
+            }
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+#pragma unroll
+            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
+            const float r = 1.f / sqrtf(ss * (1.f / HD) + p.eps);
+            float* v = BWD ? z : f;
+            if constexpr (!BWD) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = f[e] * r * (isq ? gq[e] : gk[e]);
+            }
+            if (turned) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 cs = turn[t][pr + e];
+                    const float s = BWD ? -cs.y : cs.y;
+                    if (p.inter) {
+                        const float a = v[2 * e], b = v[2 * e + 1];
+                        v[2 * e] = a * cs.x - b * s;
+                        v[2 * e + 1] = b * cs.x + a * s;
+                    } else {
+                        const float a = v[e], b = v[4 + e];
+                        v[e] = a * cs.x - b * s;
+                        v[4 + e] = b * cs.x + a * s;
+                    }
+                }
+            }
+            if constexpr (BWD) {
+                float dot = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    f[e] *= r;
+                    const float w = z[e] * f[e];
+                    if (isq) sq[e] += w;
+                    else sk[e] += w;
+                    z[e] *= isq ? gq[e] : gk[e];
+                    dot += f[e] * z[e];
+                }
+#pragma unroll
+                for (int o = LPH / 2; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
+                dot *= 1.f / HD;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) z[e] = r * (z[e] - f[e] * dot);
+            }
+            T* y = (T*)(isq ? p.qo : p.ko) + row * (isq ? p.ldqo : p.ldko) + hh * HD;
+            store4(y + lo, v);
+            store4(y + hi, v + 4);
+        }
+        __syncthreads();
+    }
+    if constexpr (BWD) {      // the workgroup's share of dg: head rows in flight added in order
+        __shared__ float red[2][NG][HD];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int d = (e < 4 ? lo : hi - 4) + e;
+            red[0][grp][d] = sq[e];
+            red[1][grp][d] = sk[e];
+        }
+        __syncthreads();
+        for (int i = tid; i < 2 * HD; i += 256) {
+            const int w = i / HD, d = i - w * HD;
+            float s = 0.f;
+            for (int g = 0; g < NG; ++g) s += red[w][g][d];
+            p.part[(size_t)blockIdx.x * (2 * HD) + i] = s;
+        }
+    }
+}
+
+// dg[i] = sum over the n workgroups of part[w][i], in a fixed order (fp64: up to 1024 terms); 16 outputs per workgroup
+__global__ __launch_bounds__(256) void qk_rope_gain_kernel(const float* __restrict__ part, int n, int hd, float* __restrict__ dqg,
+                                                           float* __restrict__ dkg) {
+    __shared__ double red[16][17];
+    const int c = threadIdx.x & 15, s = threadIdx.x >> 4, i = blockIdx.x * 16 + c;
+    double a = 0;
+    for (int w = s; w < n; w += 16) a += part[(size_t)w * (2 * hd) + i];
+    red[s][c] = a;
+    __syncthreads();
+    if (s == 0) {
+        for (int w = 1; w < 16; ++w) a += red[w][c];
+        float* out = i < hd ? dqg : dkg;
+        if (out) out[i < hd ? i : i - hd] = (float)a;
+    }
+}
+
+// tokens per workgroup: 1 until the grid fills the chip, then 4 share one pass over the angles
+int rope_tok(int rows) { return rows >= 4096 ? MAXTOK : 1; }
+int rope_bwd_groups(int rows) {
+    const int n = (rows + rope_tok(rows) - 1) / rope_tok(rows);
+    return n < 1024 ? n : 1024;
+}
+
+int check(int dtype, const RopeP& p, int hd, bool bwd) {
+    PGT_CHECK(dtype == PGT_F32 || dtype == PGT_BF16 || dtype == PGT_F16, "qk_norm_rope: bad dtype %d", dtype);
+    PGT_CHECK(hd == 32 || hd == 64 || hd == 128 || hd == 256, "qk_norm_rope: head_dim=%d unsupported (32, 64, 128, 256)", hd);
+    PGT_CHECK(p.rows >= 0 && p.heads >= 0 && p.kv_heads >= 0 && p.heads + p.kv_heads > 0 && (int64_t)p.heads * hd < (1 << 30) &&
+              (int64_t)p.kv_heads * hd < (1 << 30), "qk_norm_rope: rows=%d heads=%d kv_heads=%d", p.rows, p.heads, p.kv_heads);
+    PGT_CHECK(p.rot >= 0 && p.rot <= hd && p.rot % 8 == 0, "qk_norm_rope: %d rotated elements of %d (a multiple of 8)", p.rot, hd);
+    PGT_CHECK(p.eps >= 0.f, "qk_norm_rope: eps=%g", p.eps);
+    PGT_CHECK(!p.heads || p.rows == 0 || (p.q && p.qo && (!bwd || p.dq)), "qk_norm_rope: null argument");
+    PGT_CHECK(!p.kv_heads || p.rows == 0 || (p.k && p.ko && (!bwd || p.dk)), "qk_norm_rope: null argument");
+    PGT_CHECK(!p.rot || p.rows == 0 || (p.pos && p.freqs), "qk_norm_rope: a rotation needs positions and freqs");
+    const int al = dtype == PGT_F32 ? 4 : 8;      // elements of 16 bytes
+    const int nq = p.heads ? 1 : 0, nk = p.kv_heads ? 1 : 0;
+    PGT_CHECK((!nq || (p.ldq >= p.heads * hd && p.ldqo >= p.heads * hd && (!bwd || p.lddq >= p.heads * hd))) &&
+              (!nk || (p.ldk >= p.kv_heads * hd && p.ldko >= p.kv_heads * hd && (!bwd || p.lddk >= p.kv_heads * hd))),
+              "qk_norm_rope: a row stride is shorter than its row");
+    PGT_CHECK(nq * (p.ldq | p.ldqo | (bwd ? p.lddq : 0)) % al == 0 && nk * (p.ldk | p.ldko | (bwd ? p.lddk : 0)) % al == 0,
+              "qk_norm_rope: row strides must be multiples of 16 bytes");
+    const uintptr_t a = nq * ((uintptr_t)p.q | (uintptr_t)p.qo | (uintptr_t)p.dq) | nk * ((uintptr_t)p.k | (uintptr_t)p.ko | (uintptr_t)p.dk);
+    PGT_CHECK((a & 15) == 0, "qk_norm_rope: misaligned pointer");
+    return 0;
+}
+
+template <bool BWD> void launch(int dtype, int hd, const RopeP& p, dim3 grid, hipStream_t st) {
+#define ROPE_GO(TT, HD) hipLaunchKernelGGL((qk_rope_kernel<TT, HD, BWD>), grid, dim3(256), 0, st, p)
+#define ROPE_HD(TT)                                                                                                       \
+    do {                                                                                                                  \
+        if (hd == 32) ROPE_GO(TT, 32);                                                                                    \
+        else if (hd == 64) ROPE_GO(TT, 64);                                                                               \
+        else if (hd == 128) ROPE_GO(TT, 128);                                                                             \
+        else ROPE_GO(TT, 256);                                                                                            \
+    } while (0)
+    if (dtype == PGT_F32) ROPE_HD(float);
+    else if (dtype == PGT_BF16) ROPE_HD(bf16_t);
+    else ROPE_HD(half_t);
+#undef ROPE_HD
+#undef ROPE_GO
+}
+
+}  // namespace
+
+extern "C" int pgt_qk_norm_rope(int32_t dtype, const void* q, int32_t ldq, const void* k, int32_t ldk, int32_t rows, int32_t heads,
+                                int32_t kv_heads, int32_t hd, const int32_t* positions, const double* freqs, int32_t rot,
+                                int32_t interleaved, const float* q_gain, const float* k_gain, float eps, void* q_out, int32_t ldqo,
+                                void* k_out, int32_t ldko, pgt_stream_t stream) {
+    RopeP p = {};
+    p.q = q; p.k = k; p.qo = q_out; p.ko = k_out; p.pos = positions; p.freqs = freqs; p.qg = q_gain; p.kg = k_gain;
+    p.ldq = ldq; p.ldk = ldk; p.ldqo = ldqo; p.ldko = ldko;
+    p.rows = rows; p.heads = heads; p.kv_heads = kv_heads; p.rot = rot; p.inter = interleaved != 0; p.eps = eps;
+    if (const int rc = check(dtype, p, hd, false)) return rc;
+    if (rows == 0) return 0;
+    p.tok = rope_tok(rows);
+    const int ng = 256 / (hd / 8), nh = heads + kv_heads;
+    const dim3 grid((rows + p.tok - 1) / p.tok, p.tok == 1 ? (nh + ng - 1) / ng : 1);
+    PGT_CHECK(grid.y <= 65535, "qk_norm_rope: %d heads", nh);
+    launch<false>(dtype, hd, p, grid, (hipStream_t)stream);
+    PGT_LAUNCH_CHECK();
+    return 0;
+}
+
+extern "C" size_t pgt_qk_norm_rope_backward_workspace_bytes(int32_t rows, int32_t hd) {
+    return rows <= 0 || hd <= 0 ? 0 : (size_t)rope_bwd_groups(rows) * 2 * hd * sizeof(float);
+}
+
+extern "C" int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const void* dk, int32_t lddk, const void* q,
+                                         int32_t ldq, const void* k, int32_t ldk, int32_t rows, int32_t heads, int32_t kv_heads,
+                                         int32_t hd, const int32_t* positions, const double* freqs, int32_t rot, int32_t interleaved,
+                                         const float* q_gain, const float* k_gain, float eps, void* dq_in, int32_t lddqi, void* dk_in,
+                                         int32_t lddki, float* dq_gain, float* dk_gain, void* workspace, size_t workspace_bytes,
+                                         pgt_stream_t stream) {
+    RopeP p = {};
+    p.q = q; p.k = k; p.dq = dq; p.dk = dk; p.qo = dq_in; p.ko = dk_in; p.pos = positions; p.freqs = freqs; p.qg = q_gain; p.kg = k_gain;
+    p.ldq = ldq; p.ldk = ldk; p.lddq = lddq; p.lddk = lddk; p.ldqo = lddqi; p.ldko = lddki;
+    p.rows = rows; p.heads = heads; p.kv_heads = kv_heads; p.rot = rot; p.inter = interleaved != 0; p.eps = eps;
+    if (const int rc = check(dtype, p, hd, true)) return rc;
+    const size_t need = pgt_qk_norm_rope_backward_workspace_bytes(rows, hd);
+    PGT_CHECK(workspace_bytes >= need && (need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0)),
+              "qk_norm_rope_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    p.part = (float*)workspace;
+    p.tok = rope_tok(rows);
+    hipStream_t st = (hipStream_t)stream;
+    const int groups = rows ? rope_bwd_groups(rows) : 0;
+    if (rows) launch<true>(dtype, hd, p, dim3(groups), st);
+    PGT_LAUNCH_CHECK();
+    if (dq_gain || dk_gain)
+        hipLaunchKernelGGL(qk_rope_gain_kernel, dim3(2 * hd / 16), dim3(256), 0, st, p.part, groups, hd, dq_gain, dk_gain);
+    PGT_LAUNCH_CHECK();
+    return 0;
+}

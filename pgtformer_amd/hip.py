@@ -69,6 +69,13 @@ SIGNATURES = {
     "pgt_layernorm_x3": [vp, i32, i32, i32, i32, vp, vp, f32, vp, i32, i32, vp, i32, i32, vp, i32, i32, vp],
     "pgt_window_attention_x3": [vp, i32, i32, vp, i32, i32, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, vp],
     "pgt_mha_x3": [vp, i32, i32, vp, i32, i32, vp, i32, i32, vp, i32, i32, i32, i32, i32, i32, f32, vp],
+    "pgt_qk_norm_rope": [i32, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp, i32, i32, vp, vp, f32, vp, i32, vp, i32, vp],
+    "pgt_qk_norm_rope_backward_workspace_bytes": [i32, i32],
+    "pgt_qk_norm_rope_backward": [i32, vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp, i32, i32, vp, vp, f32, vp, i32, vp, i32, vp, vp, vp, sz, vp],
+    "pgt_kv_append": [i32, vp, i32, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp],
+    "pgt_kv_read": [i32, vp, i32, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp],
+    "pgt_kv_attention_workspace_bytes": [i32, i32, i32, i32, i32, i32, i32],
+    "pgt_kv_attention": [i32, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, i32, f32, i32, i32, vp, i32, vp, sz, vp],
     "pgt_x3_split": [vp, i32, vp, i32, i32, i64, i32, vp],
     "pgt_x3_merge": [vp, i32, i32, vp, i32, i64, i32, vp],
     "pgt_x3_to_half": [vp, i32, i32, vp, i32, i64, i32, vp],
@@ -108,6 +115,7 @@ _RESTYPES = {"pgt_version": C.c_char_p, "pgt_last_error": C.c_char_p, "pgt_group
              "pgt_commit_loss_workspace_bytes": sz, "pgt_conv_gn_workspace_bytes": sz,
              "pgt_conv2d_workspace_bytes": sz, "pgt_packed_weight_bytes": sz, "pgt_attn_proj_mlp_sample_workspace_bytes": sz, "pgt_sampled_rownorm_workspace_bytes": sz,
              "pgt_frame_bias_workspace_bytes": sz, "pgt_program_workspace_bytes": sz, "pgt_program_info": C.c_char_p,
+             "pgt_qk_norm_rope_backward_workspace_bytes": sz, "pgt_kv_attention_workspace_bytes": sz,
              "pgt_program_destroy": None}
 
 

@@ -7,6 +7,7 @@ dtype torch.float32 selects the exact-f32 kernels, torch.bfloat16 / torch.float1
 significand bits; IEEE half: 11 - the decoder-side type of the default precision mode).
 """
 import ctypes as C
+import math
 
 import torch
 
@@ -1026,6 +1027,212 @@ def mha(q, k, v, B, L, heads, hd, scale, x3=None):
     return out
 
 
+# ---- attention over a cache of earlier tokens (include/pgt_hip.h has the definitions) ----------------------------------------
+def _need(ok, what, *args):
+    if not ok:
+        raise hip.PgtError(what % args if args else what)
+
+
+def _rows(t, cols, what):
+    """(row stride) of a (rows, cols) matrix of a supported type whose rows are 16-byte aligned"""
+    _need(t.dim() == 2 and t.shape[1] == cols, "%s: shape %s, (rows, %d) wanted", what, tuple(t.shape), cols)
+    if t.shape[0] <= 1:
+        _need(t.stride(1) == 1, "%s: elements of a row must be adjacent", what)
+        return cols
+    _need(t.stride(1) == 1 and t.stride(0) >= cols, "%s: strides %s (rows must not overlap, elements of a row be adjacent)", what, t.stride())
+    return t.stride(0)
+
+
+def _apart(outs, ins, what):
+    """outputs a caller passed: each may be one of the inputs itself, but must not overlap one in another way, nor another output"""
+    for i, o in enumerate(outs):
+        for x in list(ins) + list(outs[:i]):
+            if o.numel() == 0 or x.numel() == 0 or o.untyped_storage().data_ptr() != x.untyped_storage().data_ptr():
+                continue
+            es, ld = o.element_size(), (o.stride(0) if o.shape[0] > 1 else x.stride(0))
+            if any(x is t for t in ins) and o.data_ptr() == x.data_ptr() and (o.stride(0) == x.stride(0) or o.shape[0] <= 1) and o.shape == x.shape:
+                continue
+            end = lambda t: t.data_ptr() + es * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])      # noqa: E731
+            if end(o) <= x.data_ptr() or end(x) <= o.data_ptr():
+                continue
+            d = ((o.data_ptr() - x.data_ptr()) // es) % ld if ld else 0      # columns of one wider buffer?
+            _need(o.stride(0) == x.stride(0) and d >= x.shape[1] and d + o.shape[1] <= ld, "%s: an output overlaps another tensor", what)
+
+
+def _index(t, n, what):
+    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), "%s: %s %s, contiguous int32 (%d,) wanted", what,
+          t.dtype, tuple(t.shape), n)
+    return t
+
+
+def _f32_vec(t, n, what):
+    _need(t is None or (t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous()), "%s: contiguous float32 (%d,) wanted", what, n)
+    return t
+
+
+def rope_freqs(rot, base=10000.0, device="cuda"):
+    """Rotation frequencies of qk_norm_rope in revolutions per position, fp64 (rot / 2,): base ** (-2 i / rot) / (2 pi)."""
+    _need(rot >= 0 and rot % 8 == 0, "rope_freqs: %d rotated elements (a multiple of 8)", rot)
+    i = torch.arange(rot // 2, dtype=torch.float64)
+    return (float(base) ** (-2.0 * i / max(rot, 1)) / (2 * math.pi)).to(device)
+
+
+def _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, what):
+    rows = q.shape[0]
+    _need(q.dim() == 2 and heads > 0 and q.shape[1] % heads == 0, "%s: q %s over %d heads", what, tuple(q.shape), heads)
+    hd = q.shape[1] // heads
+    _need(k.shape[0] == rows and k.dtype == q.dtype, "%s: k %s %s, q %s %s", what, tuple(k.shape), k.dtype, tuple(q.shape), q.dtype)
+    rot = 0 if freqs is None else 2 * freqs.numel()
+    if rot:
+        _need(freqs.dtype == torch.float64 and freqs.is_contiguous(), "%s: freqs must be contiguous float64 (ops.rope_freqs)", what)
+        _need(positions is not None, "%s: a rotation needs positions", what)
+        _index(positions, rows, what + ": positions")
+    _f32_vec(q_gain, hd, what + ": q_gain")
+    _f32_vec(k_gain, hd, what + ": k_gain")
+    return rows, hd, rot
+
+
+def qk_norm_rope(q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_heads, eps=1e-6, interleaved=False, out=None):
+    """Per-head RMS norm (gains fp32 (hd,) or None) of q (rows, heads * hd) and k (rows, kv_heads * hd) and the rotation by their positions
+    (int32 (rows,); freqs: rope_freqs(rot), None = no rotation) in one pass -> (q_out, k_out).  out: the two outputs, which may be q and
+    k themselves.  interleaved: pairs (2i, 2i + 1) instead of (i, i + rot / 2)."""
+    rows, hd, rot = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, "qk_norm_rope")
+    qo, ko = out if out is not None else (torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype),
+                                          torch.empty((rows, kv_heads * hd), device=q.device, dtype=q.dtype))
+    _need(qo.dtype == q.dtype and ko.dtype == q.dtype and qo.shape[0] == rows and ko.shape[0] == rows, "qk_norm_rope: outputs of another type or length")
+    ld = (_rows(q, heads * hd, "qk_norm_rope: q"), _rows(k, kv_heads * hd, "qk_norm_rope: k"), _rows(qo, heads * hd, "qk_norm_rope: out"),
+          _rows(ko, kv_heads * hd, "qk_norm_rope: out"))
+    if out is not None:
+        _apart((qo, ko), (q, k), "qk_norm_rope")
+    with _Prof("qk_norm_rope", 9.0 * rows * (heads + kv_heads) * hd, _nb(q, k, qo, ko)):
+        hip.check(hip.lib().pgt_qk_norm_rope(_dt(q), _p(q), ld[0], _p(k), ld[1], rows, heads, kv_heads, hd, _p(positions), _p(freqs), rot,
+                                             int(interleaved), _p(q_gain), _p(k_gain), eps, _p(qo), ld[2], _p(ko), ld[3], _stream()),
+                  "pgt_qk_norm_rope")
+    return qo, ko
+
+
+def qk_norm_rope_backward(dq, dk, q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_heads, eps=1e-6, interleaved=False, out=None):
+    """Gradients of qk_norm_rope: (dq, dk) of its outputs, its inputs q, k -> (gradient of q, of k, of q_gain, of k_gain; the gains' fp32
+    (hd,)).  out: where the first two go (dq, dk themselves are allowed)."""
+    what = "qk_norm_rope_backward"
+    rows, hd, rot = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, what)
+    qo, ko = out if out is not None else (torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype),
+                                          torch.empty((rows, kv_heads * hd), device=q.device, dtype=q.dtype))
+    for t in (dq, dk, qo, ko):
+        _need(t.dtype == q.dtype and t.shape[0] == rows, "%s: gradients of another type or length", what)
+    ld = [_rows(t, n * hd, what) for t, n in ((dq, heads), (dk, kv_heads), (q, heads), (k, kv_heads), (qo, heads), (ko, kv_heads))]
+    if out is not None:
+        _apart((qo, ko), (dq, dk, q, k), what)
+    gains = torch.empty((2, hd), device=q.device, dtype=torch.float32)
+    L = hip.lib()
+    nbytes = L.pgt_qk_norm_rope_backward_workspace_bytes(rows, hd)
+    ws = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32)
+    with _Prof("qk_norm_rope_backward", 17.0 * rows * (heads + kv_heads) * hd, _nb(dq, dk, q, k, qo, ko)):
+        hip.check(L.pgt_qk_norm_rope_backward(_dt(q), _p(dq), ld[0], _p(dk), ld[1], _p(q), ld[2], _p(k), ld[3], rows, heads, kv_heads, hd,
+                                              _p(positions), _p(freqs), rot, int(interleaved), _p(q_gain), _p(k_gain), eps, _p(qo), ld[4],
+                                              _p(ko), ld[5], _p(gains[0]), _p(gains[1]), _p(ws), nbytes, _stream()), "pgt_qk_norm_rope_backward")
+    return qo, ko, gains[0], gains[1]
+
+
+class KvCache:
+    """Paged 8-bit key / value cache: codes uint8 k_pages (pages, kv_heads, hd / 16, page, 16), v_pages (pages, kv_heads, page / 16, hd, 16), fp32
+    power-of-two scales (pages, kv_heads).  Which pages a sequence owns is the caller's: an int32 table (B, width)."""
+    __slots__ = ("k_pages", "v_pages", "k_scale", "v_scale", "pages", "page", "kv_heads", "hd")
+
+    def __init__(self, k_pages, v_pages, k_scale, v_scale):
+        _need(k_pages.dim() == 5 and k_pages.shape[4] == 16, "KvCache: k_pages %s, (pages, kv_heads, hd / 16, page, 16) wanted", tuple(k_pages.shape))
+        n, kv, c, page, _ = k_pages.shape
+        _need(v_pages.shape == (n, kv, page // 16, 16 * c, 16), "KvCache: v_pages %s do not belong to k_pages %s", tuple(v_pages.shape),
+              tuple(k_pages.shape))
+        _need(k_scale.shape == (n, kv) and v_scale.shape == (n, kv), "KvCache: one scale per page and kv head wanted")
+        for t, want in ((k_pages, torch.uint8), (v_pages, torch.uint8), (k_scale, torch.float32), (v_scale, torch.float32)):
+            _need(t.dtype == want and t.is_contiguous(), "KvCache: contiguous uint8 pages and float32 scales wanted")
+        self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
+        self.pages, self.page, self.kv_heads, self.hd = n, page, kv, 16 * c
+
+    @classmethod
+    def alloc(cls, pages, kv_heads, page, hd, device="cuda"):
+        _need(pages > 0 and kv_heads > 0 and page in (16, 32, 64, 128) and hd in (64, 128),
+              "KvCache: pages=%d kv_heads=%d page=%d (16, 32, 64, 128) head_dim=%d (64, 128)", pages, kv_heads, page, hd)
+        z = lambda *shape, dt=torch.uint8: torch.zeros(shape, dtype=dt, device=device)      # noqa: E731
+        return cls(z(pages, kv_heads, hd // 16, page, 16), z(pages, kv_heads, page // 16, hd, 16),
+                   z(pages, kv_heads, dt=torch.float32), z(pages, kv_heads, dt=torch.float32))
+
+    def _c(self):
+        """the cache's arguments of a launch"""
+        return (_p(self.k_pages), _p(self.v_pages), _p(self.k_scale), _p(self.v_scale), self.pages, self.page, self.kv_heads, self.hd)
+
+
+def _seq_args(table, lens, cu, rows, most, what):
+    """(B, width, row stride of the table, tokens per sequence at most) of ragged (cu) or equal sequences over packed rows"""
+    _need(table.dtype == torch.int32 and table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1) and
+          (table.shape[0] <= 1 or table.stride(0) >= table.shape[1]), "%s: int32 table (B, width) wanted, got %s %s", what, table.dtype, tuple(table.shape))
+    B, width = table.shape
+    _index(lens, B, what + ": lens")
+    if cu is None:
+        _need(B > 0 and rows % B == 0, "%s: %d rows over %d sequences (pass cu)", what, rows, B)
+        _need(most is None or most == rows // B, "%s: %d tokens per sequence without cu, not %s", what, rows // max(B, 1), most)
+        most = rows // B
+    else:
+        _index(cu, B + 1, what + ": cu")
+        most = rows if most is None else int(most)
+        _need(0 <= most <= rows, "%s: at most %d tokens per sequence of %d rows", what, most, rows)
+    return B, width, table.stride(0) if B > 1 else width, most
+
+
+def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
+    """Quantise the rows k, v (rows, kv_heads * hd) into the cache: sequence b's (rows cu[b] .. cu[b + 1] - 1; cu None: rows / B each) become
+    its tokens lens[b] .. .  lens: int32 (B,), tokens BEFORE the call (the caller counts on).  max_new: most rows of one sequence - the
+    launch covers so many (default with cu: all rows, correct but a larger launch)."""
+    rows = k.shape[0]
+    B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_append")
+    n = cache.kv_heads * cache.hd
+    _need(k.dtype == v.dtype and v.shape[0] == rows, "kv_append: k %s %s, v %s %s", tuple(k.shape), k.dtype, tuple(v.shape), v.dtype)
+    ldk, ldv = _rows(k, n, "kv_append: k"), _rows(v, n, "kv_append: v")
+    with _Prof("kv_append", 8.0 * rows * n, _nb(k, v) + 2 * rows * n):
+        hip.check(hip.lib().pgt_kv_append(_dt(k), _p(k), ldk, _p(v), ldv, *cache._c(), _p(table), ldt, width, _p(lens), _p(cu), B, rows, most,
+                                          _stream()), "pgt_kv_append")
+
+
+def kv_read(cache, table, start, rows, dtype, cu=None, *, max_rows=None, out=None):
+    """The cache's values as (k, v), each (rows, kv_heads * hd) of dtype: the rows of sequence b (cu as in kv_append) are its tokens start[b] .. .
+    Rows that no sequence owns stay as they are in `out`; tokens that no page holds are zeros."""
+    n = cache.kv_heads * cache.hd
+    ko, vo = out if out is not None else [torch.empty((rows, n), device=cache.k_pages.device, dtype=dtype) for _ in range(2)]
+    _need(ko.dtype == dtype and vo.dtype == dtype and ko.shape[0] == rows and vo.shape[0] == rows, "kv_read: outputs of another type or length")
+    B, width, ldt, most = _seq_args(table, start, cu, rows, max_rows, "kv_read")
+    ldk, ldv = _rows(ko, n, "kv_read: out"), _rows(vo, n, "kv_read: out")
+    if out is not None:
+        _apart((ko, vo), (), "kv_read")
+    with _Prof("kv_read", 2.0 * rows * n, _nb(ko, vo) + 2 * rows * n):
+        hip.check(hip.lib().pgt_kv_read(_dt(ko), _p(ko), ldk, _p(vo), ldv, *cache._c(), _p(table), ldt, width, _p(start), _p(cu), B, rows, most,
+                                        _stream()), "pgt_kv_read")
+    return ko, vo
+
+
+def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=1, window=0, scale=None, out=None):
+    """softmax(scale * q K^T) V over the cache: q (rows, heads * hd), row i of the n rows of sequence b at position lens[b] - n + i, lens[b]
+    (int32) the tokens the cache holds INCLUDING these rows'.  causal: 0 = every token, c = those up to the end of the block of c tokens that
+    the position lies in (1 = token by token, tokens per frame = whole frames); window > 0: only the last `window` of these.  A row that
+    sees nothing is zero; rows that no sequence owns stay as they are in `out`.  scale: default hd ** -0.5."""
+    rows, hd = q.shape[0], cache.hd
+    B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_attention")
+    if out is None:
+        out = torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype)
+    _need(out.dtype == q.dtype and out.shape[0] == rows, "kv_attention: output of another type or length")
+    ldq, ldo = _rows(q, heads * hd, "kv_attention: q"), _rows(out, heads * hd, "kv_attention: out")
+    _apart((out,), (q,), "kv_attention")
+    L = hip.lib()
+    nbytes = L.pgt_kv_attention_workspace_bytes(B, most, heads, cache.kv_heads, hd, width, cache.page)
+    ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
+    tokens = width * cache.page
+    with _Prof("kv_attention", 4.0 * rows * tokens * heads * hd, _nb(q, out) + 2 * B * tokens * cache.kv_heads * hd):
+        hip.check(L.pgt_kv_attention(_dt(q), _p(q), ldq, *cache._c(), _p(table), ldt, width, _p(lens), _p(cu), B, rows, most, heads,
+                                     hd ** -0.5 if scale is None else scale, causal, window, _p(out), ldo, _p(ws), nbytes, _stream()),
+                  "pgt_kv_attention")
+    return out
+
+
 def argmax_rows(logits):
     rows, k = logits.shape
     assert logits.dtype == torch.float32
@@ -1305,7 +1512,7 @@ def _range_wrap(fn):
 
 
 for _n in ("conv2d", "affine_act", "layernorm", "ln_linear", "ln_mlp", "attn_proj_mlp", "window_attention", "window_attention3d", "mha",
-           "to_x3", "x3_to_half"):
+           "qk_norm_rope", "kv_read", "kv_attention", "to_x3", "x3_to_half"):
     globals()[_n] = _range_wrap(globals()[_n])
 
 
