@@ -6,6 +6,7 @@ and the pixel/row stride may exceed C (channel slices of a wider buffer are vali
 dtype torch.float32 selects the exact-f32 kernels, torch.bfloat16 / torch.float16 the 16-bit MFMA kernels (bf16: 8
 significand bits; IEEE half: 11 - the decoder-side type of the default precision mode).
 """
+import contextlib
 import ctypes as C
 import math
 
@@ -1034,13 +1035,35 @@ def _need(ok, what, *args):
 
 
 def _rows(t, cols, what):
-    """(row stride) of a (rows, cols) matrix of a supported type whose rows are 16-byte aligned"""
-    _need(t.dim() == 2 and t.shape[1] == cols, "%s: shape %s, (rows, %d) wanted", what, tuple(t.shape), cols)
-    if t.shape[0] <= 1:
-        _need(t.stride(1) == 1, "%s: elements of a row must be adjacent", what)
-        return cols
-    _need(t.stride(1) == 1 and t.stride(0) >= cols, "%s: strides %s (rows must not overlap, elements of a row be adjacent)", what, t.stride())
-    return t.stride(0)
+    """row stride of a (rows, cols) matrix whose rows do not overlap"""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 2 and shape[1] == cols and stride[1] == 1:
+        if shape[0] <= 1:
+            return cols
+        if stride[0] >= cols:
+            return stride[0]
+    raise hip.PgtError("%s: shape %s, strides %s; (rows, %d) wanted, elements of a row adjacent, rows not overlapping" % (
+        what, tuple(shape), stride, cols))
+
+
+def _pointers(*ts):
+    """(pointer of every tensor, ..., stream): the first tensor names the device, which has to be the current one; all others live there.
+    What _p and _stream do, with one look at the current device per launch (a serving step is made of such small launches)."""
+    if hip.TRACE is not None or hip.TRACE_TENSORS is not None:
+        return [_p(t) for t in ts] + [_stream()]
+    dev = ts[0].get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        _dev(ts[0])
+    out = []
+    for t in ts:
+        if t is None:
+            out.append(None)
+        elif t.get_device() != dev:
+            raise hip.PgtError("pgtformer_amd ops run on one GPU: tensors on %s and %s" % (ts[0].device, _dev(t).device))
+        else:
+            out.append(t.data_ptr())
+    out.append(torch._C._cuda_getCurrentRawStream(dev))
+    return out
 
 
 def _apart(outs, ins, what):
@@ -1060,14 +1083,21 @@ def _apart(outs, ins, what):
 
 
 def _index(t, n, what):
-    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and t.is_contiguous(), "%s: %s %s, contiguous int32 (%d,) wanted", what,
-          t.dtype, tuple(t.shape), n)
-    return t
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
+        raise hip.PgtError("%s: %s %s, contiguous int32 (%d,) wanted" % (what, t.dtype, tuple(t.shape), n))
 
 
 def _f32_vec(t, n, what):
-    _need(t is None or (t.dtype == torch.float32 and t.shape == (n,) and t.is_contiguous()), "%s: contiguous float32 (%d,) wanted", what, n)
-    return t
+    if t is not None and (t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous()):
+        raise hip.PgtError("%s: contiguous float32 (%d,) wanted" % (what, n))
+
+
+def _profiled(kernel, flops, *tensors, more=0.0):
+    """_Prof of a launch, its bytes counted only if somebody records"""
+    return _NOT_PROFILED if PROFILE is None else _Prof(kernel, flops, _nb(*tensors) + more)
+
+
+_NOT_PROFILED = contextlib.nullcontext()
 
 
 def rope_freqs(rot, base=10000.0, device="cuda"):
@@ -1077,37 +1107,41 @@ def rope_freqs(rot, base=10000.0, device="cuda"):
     return (float(base) ** (-2.0 * i / max(rot, 1)) / (2 * math.pi)).to(device)
 
 
-def _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, what):
-    rows = q.shape[0]
-    _need(q.dim() == 2 and heads > 0 and q.shape[1] % heads == 0, "%s: q %s over %d heads", what, tuple(q.shape), heads)
-    hd = q.shape[1] // heads
-    _need(k.shape[0] == rows and k.dtype == q.dtype, "%s: k %s %s, q %s %s", what, tuple(k.shape), k.dtype, tuple(q.shape), q.dtype)
+def _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, what):
+    """(rows, hd, rot, outputs, row strides of q, k and the outputs)"""
+    rows, cols = q.shape
+    if heads <= 0 or cols % heads:
+        raise hip.PgtError("%s: q %s over %d heads" % (what, tuple(q.shape), heads))
+    hd = cols // heads
+    if k.shape[0] != rows or k.dtype is not q.dtype:
+        raise hip.PgtError("%s: k %s %s, q %s %s" % (what, tuple(k.shape), k.dtype, tuple(q.shape), q.dtype))
+    ldq, ldk = _rows(q, cols, what + ": q"), _rows(k, kv_heads * hd, what + ": k")
     rot = 0 if freqs is None else 2 * freqs.numel()
     if rot:
-        _need(freqs.dtype == torch.float64 and freqs.is_contiguous(), "%s: freqs must be contiguous float64 (ops.rope_freqs)", what)
+        _need(freqs.dtype is torch.float64 and freqs.is_contiguous(), "%s: freqs must be contiguous float64 (ops.rope_freqs)", what)
         _need(positions is not None, "%s: a rotation needs positions", what)
         _index(positions, rows, what + ": positions")
     _f32_vec(q_gain, hd, what + ": q_gain")
     _f32_vec(k_gain, hd, what + ": k_gain")
-    return rows, hd, rot
+    if out is None:
+        qo, ko = (torch.empty((rows, n * hd), device=q.device, dtype=q.dtype) for n in (heads, kv_heads))
+        return rows, hd, rot, qo, ko, ldq, ldk, cols, kv_heads * hd
+    qo, ko = out
+    _need(qo.dtype is q.dtype and ko.dtype is q.dtype and qo.shape[0] == rows and ko.shape[0] == rows, "%s: outputs of another type or length", what)
+    return rows, hd, rot, qo, ko, ldq, ldk, _rows(qo, cols, what + ": out"), _rows(ko, kv_heads * hd, what + ": out")
 
 
 def qk_norm_rope(q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_heads, eps=1e-6, interleaved=False, out=None):
     """Per-head RMS norm (gains fp32 (hd,) or None) of q (rows, heads * hd) and k (rows, kv_heads * hd) and the rotation by their positions
     (int32 (rows,); freqs: rope_freqs(rot), None = no rotation) in one pass -> (q_out, k_out).  out: the two outputs, which may be q and
     k themselves.  interleaved: pairs (2i, 2i + 1) instead of (i, i + rot / 2)."""
-    rows, hd, rot = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, "qk_norm_rope")
-    qo, ko = out if out is not None else (torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype),
-                                          torch.empty((rows, kv_heads * hd), device=q.device, dtype=q.dtype))
-    _need(qo.dtype == q.dtype and ko.dtype == q.dtype and qo.shape[0] == rows and ko.shape[0] == rows, "qk_norm_rope: outputs of another type or length")
-    ld = (_rows(q, heads * hd, "qk_norm_rope: q"), _rows(k, kv_heads * hd, "qk_norm_rope: k"), _rows(qo, heads * hd, "qk_norm_rope: out"),
-          _rows(ko, kv_heads * hd, "qk_norm_rope: out"))
+    rows, hd, rot, qo, ko, ldq, ldk, ldqo, ldko = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, "qk_norm_rope")
     if out is not None:
         _apart((qo, ko), (q, k), "qk_norm_rope")
-    with _Prof("qk_norm_rope", 9.0 * rows * (heads + kv_heads) * hd, _nb(q, k, qo, ko)):
-        hip.check(hip.lib().pgt_qk_norm_rope(_dt(q), _p(q), ld[0], _p(k), ld[1], rows, heads, kv_heads, hd, _p(positions), _p(freqs), rot,
-                                             int(interleaved), _p(q_gain), _p(k_gain), eps, _p(qo), ld[2], _p(ko), ld[3], _stream()),
-                  "pgt_qk_norm_rope")
+    pq, pk, pp, pf, pqg, pkg, pqo, pko, st = _pointers(q, k, positions, freqs, q_gain, k_gain, qo, ko)
+    with _profiled("qk_norm_rope", 9.0 * rows * (heads + kv_heads) * hd, q, k, qo, ko):
+        hip.check(hip.lib().pgt_qk_norm_rope(_dt(q), pq, ldq, pk, ldk, rows, heads, kv_heads, hd, pp, pf, rot, int(interleaved), pqg, pkg, eps,
+                                             pqo, ldqo, pko, ldko, st), "pgt_qk_norm_rope")
     return qo, ko
 
 
@@ -1115,23 +1149,22 @@ def qk_norm_rope_backward(dq, dk, q, k, positions, freqs, q_gain=None, k_gain=No
     """Gradients of qk_norm_rope: (dq, dk) of its outputs, its inputs q, k -> (gradient of q, of k, of q_gain, of k_gain; the gains' fp32
     (hd,)).  out: where the first two go (dq, dk themselves are allowed)."""
     what = "qk_norm_rope_backward"
-    rows, hd, rot = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, what)
-    qo, ko = out if out is not None else (torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype),
-                                          torch.empty((rows, kv_heads * hd), device=q.device, dtype=q.dtype))
-    for t in (dq, dk, qo, ko):
-        _need(t.dtype == q.dtype and t.shape[0] == rows, "%s: gradients of another type or length", what)
-    ld = [_rows(t, n * hd, what) for t, n in ((dq, heads), (dk, kv_heads), (q, heads), (k, kv_heads), (qo, heads), (ko, kv_heads))]
+    rows, hd, rot, qo, ko, ldq, ldk, ldqo, ldko = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, what)
+    _need(dq.dtype is q.dtype and dk.dtype is q.dtype and dq.shape[0] == rows and dk.shape[0] == rows, "%s: gradients of another type or length", what)
+    lddq, lddk = _rows(dq, heads * hd, what + ": dq"), _rows(dk, kv_heads * hd, what + ": dk")
     if out is not None:
         _apart((qo, ko), (dq, dk, q, k), what)
     gains = torch.empty((2, hd), device=q.device, dtype=torch.float32)
     L = hip.lib()
     nbytes = L.pgt_qk_norm_rope_backward_workspace_bytes(rows, hd)
     ws = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32)
-    with _Prof("qk_norm_rope_backward", 17.0 * rows * (heads + kv_heads) * hd, _nb(dq, dk, q, k, qo, ko)):
-        hip.check(L.pgt_qk_norm_rope_backward(_dt(q), _p(dq), ld[0], _p(dk), ld[1], _p(q), ld[2], _p(k), ld[3], rows, heads, kv_heads, hd,
-                                              _p(positions), _p(freqs), rot, int(interleaved), _p(q_gain), _p(k_gain), eps, _p(qo), ld[4],
-                                              _p(ko), ld[5], _p(gains[0]), _p(gains[1]), _p(ws), nbytes, _stream()), "pgt_qk_norm_rope_backward")
-    return qo, ko, gains[0], gains[1]
+    gq, gk = gains.unbind(0)
+    pdq, pdk, pq, pk, pp, pf, pqg, pkg, pqo, pko, pgq, pgk, pws, st = _pointers(dq, dk, q, k, positions, freqs, q_gain, k_gain, qo, ko, gq, gk, ws)
+    with _profiled("qk_norm_rope_backward", 17.0 * rows * (heads + kv_heads) * hd, dq, dk, q, k, qo, ko):
+        hip.check(L.pgt_qk_norm_rope_backward(_dt(q), pdq, lddq, pdk, lddk, pq, ldq, pk, ldk, rows, heads, kv_heads, hd, pp, pf, rot,
+                                              int(interleaved), pqg, pkg, eps, pqo, ldqo, pko, ldko, pgq, pgk, pws, nbytes, st),
+                  "pgt_qk_norm_rope_backward")
+    return qo, ko, gq, gk
 
 
 class KvCache:
@@ -1158,26 +1191,24 @@ class KvCache:
         return cls(z(pages, kv_heads, hd // 16, page, 16), z(pages, kv_heads, page // 16, hd, 16),
                    z(pages, kv_heads, dt=torch.float32), z(pages, kv_heads, dt=torch.float32))
 
-    def _c(self):
-        """the cache's arguments of a launch"""
-        return (_p(self.k_pages), _p(self.v_pages), _p(self.k_scale), _p(self.v_scale), self.pages, self.page, self.kv_heads, self.hd)
-
 
 def _seq_args(table, lens, cu, rows, most, what):
     """(B, width, row stride of the table, tokens per sequence at most) of ragged (cu) or equal sequences over packed rows"""
-    _need(table.dtype == torch.int32 and table.dim() == 2 and (table.shape[1] <= 1 or table.stride(1) == 1) and
-          (table.shape[0] <= 1 or table.stride(0) >= table.shape[1]), "%s: int32 table (B, width) wanted, got %s %s", what, table.dtype, tuple(table.shape))
-    B, width = table.shape
+    shape, stride = table.shape, table.stride()
+    if len(shape) != 2 or table.dtype is not torch.int32 or (shape[1] > 1 and stride[1] != 1) or (shape[0] > 1 and stride[0] < shape[1]):
+        raise hip.PgtError("%s: int32 table (B, width) wanted, got %s %s" % (what, table.dtype, tuple(shape)))
+    B, width = shape
     _index(lens, B, what + ": lens")
     if cu is None:
-        _need(B > 0 and rows % B == 0, "%s: %d rows over %d sequences (pass cu)", what, rows, B)
-        _need(most is None or most == rows // B, "%s: %d tokens per sequence without cu, not %s", what, rows // max(B, 1), most)
+        if B <= 0 or rows % B or (most is not None and most != rows // B):
+            raise hip.PgtError("%s: %d rows over %d sequences, %s each (ragged: pass cu)" % (what, rows, B, most))
         most = rows // B
     else:
         _index(cu, B + 1, what + ": cu")
         most = rows if most is None else int(most)
-        _need(0 <= most <= rows, "%s: at most %d tokens per sequence of %d rows", what, most, rows)
-    return B, width, table.stride(0) if B > 1 else width, most
+        if not 0 <= most <= rows:
+            raise hip.PgtError("%s: at most %d tokens per sequence of %d rows" % (what, most, rows))
+    return B, width, stride[0] if B > 1 else width, most
 
 
 def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
@@ -1189,24 +1220,29 @@ def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
     n = cache.kv_heads * cache.hd
     _need(k.dtype == v.dtype and v.shape[0] == rows, "kv_append: k %s %s, v %s %s", tuple(k.shape), k.dtype, tuple(v.shape), v.dtype)
     ldk, ldv = _rows(k, n, "kv_append: k"), _rows(v, n, "kv_append: v")
-    with _Prof("kv_append", 8.0 * rows * n, _nb(k, v) + 2 * rows * n):
-        hip.check(hip.lib().pgt_kv_append(_dt(k), _p(k), ldk, _p(v), ldv, *cache._c(), _p(table), ldt, width, _p(lens), _p(cu), B, rows, most,
-                                          _stream()), "pgt_kv_append")
+    pk, pv, kp, vp, ks, vs, pt, pl, pc, st = _pointers(k, v, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, lens, cu)
+    with _profiled("kv_append", 8.0 * rows * n, k, v, more=2 * rows * n):
+        hip.check(hip.lib().pgt_kv_append(_dt(k), pk, ldk, pv, ldv, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, cache.hd, pt, ldt,
+                                          width, pl, pc, B, rows, most, st), "pgt_kv_append")
 
 
 def kv_read(cache, table, start, rows, dtype, cu=None, *, max_rows=None, out=None):
     """The cache's values as (k, v), each (rows, kv_heads * hd) of dtype: the rows of sequence b (cu as in kv_append) are its tokens start[b] .. .
     Rows that no sequence owns stay as they are in `out`; tokens that no page holds are zeros."""
     n = cache.kv_heads * cache.hd
-    ko, vo = out if out is not None else [torch.empty((rows, n), device=cache.k_pages.device, dtype=dtype) for _ in range(2)]
-    _need(ko.dtype == dtype and vo.dtype == dtype and ko.shape[0] == rows and vo.shape[0] == rows, "kv_read: outputs of another type or length")
     B, width, ldt, most = _seq_args(table, start, cu, rows, max_rows, "kv_read")
-    ldk, ldv = _rows(ko, n, "kv_read: out"), _rows(vo, n, "kv_read: out")
-    if out is not None:
+    if out is None:
+        ko, vo = (torch.empty((rows, n), device=cache.k_pages.device, dtype=dtype) for _ in range(2))
+        ldk = ldv = n
+    else:
+        ko, vo = out
+        _need(ko.dtype is dtype and vo.dtype is dtype and ko.shape[0] == rows and vo.shape[0] == rows, "kv_read: outputs of another type or length")
+        ldk, ldv = _rows(ko, n, "kv_read: out"), _rows(vo, n, "kv_read: out")
         _apart((ko, vo), (), "kv_read")
-    with _Prof("kv_read", 2.0 * rows * n, _nb(ko, vo) + 2 * rows * n):
-        hip.check(hip.lib().pgt_kv_read(_dt(ko), _p(ko), ldk, _p(vo), ldv, *cache._c(), _p(table), ldt, width, _p(start), _p(cu), B, rows, most,
-                                        _stream()), "pgt_kv_read")
+    pk, pv, kp, vp, ks, vs, pt, pl, pc, st = _pointers(ko, vo, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, start, cu)
+    with _profiled("kv_read", 2.0 * rows * n, ko, vo, more=2 * rows * n):
+        hip.check(hip.lib().pgt_kv_read(_dt(ko), pk, ldk, pv, ldv, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, cache.hd, pt, ldt,
+                                        width, pl, pc, B, rows, most, st), "pgt_kv_read")
     return ko, vo
 
 
@@ -1217,18 +1253,21 @@ def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=
     sees nothing is zero; rows that no sequence owns stay as they are in `out`.  scale: default hd ** -0.5."""
     rows, hd = q.shape[0], cache.hd
     B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_attention")
+    ldq = _rows(q, heads * hd, "kv_attention: q")
     if out is None:
-        out = torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype)
-    _need(out.dtype == q.dtype and out.shape[0] == rows, "kv_attention: output of another type or length")
-    ldq, ldo = _rows(q, heads * hd, "kv_attention: q"), _rows(out, heads * hd, "kv_attention: out")
-    _apart((out,), (q,), "kv_attention")
+        out, ldo = torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype), heads * hd
+    else:
+        _need(out.dtype == q.dtype and out.shape[0] == rows, "kv_attention: output of another type or length")
+        ldo = _rows(out, heads * hd, "kv_attention: out")
+        _apart((out,), (q,), "kv_attention")
     L = hip.lib()
     nbytes = L.pgt_kv_attention_workspace_bytes(B, most, heads, cache.kv_heads, hd, width, cache.page)
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     tokens = width * cache.page
-    with _Prof("kv_attention", 4.0 * rows * tokens * heads * hd, _nb(q, out) + 2 * B * tokens * cache.kv_heads * hd):
-        hip.check(L.pgt_kv_attention(_dt(q), _p(q), ldq, *cache._c(), _p(table), ldt, width, _p(lens), _p(cu), B, rows, most, heads,
-                                     hd ** -0.5 if scale is None else scale, causal, window, _p(out), ldo, _p(ws), nbytes, _stream()),
+    pq, kp, vp, ks, vs, pt, pl, pc, po, pw, st = _pointers(q, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, lens, cu, out, ws)
+    with _profiled("kv_attention", 4.0 * rows * tokens * heads * hd, q, out, more=2 * B * tokens * cache.kv_heads * hd):
+        hip.check(L.pgt_kv_attention(_dt(q), pq, ldq, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, hd, pt, ldt, width, pl, pc, B,
+                                     rows, most, heads, hd ** -0.5 if scale is None else scale, causal, window, po, ldo, pw, nbytes, st),
                   "pgt_kv_attention")
     return out
 
