@@ -51,7 +51,7 @@ struct AttnP {
     const int32_t *table, *lens, *cu;
     float *po, *pml;                  // partial results of the splits: (slot, split, hd), (slot, split, {m, l})
     int64_t ldq, ldo;
-    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, nct, nsplit, causal, window;
+    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, nct, nsplit, chunk, causal, window;      // chunk: tiles of 64 tokens per split
     float c;                          // scale * log2 e
 };
 
@@ -85,6 +85,7 @@ __device__ __forceinline__ void sees(const AttnP& p, int len, int pos, int& lo, 
     lo = min(lo, hi);
 }
 
+constexpr int MAX_SPLIT = 256;
 constexpr int NW = 4;      // waves per workgroup, each with its own share of the tokens
 
 template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn_kernel(const AttnP p) {
@@ -112,9 +113,8 @@ template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn
     sees(p, s.len, s.len - s.n + ct * 16 / p.group, lo_a, hi_a);
     sees(p, s.len, s.len - s.n + min(ct * 16 + 15, cols - 1) / p.group, lo_z, hi_z);
     const int t_first = lo_a >> 6, t_end = (hi_z + 63) >> 6;
-    const int tiles = max(t_end - t_first, 0);
-    const int per = (tiles + p.nsplit * NW - 1) / (p.nsplit * NW);
-    const int tb = min(t_first + (split * NW + wave) * per, t_end), te = min(tb + per, t_end);
+    const int t0 = t_first + split * p.chunk, te = min(t0 + p.chunk, t_end);
+    if (p.nsplit > 1 && t0 >= te) return;      // the join does not look at it
 
     // Q^T operand: k-step 2 s + h covers dims 64 s + 16 g + 8 h .. + 7 of lane group g - the order of the K loads
     uint4 qf[QP][KS];
@@ -151,7 +151,7 @@ template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn
     const size_t page_bytes = (size_t)page * HD, head_off = (size_t)hk * page_bytes, stride = (size_t)p.kv * page_bytes;
     const int32_t* tab = p.table + (size_t)b * p.ldt;
 
-    for (int t = tb; t < te; ++t) {
+    for (int t = t0 + wave; t < te; t += NW) {
         // the page of the block whose K rows this lane loads, and of its own block (V, scales)
         const int tk = t * 64 + 16 * kblk, tv = t * 64 + 16 * g;
         const int ik = tk >> p.pshift, iv = tv >> p.pshift;
@@ -331,47 +331,78 @@ template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn
     }
 }
 
-// out = sum of the splits' results against their common reference; one workgroup of HD threads per (sequence, token, head)
-template <typename T, int HD> __global__ __launch_bounds__(HD) void kv_attn_join_kernel(const AttnP p) {
+// out = the splits' results against their common reference.  One workgroup per (sequence, token, head): HD / 4 threads hold the row, the
+// rest of the 256 take other splits, four loads in flight each.
+template <typename T, int HD> __global__ __launch_bounds__(256) void kv_attn_join_kernel(const AttnP p) {
+    constexpr int LP = HD / 4, NS = 256 / LP;
+    __shared__ float2 ml[MAX_SPLIT];
+    __shared__ f32x4 so[NS][LP];
+    __shared__ float sm[4], sl[4];
     int id = blockIdx.x;
     const int head = id % p.heads; id /= p.heads;
-    const int qi = id % p.max_new, b = id / p.max_new;
+    const int qi = id % p.max_new, b = id / p.max_new, tid = threadIdx.x;
     const Seq s = seq_of(p, b);
     if (qi >= s.n) return;
+    // the splits that hold tokens of this query's column tile
+    const int col0 = (qi * p.group + head % p.group) & ~15, colz = min(col0 + 15, s.n * p.group - 1);
+    int lo_a, hi_z, dummy;
+    sees(p, s.len, s.len - s.n + col0 / p.group, lo_a, dummy);
+    sees(p, s.len, s.len - s.n + colz / p.group, dummy, hi_z);
+    const int tiles = ((hi_z + 63) >> 6) - (lo_a >> 6), n = tiles > 0 ? (tiles + p.chunk - 1) / p.chunk : 0;
     const size_t slot = ((size_t)b * p.max_new + qi) * p.heads + head;
-    const float2* ml = reinterpret_cast<const float2*>(p.pml) + slot * p.nsplit;
-    const float* po = p.po + slot * p.nsplit * HD + threadIdx.x;
-    float m = -INFINITY;
-    for (int i = 0; i < p.nsplit; ++i) m = fmaxf(m, ml[i].x);
-    float l = 0.f, o = 0.f;
-    for (int i = 0; i < p.nsplit; ++i) {
-        const float2 w = ml[i];
-        const float al = w.x == -INFINITY ? 1.f : exp2_(w.x - m);      // a split that saw nothing holds zeros (or NaN)
-        l += w.y * al;
-        o += po[(size_t)i * HD] * al;
-    }
-    o = l == 0.f ? 0.f : o / l;
-    if constexpr (__is_same(T, half_t)) o = clamp_half(o);
-    T* op = (T*)p.out + (s.r0 + qi) * p.ldo + head * HD + threadIdx.x;
-    if constexpr (__is_same(T, half_t)) op->v = (_Float16)o;
-    else stf(op, o);
+    const float2 w = tid < n ? reinterpret_cast<const float2*>(p.pml)[slot * p.nsplit + tid] : make_float2(-INFINITY, 0.f);
+    float m = wave_max(w.x);
+    if ((tid & 63) == 0) sm[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    const float al = w.x == -INFINITY ? 1.f : exp2_(w.x - m);      // a split that saw nothing holds zeros (or NaN)
+    if (tid < n) ml[tid] = make_float2(al, w.y * al);
+    const float lw = wave_sum(tid < n ? w.y * al : 0.f);
+    if ((tid & 63) == 0) sl[tid >> 6] = lw;
+    __syncthreads();
+    const float l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    const int c = tid % LP, k = tid / LP;
+    const f32x4* po = reinterpret_cast<const f32x4*>(p.po + slot * p.nsplit * HD) + c;
+    f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = k; i < n; i += NS) o += po[(size_t)i * LP] * ml[i].x;
+    so[k][c] = o;
+    __syncthreads();
+    if (k) return;
+#pragma unroll
+    for (int i = 1; i < NS; ++i) o += so[i][c];
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = l == 0.f ? 0.f : o[e] / l;
+    store4((T*)p.out + (s.r0 + qi) * p.ldo + head * HD + 4 * c, f);
 }
 
-// Splits of the tokens: enough workgroups to fill the chip, but a wave keeps at least one 64-token tile
-int splits(int B, int max_new, int kv, int group, int width, int pshift) {
+// Splits of the tokens, and tiles of 64 tokens in each: about 2048 workgroups of equal work (ragged lengths: what is past a sequence's
+// end exits at once), at least a tile per wave, and one split where the whole length is short
+struct Split {
+    int n, chunk;
+};
+Split splits(int B, int max_new, int kv, int group, int width, int pshift, int causal, int window) {
     const int64_t base = (int64_t)B * kv * (((int64_t)max_new * group + 15) / 16);
-    const int64_t tiles = (((int64_t)width << pshift) + 63) / 64;
-    int64_t n = base >= 768 ? 1 : 768 / (base > 0 ? base : 1);
-    if (n > (tiles + NW - 1) / NW) n = (tiles + NW - 1) / NW;
-    return (int)(n < 1 ? 1 : (n > 256 ? 256 : n));
+    int64_t tiles = (((int64_t)width << pshift) + 63) / 64;
+    if (causal && window) {      // a column tile's queries lie at most 15 tokens apart
+        const int64_t w = ((int64_t)window + causal + 15 + 63) / 64 + 1;
+        if (w < tiles) tiles = w;
+    }
+    if (tiles <= 4 * NW || base <= 0) return {1, (int)(tiles > 0 ? tiles : 1)};
+    int64_t chunk = (tiles * base + 2047) / 2048;
+    if (chunk < (tiles + MAX_SPLIT - 1) / MAX_SPLIT) chunk = (tiles + MAX_SPLIT - 1) / MAX_SPLIT;
+    chunk = (chunk + NW - 1) / NW * NW;
+    if (chunk >= tiles) return {1, (int)tiles};
+    return {(int)((tiles + chunk - 1) / chunk), (int)chunk};
 }
 
 }  // namespace
 
 extern "C" size_t pgt_kv_attention_workspace_bytes(int32_t B, int32_t max_new, int32_t heads, int32_t kv_heads, int32_t hd, int32_t width,
-                                                   int32_t page) {
-    if (B <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || hd <= 0 || width <= 0 || kv_page_shift(page) < 0 || heads % kv_heads) return 0;
-    const int n = splits(B, max_new, kv_heads, heads / kv_heads, width, kv_page_shift(page));
+                                                   int32_t page, int32_t causal, int32_t window) {
+    if (B <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || hd <= 0 || width <= 0 || kv_page_shift(page) < 0 || heads % kv_heads || causal < 0 || window < 0) return 0;
+    const int n = splits(B, max_new, kv_heads, heads / kv_heads, width, kv_page_shift(page), causal, window).n;
     return n == 1 ? 0 : (size_t)B * max_new * heads * n * (hd + 2) * sizeof(float);
 }
 
@@ -405,7 +436,9 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     PGT_CHECK((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "kv_attention: misaligned pointer");
     p.group = heads / kv_heads;
     p.nct = (int)(((int64_t)max_new * p.group + 15) / 16);
-    p.nsplit = width > 0 ? splits(B, max_new, kv_heads, p.group, width, p.pshift) : 1;
+    const Split sp = splits(B, max_new, kv_heads, p.group, width, p.pshift, causal, window);
+    p.nsplit = sp.n;
+    p.chunk = sp.chunk;
     const int64_t wgs = (int64_t)B * kv_heads * p.nct * p.nsplit, slots = (int64_t)B * max_new * heads;
     PGT_CHECK((int64_t)max_new * p.group < (1 << 30) && wgs < (1LL << 31) && slots < (1LL << 31),
               "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
@@ -420,7 +453,7 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
 #define ATTN_GO(TT, HD_)                                                                                              \
     do {                                                                                                              \
         hipLaunchKernelGGL((kv_attn_kernel<TT, HD_>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);                  \
-        if (p.nsplit > 1) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)slots), dim3(HD_), 0, st, p); \
+        if (p.nsplit > 1) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)slots), dim3(256), 0, st, p); \
     } while (0)
 #define ATTN_HD(TT)                                                                                                   \
     do {                                                                                                              \
