@@ -57,9 +57,9 @@ struct AttnP {
     const uint8_t *kp, *vp;
     const float *ks, *vs;
     const int32_t *table, *lens, *cu;
-    float *po, *pml;                  // partial results of the splits: (slot, split, hd), (slot, split, {m, l})
+    float *po, *pml;                  // partial results: (slot, 16 columns, hd), (slot, 16 columns, {m, l})
     int64_t ldq, ldo;
-    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, nct, nsplit, chunk, causal, window;      // chunk: tiles of 64 tokens per split
+    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, nct, wgs, causal, window;      // wgs: workgroups that share the work, 0 = one per column tile
     float c;                          // scale * log2 e
 };
 
@@ -93,8 +93,84 @@ __device__ __forceinline__ void sees(const AttnP& p, int len, int pos, int& lo, 
     lo = min(lo, hi);
 }
 
-constexpr int MAX_SPLIT = 256;
 constexpr int NW = 4;      // waves per workgroup, each with its own share of the tokens
+
+// Work sharing (wgs > 0).  The tiles of 64 tokens of all (sequence, kv head, column tile) in this order are one line that is cut into wgs equal
+// pieces, whatever the lengths: every workgroup streams the same number of bytes, and as many run as fit the chip at once.  A column tile
+// that is cut leaves a partial result per piece - workgroup w and column tile i meet in slot w + i, which no other pair has - and the join
+// adds them.  Lengths are only known on the device: each workgroup sums them up.
+struct Line {
+    int total, share;
+};
+// tiles of each column tile of sequence b (the range that its first to last query see), and its column tiles
+__device__ __forceinline__ int seq_tiles(const AttnP& p, const Seq& s, int& first, int& nct) {
+    int lo, hi, dummy;
+    sees(p, s.len, s.len - s.n, lo, dummy);
+    sees(p, s.len, s.len - 1, dummy, hi);
+    first = lo >> 6;
+    nct = (s.n * p.group + 15) >> 4;
+    return s.n > 0 ? max(((hi + 63) >> 6) - first, 0) : 0;
+}
+__device__ __forceinline__ int seq_units(const AttnP& p, int b) {
+    int first, nct;
+    const int t = seq_tiles(p, seq_of(p, b), first, nct);
+    return t * nct * p.kv;
+}
+__device__ __forceinline__ int wave_sum_i(int v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+// the whole line, and the part of it before sequence b (all 256 threads; red: 8 ints)
+__device__ __forceinline__ Line line_of(const AttnP& p, int b, int& before, int* red) {
+    int all = 0, pre = 0;
+    for (int i = threadIdx.x; i < p.B; i += 64 * NW) {
+        const int u = seq_units(p, i);
+        all += u;
+        if (i < b) pre += u;
+    }
+    all = wave_sum_i(all);
+    pre = wave_sum_i(pre);
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6] = all;
+        red[4 + (threadIdx.x >> 6)] = pre;
+    }
+    __syncthreads();
+    Line l;
+    l.total = red[0] + red[1] + red[2] + red[3];
+    before = red[4] + red[5] + red[6] + red[7];
+    l.share = max((l.total + p.wgs - 1) / p.wgs, NW);
+    return l;
+}
+// the sequence that place `pos` of the line lies in, and the line before it
+__device__ __forceinline__ void locate(const AttnP& p, int pos, int& b, int& before, int* red) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int run = 0;
+    for (int c = 0; c < p.B; c += 64 * NW) {
+        const int u = c + tid < p.B ? seq_units(p, c + tid) : 0;
+        int v = u;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int w = __shfl_up(v, o, 64);
+            if (lane >= o) v += w;
+        }
+        __syncthreads();
+        if (lane == 63) red[wave] = v;
+        __syncthreads();
+        int e = run + v - u;
+        for (int w = 0; w < wave; ++w) e += red[w];
+        if (pos >= e && pos < e + u) {
+            red[4] = c + tid;
+            red[5] = e;
+        }
+        run += red[0] + red[1] + red[2] + red[3];
+        if (run > pos) break;
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(red[4]);
+    before = __builtin_amdgcn_readfirstlane(red[5]);
+    __syncthreads();
+}
 
 template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2) void kv_attn_kernel(const AttnP p) {
     constexpr bool F32 = __is_same(T, float);
@@ -104,13 +180,40 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     constexpr int ND = HD / 16;              // row tiles of O^T
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int col = lane & 15, g = lane >> 4;
-    int id = blockIdx.x;
-    const int split = id % p.nsplit; id /= p.nsplit;
-    const int ct = id % p.nct; id /= p.nct;
-    const int hk = id % p.kv, b = id / p.kv;
+    __shared__ int red[8];
+    __shared__ float sm[NW][16], sl[NW][16];
+    __shared__ __attribute__((aligned(16))) float so[NW][16][HD + 4];
+    int b, before = 0, pos = 0, pos_end = 0;
+    if (p.wgs == 0) {
+        b = blockIdx.x / (p.nct * p.kv);
+    } else {
+        const Line line = line_of(p, 0, before, red);
+        pos = blockIdx.x * line.share;
+        pos_end = min(pos + line.share, line.total);
+        if (pos >= pos_end) return;
+        locate(p, pos, b, before, red);
+    }
+    for (;;) {      // the column tiles that this workgroup's part of the line touches
     const Seq s = seq_of(p, b);
+    int ct, hk, t0, te, slot, units = 0;
+    if (p.wgs == 0) {
+        ct = blockIdx.x % p.nct;
+        hk = blockIdx.x / p.nct % p.kv;
+        t0 = te = slot = 0;
+        if (ct * 16 >= s.n * p.group) return;
+    } else {
+        int nct, first;
+        const int tiles = seq_tiles(p, s, first, nct);
+        units = tiles * nct * p.kv;
+        if (units == 0) { ++b; continue; }
+        const int i = (pos - before) / tiles, off = pos - before - i * tiles;
+        ct = i % nct;
+        hk = i / nct;
+        t0 = first + off;
+        te = first + min(off + pos_end - pos, tiles);
+        slot = blockIdx.x + (b * p.kv + hk) * p.nct + ct;
+    }
     const int cols = s.n * p.group;
-    if (ct * 16 >= cols) return;
     const int qc = ct * 16 + col;
     const int qi = min(qc, cols - 1) / p.group;
     const int head = hk * p.group + min(qc, cols - 1) % p.group;
@@ -120,9 +223,10 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     int lo_a, hi_a, lo_z, hi_z;
     sees(p, s.len, s.len - s.n + ct * 16 / p.group, lo_a, hi_a);
     sees(p, s.len, s.len - s.n + min(ct * 16 + 15, cols - 1) / p.group, lo_z, hi_z);
-    const int t_first = lo_a >> 6, t_end = (hi_z + 63) >> 6;
-    const int t0 = t_first + split * p.chunk, te = min(t0 + p.chunk, t_end);
-    if (p.nsplit > 1 && t0 >= te) return;      // the join does not look at it
+    if (p.wgs == 0) {
+        t0 = lo_a >> 6;
+        te = (hi_z + 63) >> 6;
+    }
 
     // Q^T operand: k-step 2 s + h covers dims 64 s + 16 g + 8 h .. + 7 of lane group g - the order of the K loads
     uint4 qf[QP][KS];
@@ -318,8 +422,6 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     l += __shfl_xor(l, 32, 64);
 
     // join the waves: every one against the common reference
-    __shared__ float sm[NW][16], sl[NW][16];
-    __shared__ __attribute__((aligned(16))) float so[NW][16][HD + 4];
     if (g == 0) sm[wave][col] = m;
     __syncthreads();
     float mm = sm[0][col];
@@ -336,7 +438,6 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     // thread: column tid / 16, HD / 16 consecutive dims
     constexpr int PD = HD / 16;
     const int c2 = tid >> 4, d2 = (tid & 15) * PD, qc2 = ct * 16 + c2;
-    if (qc2 >= cols) return;
     float f[PD], lt = 0.f;
 #pragma unroll
     for (int e = 0; e < PD; ++e) f[e] = 0.f;
@@ -346,63 +447,82 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
 #pragma unroll
         for (int e = 0; e < PD; ++e) f[e] += so[w][c2][d2 + e];
     }
-    const int qi2 = qc2 / p.group, head2 = hk * p.group + qc2 % p.group;
-    if (p.nsplit == 1) {
-        const float inv = lt == 0.f ? 0.f : 1.f / lt;      // a row that sees nothing is zero
-        T* op = (T*)p.out + (s.r0 + qi2) * p.ldo + head2 * HD + d2;
+    if (p.wgs == 0) {
+        if (qc2 < cols) {
+            const int qi2 = qc2 / p.group, head2 = hk * p.group + qc2 % p.group;
+            const float inv = lt == 0.f ? 0.f : 1.f / lt;      // a row that sees nothing is zero
+            T* op = (T*)p.out + (s.r0 + qi2) * p.ldo + head2 * HD + d2;
 #pragma unroll
-        for (int e = 0; e < PD; ++e) f[e] = lt == 0.f ? 0.f : f[e] * inv;
+            for (int e = 0; e < PD; ++e) f[e] = lt == 0.f ? 0.f : f[e] * inv;
 #pragma unroll
-        for (int e = 0; e < PD; e += 4) store4(op + e, f + e);
-    } else {
-        const size_t slot = ((size_t)b * p.max_new + qi2) * p.heads + head2;
-        float* w = p.po + (slot * p.nsplit + split) * HD + d2;
+            for (int e = 0; e < PD; e += 4) store4(op + e, f + e);
+        }
+        return;
+    }
+    if (qc2 < cols) {
+        float* w = p.po + ((size_t)slot * 16 + c2) * HD + d2;
 #pragma unroll
-        for (int e = 0; e < PD; ++e) w[e] = f[e];
+        for (int e = 0; e < PD; e += 4) store4(w + e, f + e);
         if ((tid & 15) == 0) {
             float mm2 = sm[0][c2];
 #pragma unroll
             for (int k = 1; k < NW; ++k) mm2 = fmaxf(mm2, sm[k][c2]);
-            *reinterpret_cast<float2*>(p.pml + (slot * p.nsplit + split) * 2) = make_float2(mm2, lt);
+            store2(p.pml + ((size_t)slot * 16 + c2) * 2, mm2, lt);
         }
+    }
+    pos += te - t0;
+    if (pos >= pos_end) return;
+    if (pos - before >= units) {
+        before += units;
+        ++b;
+    }
+    __syncthreads();
     }
 }
 
-// out = the splits' results against their common reference.  One workgroup per (sequence, token, head): HD / 4 threads hold the row, the
-// rest of the 256 take other splits, four loads in flight each.
-template <typename T, int HD> __global__ __launch_bounds__(256) void kv_attn_join_kernel(const AttnP p) {
-    constexpr int LP = HD / 4, NS = 256 / LP;
-    __shared__ float2 ml[MAX_SPLIT];
+// out = the pieces' results against their common reference.  One workgroup per (sequence, token, head): HD / 4 threads hold the row, the
+// rest of the 256 take other pieces, four loads in flight each.
+constexpr int MAX_WGS = 768;
+template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn_join_kernel(const AttnP p) {
+    constexpr int LP = HD / 4, NS = 64 * NW / LP;
+    __shared__ float al[MAX_WGS];
     __shared__ f32x4 so[NS][LP];
-    __shared__ float sm[4], sl[4];
+    __shared__ float sm[NW], sl[NW];
+    __shared__ int red[8];
     int id = blockIdx.x;
     const int head = id % p.heads; id /= p.heads;
     const int qi = id % p.max_new, b = id / p.max_new, tid = threadIdx.x;
     const Seq s = seq_of(p, b);
     if (qi >= s.n) return;
-    // the splits that hold tokens of this query's column tile
-    const int col0 = (qi * p.group + head % p.group) & ~15, colz = min(col0 + 15, s.n * p.group - 1);
-    int lo_a, hi_z, dummy;
-    sees(p, s.len, s.len - s.n + col0 / p.group, lo_a, dummy);
-    sees(p, s.len, s.len - s.n + colz / p.group, dummy, hi_z);
-    const int tiles = ((hi_z + 63) >> 6) - (lo_a >> 6), n = tiles > 0 ? (tiles + p.chunk - 1) / p.chunk : 0;
-    const size_t slot = ((size_t)b * p.max_new + qi) * p.heads + head;
-    const float2 w = tid < n ? reinterpret_cast<const float2*>(p.pml)[slot * p.nsplit + tid] : make_float2(-INFINITY, 0.f);
-    float m = wave_max(w.x);
+    int before, first, nct;
+    const Line line = line_of(p, b, before, red);
+    const int tiles = seq_tiles(p, s, first, nct);
+    const int qc = qi * p.group + head % p.group, ct = qc >> 4, hk = head / p.group;
+    const int begin = before + (hk * nct + ct) * tiles;      // this column tile's part of the line, and the workgroups that hold some of it
+    const int w0 = begin / line.share, n = tiles > 0 ? (begin + tiles - 1) / line.share - w0 + 1 : 0;
+    const size_t slot = (size_t)w0 + (size_t)(b * p.kv + hk) * p.nct + ct;      // the next workgroup's is the next slot
+    const float2* ml = reinterpret_cast<const float2*>(p.pml) + slot * 16 + (qc & 15);
+    float m = -INFINITY, l = 0.f;
+    for (int i = tid; i < n; i += 64 * NW) m = fmaxf(m, ml[i * 16].x);
+    m = wave_max(m);
     if ((tid & 63) == 0) sm[tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    const float al = w.x == -INFINITY ? 1.f : exp2_(w.x - m);      // a split that saw nothing holds zeros (or NaN)
-    if (tid < n) ml[tid] = make_float2(al, w.y * al);
-    const float lw = wave_sum(tid < n ? w.y * al : 0.f);
-    if ((tid & 63) == 0) sl[tid >> 6] = lw;
+    for (int i = tid; i < n; i += 64 * NW) {
+        const float2 w = ml[i * 16];
+        const float a = w.x == -INFINITY ? 1.f : exp2_(w.x - m);      // a piece in which this query saw nothing holds zeros (or NaN)
+        al[i] = a;
+        l += w.y * a;
+    }
+    l = wave_sum(l);
+    if ((tid & 63) == 0) sl[tid >> 6] = l;
     __syncthreads();
-    const float l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
     const int c = tid % LP, k = tid / LP;
-    const f32x4* po = reinterpret_cast<const f32x4*>(p.po + slot * p.nsplit * HD) + c;
+    const f32x4* po = reinterpret_cast<const f32x4*>(p.po + (slot * 16 + (qc & 15)) * HD) + c;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = k; i < n; i += NS) o += po[(size_t)i * LP] * ml[i].x;
+    for (int i = k; i < n; i += NS) o += po[(size_t)i * 16 * LP] * al[i];
     so[k][c] = o;
     __syncthreads();
     if (k) return;
@@ -414,24 +534,20 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void kv_attn_joi
     store4((T*)p.out + (s.r0 + qi) * p.ldo + head * HD + 4 * c, f);
 }
 
-// Splits of the tokens, and tiles of 64 tokens in each: about 1024 workgroups of equal work (ragged lengths: what is past a sequence's
-// end exits at once), at least a tile per wave, and one split where the whole length is short
-struct Split {
-    int n, chunk;
-};
-Split splits(int B, int max_new, int kv, int group, int width, int pshift, int causal, int window) {
-    const int64_t base = (int64_t)B * kv * (((int64_t)max_new * group + 15) / 16);
+// Workgroups that share the work: as many as run at once (hd 64: 3 per CU, 128: 2), or 0 = one per column tile, without a join, where no
+// sequence can be longer than 16 tiles or there are so many column tiles that the chip is full anyway
+int sharing(int B, int max_new, int kv, int group, int hd, int width, int pshift, int causal, int window) {
+    const int64_t segs = (int64_t)B * kv * (((int64_t)max_new * group + 15) / 16);
     int64_t tiles = (((int64_t)width << pshift) + 63) / 64;
-    if (causal && window) {      // a column tile's queries lie at most 15 tokens apart
-        const int64_t w = ((int64_t)window + causal + 15 + 63) / 64 + 1;
+    if (causal && window) {      // from the first query's first token to the last one's last
+        const int64_t w = ((int64_t)window + causal + max_new + 63) / 64 + 1;
         if (w < tiles) tiles = w;
     }
-    if (tiles <= 4 * NW || base <= 0) return {1, (int)(tiles > 0 ? tiles : 1)};
-    int64_t chunk = (tiles * base + 1023) / 1024;
-    if (chunk < (tiles + MAX_SPLIT - 1) / MAX_SPLIT) chunk = (tiles + MAX_SPLIT - 1) / MAX_SPLIT;
-    chunk = (chunk + NW - 1) / NW * NW;
-    if (chunk >= tiles) return {1, (int)tiles};
-    return {(int)((tiles + chunk - 1) / chunk), (int)chunk};
+    if (tiles <= 4 * NW || segs <= 0 || segs >= 4096) return 0;
+    return hd == 64 ? 768 : 512;
+}
+size_t slots_of(int B, int max_new, int kv, int group, int wgs) {
+    return wgs ? (size_t)wgs + (size_t)B * kv * (((size_t)max_new * group + 15) / 16) : 0;
 }
 
 }  // namespace
@@ -439,8 +555,8 @@ Split splits(int B, int max_new, int kv, int group, int width, int pshift, int c
 extern "C" size_t pgt_kv_attention_workspace_bytes(int32_t B, int32_t max_new, int32_t heads, int32_t kv_heads, int32_t hd, int32_t width,
                                                    int32_t page, int32_t causal, int32_t window) {
     if (B <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || hd <= 0 || width <= 0 || kv_page_shift(page) < 0 || heads % kv_heads || causal < 0 || window < 0) return 0;
-    const int n = splits(B, max_new, kv_heads, heads / kv_heads, width, kv_page_shift(page), causal, window).n;
-    return n == 1 ? 0 : (size_t)B * max_new * heads * n * (hd + 2) * sizeof(float);
+    const int group = heads / kv_heads, wgs = sharing(B, max_new, kv_heads, group, hd, width, kv_page_shift(page), causal, window);
+    return slots_of(B, max_new, kv_heads, group, wgs) * 16 * (hd + 2) * sizeof(float);
 }
 
 extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -473,25 +589,25 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     PGT_CHECK((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "kv_attention: misaligned pointer");
     p.group = heads / kv_heads;
     p.nct = (int)(((int64_t)max_new * p.group + 15) / 16);
-    const Split sp = splits(B, max_new, kv_heads, p.group, width, p.pshift, causal, window);
-    p.nsplit = sp.n;
-    p.chunk = sp.chunk;
-    const int64_t wgs = (int64_t)B * kv_heads * p.nct * p.nsplit, slots = (int64_t)B * max_new * heads;
-    PGT_CHECK((int64_t)max_new * p.group < (1 << 30) && wgs < (1LL << 31) && slots < (1LL << 31),
+    p.wgs = sharing(B, max_new, kv_heads, p.group, hd, width, p.pshift, causal, window);
+    const int64_t segs = (int64_t)B * kv_heads * p.nct, wgs = p.wgs ? p.wgs : segs, rws = (int64_t)B * max_new * heads;
+    PGT_CHECK((int64_t)max_new * p.group < (1 << 30) && segs < (1LL << 31) && rws < (1LL << 31),
               "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
-    if (p.nsplit > 1) {
-        const size_t need = (size_t)slots * p.nsplit * (hd + 2) * sizeof(float);
+    if (p.wgs) {
+        PGT_CHECK((double)segs * (((int64_t)width << p.pshift) / 64 + 1) < 2147483648.0,
+                  "kv_attention: %d sequences of up to %d pages of %d tokens exceed one launch", B, width, page);
+        const size_t slots = slots_of(B, max_new, kv_heads, p.group, p.wgs), need = slots * 16 * (hd + 2) * sizeof(float);
         PGT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                   "kv_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         p.po = (float*)workspace;
-        p.pml = p.po + (size_t)slots * p.nsplit * hd;
+        p.pml = p.po + slots * 16 * hd;
     }
     hipStream_t st = (hipStream_t)stream;
 #define ATTN_GO(TT, HD_)                                                                                              \
     do {                                                                                                              \
         if (p.nct == 1) hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, true>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p); \
         else hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, false>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);      \
-        if (p.nsplit > 1) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)slots), dim3(256), 0, st, p); \
+        if (p.wgs) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)rws), dim3(64 * NW), 0, st, p);   \
     } while (0)
 #define ATTN_HD(TT)                                                                                                   \
     do {                                                                                                              \
