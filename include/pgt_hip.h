@@ -362,8 +362,8 @@ int pgt_kv_read(int32_t dtype, void* k_out, int32_t ldk, void* v_out, int32_t ld
                 const float* k_scale, const float* v_scale, int32_t pages, int32_t page, int32_t kv_heads, int32_t hd,
                 const int32_t* table, int32_t ld_table, int32_t width, const int32_t* start, const int32_t* cu, int32_t B,
                 int32_t rows, int32_t max_rows, pgt_stream_t stream);
-size_t pgt_kv_attention_workspace_bytes(int32_t B, int32_t max_new, int32_t heads, int32_t kv_heads, int32_t hd, int32_t width,
-                                        int32_t page, int32_t causal, int32_t window);
+size_t pgt_kv_attention_workspace_bytes(int32_t dtype, int32_t B, int32_t max_new, int32_t heads, int32_t kv_heads, int32_t hd,
+                                        int32_t width, int32_t page, int32_t causal, int32_t window);
 int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const void* k_pages, const void* v_pages, const float* k_scale,
                      const float* v_scale, int32_t pages, int32_t page, int32_t kv_heads, int32_t hd, const int32_t* table,
                      int32_t ld_table, int32_t width, const int32_t* lens, const int32_t* cu, int32_t B, int32_t rows,

@@ -13,164 +13,12 @@
 // belong to block lane / 16 - one K and one V scale per lane - and are, in order, the 16 tokens that the lane's 16-byte load of V
 // holds: P goes from the accumulators into the operand without an exchange, and nothing passes through LDS.
 // The query columns are the group's heads times the tokens (column = token * group + head in group).
-#include "kv_common.h"
+#include "kv_attention.h"
 #include "pgt_internal.h"
 
 namespace {
 
-typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
-
-// 8 e4m3 codes -> 8 halves / bf16, exact
-__device__ __forceinline__ uint4 half8(uint32_t a, uint32_t b) {
-    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true)));
-}
-__device__ __forceinline__ uint4 bfloat8(uint32_t a, uint32_t b) {
-    return make_uint4(__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false)),
-                      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true)));
-}
-__device__ __forceinline__ f32x4 mma_h(const uint4& a, const uint4& b, const f32x4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(halfx8, a), __builtin_bit_cast(halfx8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ f32x4 mma_b(const uint4& a, const uint4& b, const f32x4& c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-// 16 bytes of the cache.  ONCE: with the streaming policy (7.1 instead of 6.3 TB/s on a plain read of 2 GiB), for launches in which no other
-// workgroup reads them (with it, 1024 query rows over the same pages took 1.5 times as long)
-template <bool ONCE> __device__ __forceinline__ uint4 load16(const uint8_t* p) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    const u32x4* q = reinterpret_cast<const u32x4*>(p);
-    if constexpr (ONCE) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(q));
-    else return __builtin_bit_cast(uint4, *q);
-}
-__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-// does any of the four codes stand for NaN (0x7f, 0xff)?
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-
-struct AttnP {
-    const void* q;
-    void* out;
-    const uint8_t *kp, *vp;
-    const float *ks, *vs;
-    const int32_t *table, *lens, *cu;
-    float *po, *pml;                  // partial results: (slot, 16 columns, hd), (slot, 16 columns, {m, l})
-    int64_t ldq, ldo;
-    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, nct, wgs, causal, window;      // wgs: workgroups that share the work, 0 = one per column tile
-    float c;                          // scale * log2 e
-};
-
-// sequence b: its packed rows and its tokens in the cache (which end with the rows' own)
-struct Seq {
-    int r0, n, len;
-};
-__device__ __forceinline__ Seq seq_of(const AttnP& p, int b) {
-    Seq s;
-    if (p.cu) {
-        s.r0 = min(max(p.cu[b], 0), p.rows);
-        s.n = min(min(max(p.cu[b + 1], s.r0), p.rows) - s.r0, p.max_new);
-    } else {
-        s.r0 = b * p.max_new;
-        s.n = p.max_new;
-    }
-    const int64_t cap = min((int64_t)p.width << p.pshift, (int64_t)0x7fffff00);
-    s.len = (int)min((int64_t)max(p.lens[b], 0), cap);
-    return s;
-}
-// tokens [lo, hi) that the query at position pos (of a sequence of len tokens) sees
-__device__ __forceinline__ void sees(const AttnP& p, int len, int pos, int& lo, int& hi) {
-    lo = 0;
-    hi = len;
-    if (p.causal) {
-        const uint32_t end = ((uint32_t)max(pos, 0) / (uint32_t)p.causal + 1) * (uint32_t)p.causal;      // < 2^32: pos + causal at most
-        hi = (int)min(end, (uint32_t)len);
-        if (p.window) lo = (int)min(end > (uint32_t)p.window ? end - (uint32_t)p.window : 0u, (uint32_t)len);
-    }
-    if (pos < 0) hi = 0;      // more rows than tokens: nothing to see
-    lo = min(lo, hi);
-}
-
 constexpr int NW = 4;      // waves per workgroup, each with its own share of the tokens
-
-// Work sharing (wgs > 0).  The tiles of 64 tokens of all (sequence, kv head, column tile) in this order are one line that is cut into wgs equal
-// pieces, whatever the lengths: every workgroup streams the same number of bytes, and as many run as fit the chip at once.  A column tile
-// that is cut leaves a partial result per piece - workgroup w and column tile i meet in slot w + i, which no other pair has - and the join
-// adds them.  Lengths are only known on the device: each workgroup sums them up.
-struct Line {
-    int total, share;
-};
-// tiles of each column tile of sequence b (the range that its first to last query see), and its column tiles
-__device__ __forceinline__ int seq_tiles(const AttnP& p, const Seq& s, int& first, int& nct) {
-    int lo, hi, dummy;
-    sees(p, s.len, s.len - s.n, lo, dummy);
-    sees(p, s.len, s.len - 1, dummy, hi);
-    first = lo >> 6;
-    nct = (s.n * p.group + 15) >> 4;
-    return s.n > 0 ? max(((hi + 63) >> 6) - first, 0) : 0;
-}
-__device__ __forceinline__ int seq_units(const AttnP& p, int b) {
-    int first, nct;
-    const int t = seq_tiles(p, seq_of(p, b), first, nct);
-    return t * nct * p.kv;
-}
-__device__ __forceinline__ int wave_sum_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-// the whole line, and the part of it before sequence b (all 256 threads; red: 8 ints)
-__device__ __forceinline__ Line line_of(const AttnP& p, int b, int& before, int* red) {
-    int all = 0, pre = 0;
-    for (int i = threadIdx.x; i < p.B; i += 64 * NW) {
-        const int u = seq_units(p, i);
-        all += u;
-        if (i < b) pre += u;
-    }
-    all = wave_sum_i(all);
-    pre = wave_sum_i(pre);
-    if ((threadIdx.x & 63) == 0) {
-        red[threadIdx.x >> 6] = all;
-        red[4 + (threadIdx.x >> 6)] = pre;
-    }
-    __syncthreads();
-    Line l;
-    l.total = red[0] + red[1] + red[2] + red[3];
-    before = red[4] + red[5] + red[6] + red[7];
-    l.share = max((l.total + p.wgs - 1) / p.wgs, NW);
-    return l;
-}
-// the sequence that place `pos` of the line lies in, and the line before it
-__device__ __forceinline__ void locate(const AttnP& p, int pos, int& b, int& before, int* red) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    int run = 0;
-    for (int c = 0; c < p.B; c += 64 * NW) {
-        const int u = c + tid < p.B ? seq_units(p, c + tid) : 0;
-        int v = u;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int w = __shfl_up(v, o, 64);
-            if (lane >= o) v += w;
-        }
-        __syncthreads();
-        if (lane == 63) red[wave] = v;
-        __syncthreads();
-        int e = run + v - u;
-        for (int w = 0; w < wave; ++w) e += red[w];
-        if (pos >= e && pos < e + u) {
-            red[4] = c + tid;
-            red[5] = e;
-        }
-        run += red[0] + red[1] + red[2] + red[3];
-        if (run > pos) break;
-    }
-    __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(red[4]);
-    before = __builtin_amdgcn_readfirstlane(red[5]);
-    __syncthreads();
-}
 
 template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2) void kv_attn_kernel(const AttnP p) {
     constexpr bool F32 = __is_same(T, float);
@@ -187,11 +35,11 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     if (p.wgs == 0) {
         b = blockIdx.x / (p.nct * p.kv);
     } else {
-        const Line line = line_of(p, 0, before, red);
+        const Line line = line_of<NW>(p, 0, before, red);
         pos = blockIdx.x * line.share;
         pos_end = min(pos + line.share, line.total);
         if (pos >= pos_end) return;
-        locate(p, pos, b, before, red);
+        locate<NW>(p, pos, b, before, red);
     }
     for (;;) {      // the column tiles that this workgroup's part of the line touches
     const Seq s = seq_of(p, b);
@@ -495,21 +343,21 @@ template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn
     const Seq s = seq_of(p, b);
     if (qi >= s.n) return;
     int before, first, nct;
-    const Line line = line_of(p, b, before, red);
+    const Line line = line_of<NW>(p, b, before, red);
     const int tiles = seq_tiles(p, s, first, nct);
-    const int qc = qi * p.group + head % p.group, ct = qc >> 4, hk = head / p.group;
+    const int qc = qi * p.group + head % p.group, ct = qc >> p.cshift, hk = head / p.group;
     const int begin = before + (hk * nct + ct) * tiles;      // this column tile's part of the line, and the workgroups that hold some of it
     const int w0 = begin / line.share, n = tiles > 0 ? (begin + tiles - 1) / line.share - w0 + 1 : 0;
     const size_t slot = (size_t)w0 + (size_t)(b * p.kv + hk) * p.nct + ct;      // the next workgroup's is the next slot
-    const float2* ml = reinterpret_cast<const float2*>(p.pml) + slot * 16 + (qc & 15);
+    const float2* ml = reinterpret_cast<const float2*>(p.pml) + (slot << p.cshift) + (qc & ((1 << p.cshift) - 1));
     float m = -INFINITY, l = 0.f;
-    for (int i = tid; i < n; i += 64 * NW) m = fmaxf(m, ml[i * 16].x);
+    for (int i = tid; i < n; i += 64 * NW) m = fmaxf(m, ml[(size_t)i << p.cshift].x);
     m = wave_max(m);
     if ((tid & 63) == 0) sm[tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
     for (int i = tid; i < n; i += 64 * NW) {
-        const float2 w = ml[i * 16];
+        const float2 w = ml[(size_t)i << p.cshift];
         const float a = w.x == -INFINITY ? 1.f : exp2_(w.x - m);      // a piece in which this query saw nothing holds zeros (or NaN)
         al[i] = a;
         l += w.y * a;
@@ -519,10 +367,10 @@ template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn
     __syncthreads();
     l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
     const int c = tid % LP, k = tid / LP;
-    const f32x4* po = reinterpret_cast<const f32x4*>(p.po + (slot * 16 + (qc & 15)) * HD) + c;
+    const f32x4* po = reinterpret_cast<const f32x4*>(p.po + ((slot << p.cshift) + (qc & ((1 << p.cshift) - 1))) * HD) + c;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-    for (int i = k; i < n; i += NS) o += po[(size_t)i * 16 * LP] * al[i];
+    for (int i = k; i < n; i += NS) o += po[((size_t)i << p.cshift) * LP] * al[i];
     so[k][c] = o;
     __syncthreads();
     if (k) return;
@@ -534,29 +382,41 @@ template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn
     store4((T*)p.out + (s.r0 + qi) * p.ldo + head * HD + 4 * c, f);
 }
 
-// Workgroups that share the work: as many as run at once (hd 64: 3 per CU, 128: 2), or 0 = one per column tile, without a join, where no
-// sequence can be longer than 16 tiles or there are so many column tiles that the chip is full anyway
-int sharing(int B, int max_new, int kv, int group, int hd, int width, int pshift, int causal, int window) {
-    const int64_t segs = (int64_t)B * kv * (((int64_t)max_new * group + 15) / 16);
+// How a call is run: column tiles of 16 (this file) or 256 (kv_attention_rows.hip), and the workgroups that share the work
+struct Way {
+    int cshift, wgs;
+    size_t segs, slots;      // column tiles of the launch; slots of partial results
+};
+Way way_of(int dtype, int B, int max_new, int kv, int group, int hd, int width, int pshift, int causal, int window) {
+    Way w;
+    const int64_t cols = (int64_t)max_new * group;
+    w.cshift = dtype != PGT_F32 && cols >= 64 ? (hd == 64 ? 8 : 7) : 4;
+    w.segs = (size_t)B * kv * ((cols + (1 << w.cshift) - 1) >> w.cshift);
     int64_t tiles = (((int64_t)width << pshift) + 63) / 64;
     if (causal && window) {      // from the first query's first token to the last one's last
-        const int64_t w = ((int64_t)window + causal + max_new + 63) / 64 + 1;
-        if (w < tiles) tiles = w;
+        const int64_t n = ((int64_t)window + causal + max_new + 63) / 64 + 1;
+        if (n < tiles) tiles = n;
     }
-    if (tiles <= 4 * NW || segs <= 0 || segs >= 4096) return 0;
-    return hd == 64 ? 768 : 512;
-}
-size_t slots_of(int B, int max_new, int kv, int group, int wgs) {
-    return wgs ? (size_t)wgs + (size_t)B * kv * (((size_t)max_new * group + 15) / 16) : 0;
+    if (w.cshift != 4) {
+        w.wgs = 512;
+        if (w.segs >= 192 || tiles <= MIN_SHARE) w.wgs = 0;
+    } else {
+        // as many as run at once (hd 64: 3 per CU, 128: 2), or one per column tile, without a join, where no sequence can be longer than
+        // 16 tiles or there are so many column tiles that the chip is full anyway
+        w.wgs = hd == 64 ? 768 : 512;
+        if (tiles <= 4 * NW || w.segs == 0 || w.segs >= 4096) w.wgs = 0;
+    }
+    w.slots = w.wgs ? w.wgs + w.segs : 0;
+    return w;
 }
 
 }  // namespace
 
-extern "C" size_t pgt_kv_attention_workspace_bytes(int32_t B, int32_t max_new, int32_t heads, int32_t kv_heads, int32_t hd, int32_t width,
+extern "C" size_t pgt_kv_attention_workspace_bytes(int32_t dtype, int32_t B, int32_t max_new, int32_t heads, int32_t kv_heads, int32_t hd, int32_t width,
                                                    int32_t page, int32_t causal, int32_t window) {
     if (B <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || hd <= 0 || width <= 0 || kv_page_shift(page) < 0 || heads % kv_heads || causal < 0 || window < 0) return 0;
-    const int group = heads / kv_heads, wgs = sharing(B, max_new, kv_heads, group, hd, width, kv_page_shift(page), causal, window);
-    return slots_of(B, max_new, kv_heads, group, wgs) * 16 * (hd + 2) * sizeof(float);
+    const Way w = way_of(dtype, B, max_new, kv_heads, heads / kv_heads, hd, width, kv_page_shift(page), causal, window);
+    return (w.slots << w.cshift) * (hd + 2) * sizeof(float);
 }
 
 extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -588,24 +448,29 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
               "kv_attention: row strides must cover heads * head_dim and be multiples of 16 bytes");
     PGT_CHECK((((uintptr_t)q | (uintptr_t)out) & 15) == 0, "kv_attention: misaligned pointer");
     p.group = heads / kv_heads;
-    p.nct = (int)(((int64_t)max_new * p.group + 15) / 16);
-    p.wgs = sharing(B, max_new, kv_heads, p.group, hd, width, p.pshift, causal, window);
-    const int64_t segs = (int64_t)B * kv_heads * p.nct, wgs = p.wgs ? p.wgs : segs, rws = (int64_t)B * max_new * heads;
-    PGT_CHECK((int64_t)max_new * p.group < (1 << 30) && segs < (1LL << 31) && rws < (1LL << 31),
-              "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
-    if (p.wgs) {
-        PGT_CHECK((double)segs * (((int64_t)width << p.pshift) / 64 + 1) < 2147483648.0,
+    PGT_CHECK((int64_t)max_new * p.group < (1 << 30), "kv_attention: %d tokens per sequence exceed one launch", max_new);
+    const Way w = way_of(dtype, B, max_new, kv_heads, p.group, hd, width, p.pshift, causal, window);
+    p.cshift = w.cshift;
+    p.nct = (max_new * p.group + (1 << w.cshift) - 1) >> w.cshift;
+    p.wgs = w.wgs;
+    const size_t wgs = w.wgs ? w.wgs : w.segs, rws = (size_t)B * max_new * heads;
+    PGT_CHECK(w.segs < (1ULL << 31) && rws < (1ULL << 31), "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
+    if (w.wgs) {
+        PGT_CHECK((double)w.segs * (((int64_t)width << p.pshift) / 64 + 1) < 2147483648.0,
                   "kv_attention: %d sequences of up to %d pages of %d tokens exceed one launch", B, width, page);
-        const size_t slots = slots_of(B, max_new, kv_heads, p.group, p.wgs), need = slots * 16 * (hd + 2) * sizeof(float);
+        const size_t need = (w.slots << w.cshift) * (hd + 2) * sizeof(float);
         PGT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                   "kv_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         p.po = (float*)workspace;
-        p.pml = p.po + slots * 16 * hd;
+        p.pml = p.po + (w.slots << w.cshift) * hd;
     }
     hipStream_t st = (hipStream_t)stream;
+    if (w.cshift != 4)
+        if (const int rc = pgt_kv_attention_rows_launch(&p, dtype == PGT_BF16, hd, (unsigned)wgs, st)) return rc;
 #define ATTN_GO(TT, HD_)                                                                                              \
     do {                                                                                                              \
-        if (p.nct == 1) hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, true>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p); \
+        if (w.cshift != 4) {}                                                                                         \
+        else if (p.nct == 1) hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, true>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p); \
         else hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, false>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);      \
         if (p.wgs) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)rws), dim3(64 * NW), 0, st, p);   \
     } while (0)

@@ -19,6 +19,10 @@ template <typename T> __device__ __forceinline__ void store4(T* p, const float* 
     else *reinterpret_cast<uint2*>(p) = make_uint2(pair_of<T>(f[0], f[1]), pair_of<T>(f[2], f[3]));
 }
 
+template <typename T> __device__ __forceinline__ void store_nan(T* p) {      // T: bf16_t, half_t
+    *reinterpret_cast<uint16_t*>(p) = 0x7fff;                                 // a NaN in both
+}
+
 // log2 of a page's number of tokens, -1 if it is none of 16, 32, 64, 128
 static inline int kv_page_shift(int page) {
     for (int s = 4; s <= 7; ++s)

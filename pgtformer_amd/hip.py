@@ -74,7 +74,7 @@ SIGNATURES = {
     "pgt_qk_norm_rope_backward": [i32, vp, i32, vp, i32, vp, i32, vp, i32, i32, i32, i32, i32, vp, vp, i32, i32, vp, vp, f32, vp, i32, vp, i32, vp, vp, vp, sz, vp],
     "pgt_kv_append": [i32, vp, i32, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp],
     "pgt_kv_read": [i32, vp, i32, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, vp],
-    "pgt_kv_attention_workspace_bytes": [i32] * 9,
+    "pgt_kv_attention_workspace_bytes": [i32] * 10,
     "pgt_kv_attention": [i32, vp, i32, vp, vp, vp, vp, i32, i32, i32, i32, vp, i32, i32, vp, vp, i32, i32, i32, i32, f32, i32, i32, vp, i32, vp, sz, vp],
     "pgt_x3_split": [vp, i32, vp, i32, i32, i64, i32, vp],
     "pgt_x3_merge": [vp, i32, i32, vp, i32, i64, i32, vp],

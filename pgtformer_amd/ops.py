@@ -1261,7 +1261,7 @@ def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=
         ldo = _rows(out, heads * hd, "kv_attention: out")
         _apart((out,), (q,), "kv_attention")
     L = hip.lib()
-    nbytes = L.pgt_kv_attention_workspace_bytes(B, most, heads, cache.kv_heads, hd, width, cache.page, causal, window)
+    nbytes = L.pgt_kv_attention_workspace_bytes(_dt(q), B, most, heads, cache.kv_heads, hd, width, cache.page, causal, window)
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     tokens = width * cache.page
     pq, kp, vp, ks, vs, pt, pl, pc, po, pw, st = _pointers(q, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, lens, cu, out, ws)

@@ -145,12 +145,13 @@ def test_workspace_sizes():
     L = hip.lib()
     assert L.pgt_qk_norm_rope_backward_workspace_bytes(0, 64) == 0
     assert 0 < L.pgt_qk_norm_rope_backward_workspace_bytes(1 << 20, 256) <= 1024 * 2 * 256 * 4
-    f = L.pgt_kv_attention_workspace_bytes
-    assert f(0, 1, 8, 8, 64, 4, 16, 1, 0) == 0 and f(1, 1, 8, 3, 64, 4, 16, 1, 0) == 0 and f(1, 1, 8, 8, 64, 4, 24, 1, 0) == 0
-    assert f(1, 1, 8, 8, 64, 1, 16, 1, 0) == 0                  # one tile: nothing to join
-    long = f(1, 1, 32, 8, 128, 8192, 16, 1, 0)
-    assert isinstance(long, int) and long >= f(1, 1, 32, 8, 128, 8192, 16, 1, 4096) > 0 and f(1, 1, 32, 8, 128, 8192, 16, 1, 64) == 0
-    assert f(64, 2048, 32, 8, 128, 512, 32, 1, 0) == 0          # enough rows to fill the chip
+    f = L.pgt_kv_attention_workspace_bytes      # (dtype, B, max_new, heads, kv_heads, hd, width, page, causal, window)
+    for dtype in (0, 1, 3):
+        assert f(dtype, 0, 1, 8, 8, 64, 4, 16, 1, 0) == 0 and f(dtype, 1, 1, 8, 3, 64, 4, 16, 1, 0) == 0 and f(dtype, 1, 1, 8, 8, 64, 4, 24, 1, 0) == 0
+        assert f(dtype, 1, 1, 8, 8, 64, 1, 16, 1, 0) == 0       # one tile: nothing to join
+        long = f(dtype, 1, 1, 32, 8, 128, 8192, 16, 1, 0)
+        assert isinstance(long, int) and long >= f(dtype, 1, 1, 32, 8, 128, 8192, 16, 1, 4096) > 0 and f(dtype, 1, 1, 32, 8, 128, 8192, 16, 1, 64) == 0
+        assert f(dtype, 64, 2048, 32, 8, 128, 512, 32, 1, 0) == 0      # enough rows to fill the chip
     assert C.sizeof(C.c_size_t) == 8
 
 
