@@ -145,10 +145,21 @@ template <typename T, int HD, int NQ, int NW> __global__ __launch_bounds__(64 * 
         auto store = [&](int st) {
             char* d = smem + st * STAGE;
 #pragma unroll
+            for (int i = 0; i < UN; ++i) {      // (opaque: or the compiler regroups the registers right behind the loads, and waits for them there)
+                x3_opaque(rk[i]);
+                x3_opaque(rv[i]);
+            }
+#pragma unroll
             for (int i = 0; i < UN; ++i) {
                 const uint4 w = rk[i];
                 *reinterpret_cast<uint4*>(d + k_to + i * 8192) = HQ ? half8(w.x, w.y) : bfloat8(w.x, w.y);
                 *reinterpret_cast<uint4*>(d + k_to + i * 8192 + 1024) = HQ ? half8(w.z, w.w) : bfloat8(w.z, w.w);
+            }
+#pragma unroll
+            for (int i = 0; i < UN; ++i) {
+                const uint4 w = rv[i];
+                *reinterpret_cast<uint4*>(d + v_to + i * 1024) = half8(w.x, w.y);
+                *reinterpret_cast<uint4*>(d + v_to + i * 1024 + HD * 16) = half8(w.z, w.w);
             }
             uint32_t bad = 0;
 #pragma unroll
@@ -157,16 +168,11 @@ template <typename T, int HD, int NQ, int NW> __global__ __launch_bounds__(64 * 
                 nans = 1;
 #pragma unroll
                 for (int i = 0; i < UN; ++i) {
-                    uint4& w = rv[i];
-                    w.x &= ~((nan_bytes(w.x) >> 7) * 255u); w.y &= ~((nan_bytes(w.y) >> 7) * 255u);
-                    w.z &= ~((nan_bytes(w.z) >> 7) * 255u); w.w &= ~((nan_bytes(w.w) >> 7) * 255u);
+                    const uint4 w = rv[i];
+                    auto clean = [](uint32_t v) { return v & ~((nan_bytes(v) >> 7) * 255u); };
+                    *reinterpret_cast<uint4*>(d + v_to + i * 1024) = half8(clean(w.x), clean(w.y));
+                    *reinterpret_cast<uint4*>(d + v_to + i * 1024 + HD * 16) = half8(clean(w.z), clean(w.w));
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < UN; ++i) {
-                const uint4 w = rv[i];
-                *reinterpret_cast<uint4*>(d + v_to + i * 1024) = half8(w.x, w.y);
-                *reinterpret_cast<uint4*>(d + v_to + i * 1024 + HD * 16) = half8(w.z, w.w);
             }
             if (lane == 0)      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
                 sscale[st][wave] = make_float2(ok(rpage) ? fmaxf(fabsf(p.c) * rsk, 1e-30f) : -1.f, (float)((int)((__float_as_uint(rsv) >> 23) & 255) - 127));
