@@ -43,7 +43,8 @@ struct AttnP {
     const int32_t *table, *lens, *cu;
     float *po, *pml;                  // partial results: (slot, columns, hd), (slot, columns, {m, l})
     int64_t ldq, ldo;
-    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, cshift, nct, wgs, causal, window;      // column tiles of 2^cshift; wgs: workgroups that share the work, 0 = one per column tile
+    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, cshift, nct, wgs, jrows, causal, window;      // column tiles of 2^cshift; wgs: workgroups that share the work, 0 = one per
+                                      // column tile; jrows: rows of a column tile that the join looks at
     float c;                          // scale * log2 e
 };
 
@@ -77,41 +78,60 @@ __device__ __forceinline__ void sees(const AttnP& p, int len, int pos, int& lo, 
     lo = min(lo, hi);
 }
 
-constexpr int MIN_SHARE = 4;      // tiles of a piece: one per wave of a workgroup with few rows
+// values that every lane of a wave holds alike but that came from memory, into scalar registers
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ Seq uni(const Seq& s) { return {uni(s.r0), uni(s.n), uni(s.len)}; }
+__device__ __forceinline__ void sees_uni(const AttnP& p, int len, int pos, int& lo, int& hi) {
+    sees(p, len, pos, lo, hi);
+    lo = uni(lo);
+    hi = uni(hi);
+}
 
-// Work sharing (wgs > 0).  The tiles of 64 tokens of all (sequence, kv head, column tile) in this order are one line that is cut into wgs equal
-// pieces, whatever the lengths: every workgroup streams the same number of bytes, and as many run as fit the chip at once.  A column tile
-// that is cut leaves a partial result per piece - workgroup w and column tile i meet in slot w + i, which no other pair has - and the join
-// adds them.  Lengths are only known on the device: each workgroup sums them up.
-struct Line {
-    int total, share;
+constexpr float NEVER = -1e30f;      // reference of a query that has seen nothing (finite: differences and products stay numbers)
+constexpr int MIN_SHARE = 4;         // tiles of a piece: one per wave of a workgroup with few rows
+
+// Work sharing (wgs > 0).  The tiles of 64 tokens of all segments - (sequence, kv head, column tile), in this order - are one line that is cut
+// into wgs equal pieces, whatever the lengths: every workgroup does the same work, and as many run as fit the chip at once.  A segment that
+// is cut leaves a partial result per piece - workgroup w and segment e meet in slot w + e, which no other pair has - and the join adds
+// them; one that is not is finished where it was computed.  Lengths are only known on the device: each workgroup sums them up.
+struct Segment {
+    int b, hk, ct, first, tiles;      // first tile, tiles
 };
-// tiles of each column tile of sequence b (the range that its first to last query see), and its column tiles
-__device__ __forceinline__ int seq_tiles(const AttnP& p, const Seq& s, int& first, int& nct) {
-    int lo, hi, dummy;
-    sees(p, s.len, s.len - s.n, lo, dummy);
-    sees(p, s.len, s.len - 1, dummy, hi);
-    first = lo >> 6;
-    nct = (s.n * p.group + (1 << p.cshift) - 1) >> p.cshift;
-    return s.n > 0 ? max(((hi + 63) >> 6) - first, 0) : 0;
+__device__ __forceinline__ Segment segment_of(const AttnP& p, int e) {
+    Segment g;
+    g.ct = e % p.nct;
+    e /= p.nct;
+    g.hk = e % p.kv;
+    g.b = e / p.kv;
+    const Seq s = seq_of(p, g.b);
+    const int cols = s.n * p.group, c0 = g.ct << p.cshift, cz = min(c0 + (1 << p.cshift), cols) - 1;
+    g.first = g.tiles = 0;
+    if (c0 < cols) {
+        int lo, hi, dummy;
+        sees(p, s.len, s.len - s.n + c0 / p.group, lo, dummy);
+        sees(p, s.len, s.len - s.n + cz / p.group, dummy, hi);
+        g.first = lo >> 6;
+        g.tiles = max(((hi + 63) >> 6) - g.first, 0);
+    }
+    return g;
 }
-__device__ __forceinline__ int seq_units(const AttnP& p, int b) {
-    int first, nct;
-    const int t = seq_tiles(p, seq_of(p, b), first, nct);
-    return t * nct * p.kv;
-}
+__device__ __forceinline__ Segment uni(const Segment& g) { return {uni(g.b), uni(g.hk), uni(g.ct), uni(g.first), uni(g.tiles)}; }
 __device__ __forceinline__ int wave_sum_i(int v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-// the whole line, and the part of it before sequence b (all 64 * W threads; red: 2 * W ints)
-template <int W> __device__ __forceinline__ Line line_of(const AttnP& p, int b, int& before, int* red) {
+struct Line {
+    int total, share;
+};
+// the whole line, and the part of it before segment e (all 64 * W threads; red: 2 * W ints)
+template <int W> __device__ __forceinline__ Line line_of(const AttnP& p, int e, int& before, int* red) {
+    const int segs = p.B * p.kv * p.nct;
     int all = 0, pre = 0;
-    for (int i = threadIdx.x; i < p.B; i += 64 * W) {
-        const int u = seq_units(p, i);
+    for (int i = threadIdx.x; i < segs; i += 64 * W) {
+        const int u = segment_of(p, i).tiles;
         all += u;
-        if (i < b) pre += u;
+        if (i < e) pre += u;
     }
     all = wave_sum_i(all);
     pre = wave_sum_i(pre);
@@ -127,15 +147,17 @@ template <int W> __device__ __forceinline__ Line line_of(const AttnP& p, int b, 
         l.total += red[w];
         before += red[W + w];
     }
-    l.share = max((l.total + p.wgs - 1) / p.wgs, MIN_SHARE);
+    l.total = uni(l.total);
+    before = uni(before);
+    l.share = uni(max((l.total + p.wgs - 1) / p.wgs, MIN_SHARE));
     return l;
 }
-// the sequence that place `pos` of the line lies in, and the line before it
-template <int W> __device__ __forceinline__ void locate(const AttnP& p, int pos, int& b, int& before, int* red) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// the segment that place `pos` of the line lies in, and the line before it
+template <int W> __device__ __forceinline__ void locate(const AttnP& p, int pos, int& e, int& before, int* red) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, segs = p.B * p.kv * p.nct;
     int run = 0;
-    for (int c = 0; c < p.B; c += 64 * W) {
-        const int u = c + tid < p.B ? seq_units(p, c + tid) : 0;
+    for (int c = 0; c < segs; c += 64 * W) {
+        const int u = c + tid < segs ? segment_of(p, c + tid).tiles : 0;
         int v = u;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -145,19 +167,19 @@ template <int W> __device__ __forceinline__ void locate(const AttnP& p, int pos,
         __syncthreads();
         if (lane == 63) red[wave] = v;
         __syncthreads();
-        int e = run + v - u;
-        for (int w = 0; w < wave; ++w) e += red[w];
-        if (pos >= e && pos < e + u) {
+        int at = run + v - u;
+        for (int w = 0; w < wave; ++w) at += red[w];
+        if (pos >= at && pos < at + u) {
             red[W] = c + tid;
-            red[W + 1] = e;
+            red[W + 1] = at;
         }
 #pragma unroll
         for (int w = 0; w < W; ++w) run += red[w];
         if (run > pos) break;
     }
     __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(red[W]);
-    before = __builtin_amdgcn_readfirstlane(red[W + 1]);
+    e = uni(red[W]);
+    before = uni(red[W + 1]);
     __syncthreads();
 }
 

@@ -31,37 +31,23 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     __shared__ int red[8];
     __shared__ float sm[NW][16], sl[NW][16];
     __shared__ __attribute__((aligned(16))) float so[NW][16][HD + 4];
-    int b, before = 0, pos = 0, pos_end = 0;
-    if (p.wgs == 0) {
-        b = blockIdx.x / (p.nct * p.kv);
-    } else {
+    int e = blockIdx.x, before = 0, pos = 0, pos_end = 0;
+    if (p.wgs) {
         const Line line = line_of<NW>(p, 0, before, red);
         pos = blockIdx.x * line.share;
         pos_end = min(pos + line.share, line.total);
         if (pos >= pos_end) return;
-        locate<NW>(p, pos, b, before, red);
+        locate<NW>(p, pos, e, before, red);
     }
-    for (;;) {      // the column tiles that this workgroup's part of the line touches
-    const Seq s = seq_of(p, b);
-    int ct, hk, t0, te, slot, units = 0;
-    if (p.wgs == 0) {
-        ct = blockIdx.x % p.nct;
-        hk = blockIdx.x / p.nct % p.kv;
-        t0 = te = slot = 0;
-        if (ct * 16 >= s.n * p.group) return;
-    } else {
-        int nct, first;
-        const int tiles = seq_tiles(p, s, first, nct);
-        units = tiles * nct * p.kv;
-        if (units == 0) { ++b; continue; }
-        const int i = (pos - before) / tiles, off = pos - before - i * tiles;
-        ct = i % nct;
-        hk = i / nct;
-        t0 = first + off;
-        te = first + min(off + pos_end - pos, tiles);
-        slot = blockIdx.x + (b * p.kv + hk) * p.nct + ct;
-    }
+    for (;;) {      // the segments that this workgroup's part of the line touches
+    const Segment sg = uni(segment_of(p, e));
+    if (p.wgs && sg.tiles == 0) { ++e; continue; }
+    const int b = sg.b, hk = sg.hk, ct = sg.ct;
+    const Seq s = uni(seq_of(p, b));
     const int cols = s.n * p.group;
+    if (ct * 16 >= cols) return;
+    const int t0 = sg.first + (p.wgs ? pos - before : 0), te = p.wgs ? sg.first + min(pos_end - before, sg.tiles) : sg.first + sg.tiles;
+    const bool whole = te - t0 == sg.tiles;
     const int qc = ct * 16 + col;
     const int qi = min(qc, cols - 1) / p.group;
     const int head = hk * p.group + min(qc, cols - 1) % p.group;
@@ -69,12 +55,8 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     sees(p, s.len, s.len - s.n + qi, lo, hi);
     // what the tile's first and last query see: the range to visit, and the part that every query sees
     int lo_a, hi_a, lo_z, hi_z;
-    sees(p, s.len, s.len - s.n + ct * 16 / p.group, lo_a, hi_a);
-    sees(p, s.len, s.len - s.n + min(ct * 16 + 15, cols - 1) / p.group, lo_z, hi_z);
-    if (p.wgs == 0) {
-        t0 = lo_a >> 6;
-        te = (hi_z + 63) >> 6;
-    }
+    sees_uni(p, s.len, s.len - s.n + ct * 16 / p.group, lo_a, hi_a);
+    sees_uni(p, s.len, s.len - s.n + min(ct * 16 + 15, cols - 1) / p.group, lo_z, hi_z);
 
     // Q^T operand: k-step 2 s + h covers dims 64 s + 16 g + 8 h .. + 7 of lane group g - the order of the K loads
     uint4 qf[QP][KS];
@@ -106,7 +88,7 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     f32x4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
+    float m = NEVER, l = 0.f;
     const int page = 1 << p.pshift, kblk = (lane >> 2) & 3;
     const size_t page_bytes = (size_t)page * HD, head_off = (size_t)hk * page_bytes, stride = (size_t)p.kv * page_bytes;
     const int32_t* tab = p.table + (size_t)b * p.ldt;
@@ -182,19 +164,18 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, y[e]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        if (__any(mx > m + 15.f)) {      // first tile: m = -inf
+        if (__any(mx > m + 15.f)) {
             const float mn = mx > m + 15.f ? mx - 7.f : m;      // each query by itself: its result does not depend on its neighbours
-            const float al = m == -INFINITY ? 0.f : exp2_(m - mn);
+            const float al = exp2_(m - mn);
             l *= al;
 #pragma unroll
             for (int d = 0; d < ND; ++d) o[d] *= al;
             m = mn;
         }
-        const float mr = m == -INFINITY ? 0.f : m;      // nothing seen yet: every y is -inf
         float ls = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            y[e] = exp2_(y[e] - mr);
+            y[e] = exp2_(y[e] - m);
             ls += y[e];
         }
         l += ls * __uint_as_float((uint32_t)(127 - (int)ev) << 23);      // P / vs
@@ -275,12 +256,11 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     float mm = sm[0][col];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w][col]);
-    const float al = m == -INFINITY ? 0.f : exp2_(m - mm);
-    if (g == 0) sl[wave][col] = m == -INFINITY ? l : l * al;      // (an all-NaN column keeps its NaN sum)
+    const float al = exp2_(m - mm);
+    if (g == 0) sl[wave][col] = l * al;
 #pragma unroll
     for (int d = 0; d < ND; ++d) {
-        const f32x4 v = m == -INFINITY ? o[d] : o[d] * al;
-        *reinterpret_cast<f32x4*>(&so[wave][col][16 * d + 4 * g]) = v;
+        *reinterpret_cast<f32x4*>(&so[wave][col][16 * d + 4 * g]) = o[d] * al;
     }
     __syncthreads();
     // thread: column tid / 16, HD / 16 consecutive dims
@@ -295,91 +275,97 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
 #pragma unroll
         for (int e = 0; e < PD; ++e) f[e] += so[w][c2][d2 + e];
     }
-    if (p.wgs == 0) {
-        if (qc2 < cols) {
-            const int qi2 = qc2 / p.group, head2 = hk * p.group + qc2 % p.group;
-            const float inv = lt == 0.f ? 0.f : 1.f / lt;      // a row that sees nothing is zero
-            T* op = (T*)p.out + (s.r0 + qi2) * p.ldo + head2 * HD + d2;
+    if (qc2 < cols && whole) {
+        const int qi2 = qc2 / p.group, head2 = hk * p.group + qc2 % p.group;
+        const float inv = lt == 0.f ? 0.f : 1.f / lt;      // a row that sees nothing is zero
+        T* op = (T*)p.out + (s.r0 + qi2) * p.ldo + head2 * HD + d2;
 #pragma unroll
-            for (int e = 0; e < PD; ++e) f[e] = lt == 0.f ? 0.f : f[e] * inv;
+        for (int e2 = 0; e2 < PD; ++e2) f[e2] = lt == 0.f ? 0.f : f[e2] * inv;
 #pragma unroll
-            for (int e = 0; e < PD; e += 4) store4(op + e, f + e);
-        }
-        return;
-    }
-    if (qc2 < cols) {
-        float* w = p.po + ((size_t)slot * 16 + c2) * HD + d2;
+        for (int e2 = 0; e2 < PD; e2 += 4) store4(op + e2, f + e2);
+    } else if (qc2 < cols) {
+        const size_t at = ((size_t)blockIdx.x + e) * 16 + c2;
 #pragma unroll
-        for (int e = 0; e < PD; e += 4) store4(w + e, f + e);
+        for (int e2 = 0; e2 < PD; e2 += 4) store4(p.po + at * HD + d2 + e2, f + e2);
         if ((tid & 15) == 0) {
             float mm2 = sm[0][c2];
 #pragma unroll
             for (int k = 1; k < NW; ++k) mm2 = fmaxf(mm2, sm[k][c2]);
-            store2(p.pml + ((size_t)slot * 16 + c2) * 2, mm2, lt);
+            store2(p.pml + at * 2, mm2, lt);
         }
     }
     pos += te - t0;
     if (pos >= pos_end) return;
-    if (pos - before >= units) {
-        before += units;
-        ++b;
-    }
+    before += sg.tiles;
+    ++e;
     __syncthreads();
     }
 }
 
-// out = the pieces' results against their common reference.  One workgroup per (sequence, token, head): HD / 4 threads hold the row, the
-// rest of the 256 take other pieces, four loads in flight each.
+// out = the pieces' results against their common reference, for the segments that were cut (and zeros where nothing is seen).  A workgroup
+// takes ROWS rows of a segment: HD / 4 threads hold a row, and with ROWS = 1 the rest take other pieces, four loads in flight each.
 constexpr int MAX_WGS = 768;
-template <typename T, int HD> __global__ __launch_bounds__(64 * NW) void kv_attn_join_kernel(const AttnP p) {
-    constexpr int LP = HD / 4, NS = 64 * NW / LP;
-    __shared__ float al[MAX_WGS];
-    __shared__ f32x4 so[NS][LP];
-    __shared__ float sm[NW], sl[NW];
+template <typename T, int HD, int ROWS> __global__ __launch_bounds__(256) void kv_attn_join_kernel(const AttnP p) {
+    constexpr int LP = HD / 4, NS = 256 / (LP * ROWS);
+    static_assert(LP * ROWS * NS == 256 && (NS == 1 || ROWS == 1), "either rows or pieces side by side");
     __shared__ int red[8];
-    int id = blockIdx.x;
-    const int head = id % p.heads; id /= p.heads;
-    const int qi = id % p.max_new, b = id / p.max_new, tid = threadIdx.x;
-    const Seq s = seq_of(p, b);
-    if (qi >= s.n) return;
-    int before, first, nct;
-    const Line line = line_of<NW>(p, b, before, red);
-    const int tiles = seq_tiles(p, s, first, nct);
-    const int qc = qi * p.group + head % p.group, ct = qc >> p.cshift, hk = head / p.group;
-    const int begin = before + (hk * nct + ct) * tiles;      // this column tile's part of the line, and the workgroups that hold some of it
-    const int w0 = begin / line.share, n = tiles > 0 ? (begin + tiles - 1) / line.share - w0 + 1 : 0;
-    const size_t slot = (size_t)w0 + (size_t)(b * p.kv + hk) * p.nct + ct;      // the next workgroup's is the next slot
-    const float2* ml = reinterpret_cast<const float2*>(p.pml) + (slot << p.cshift) + (qc & ((1 << p.cshift) - 1));
-    float m = -INFINITY, l = 0.f;
-    for (int i = tid; i < n; i += 64 * NW) m = fmaxf(m, ml[(size_t)i << p.cshift].x);
-    m = wave_max(m);
-    if ((tid & 63) == 0) sm[tid >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    for (int i = tid; i < n; i += 64 * NW) {
-        const float2 w = ml[(size_t)i << p.cshift];
-        const float a = w.x == -INFINITY ? 1.f : exp2_(w.x - m);      // a piece in which this query saw nothing holds zeros (or NaN)
-        al[i] = a;
-        l += w.y * a;
-    }
-    l = wave_sum(l);
-    if ((tid & 63) == 0) sl[tid >> 6] = l;
-    __syncthreads();
-    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-    const int c = tid % LP, k = tid / LP;
-    const f32x4* po = reinterpret_cast<const f32x4*>(p.po + ((slot << p.cshift) + (qc & ((1 << p.cshift) - 1))) * HD) + c;
+    const int tid = threadIdx.x, chunks = p.jrows / ROWS;
+    const int e = blockIdx.x / chunks, r0 = blockIdx.x % chunks * ROWS;
+    const Segment sg = segment_of(p, e);
+    const Seq s = seq_of(p, sg.b);
+    const int c0 = (sg.ct << p.cshift) + r0, cols = s.n * p.group;
+    if (c0 >= cols) return;
+    int before;
+    const Line line = line_of<4>(p, e, before, red);
+    const int w0 = before / line.share, n = sg.tiles > 0 ? (before + sg.tiles - 1) / line.share - w0 + 1 : 0;
+    if (n == 1) return;
+    const int c = tid % LP, row = ROWS > 1 ? tid / LP : 0, qc = c0 + row;
+    const size_t at = (((size_t)w0 + e) << p.cshift) + r0 + row;      // the next piece is in the next slot
+    const float2* ml = reinterpret_cast<const float2*>(p.pml) + at;
+    const f32x4* po = reinterpret_cast<const f32x4*>(p.po + at * HD) + c;
+    float l = 0.f, m = NEVER;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+    if constexpr (ROWS > 1) {
+        if (qc >= cols) return;
+        for (int i = 0; i < n; ++i) m = fmaxf(m, ml[(size_t)i << p.cshift].x);
+        for (int i = 0; i < n; ++i) {
+            const float2 w = ml[(size_t)i << p.cshift];
+            const float a = exp2_(w.x - m);
+            l += w.y * a;
+            o += po[((size_t)i << p.cshift) * LP] * a;
+        }
+    } else {
+        __shared__ float al[MAX_WGS];
+        __shared__ f32x4 so[NS][LP];
+        __shared__ float sm[4], sl[4];
+        for (int i = tid; i < n; i += 256) m = fmaxf(m, ml[(size_t)i << p.cshift].x);
+        m = wave_max(m);
+        if ((tid & 63) == 0) sm[tid >> 6] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+        for (int i = tid; i < n; i += 256) {
+            const float2 w = ml[(size_t)i << p.cshift];
+            const float a = exp2_(w.x - m);
+            al[i] = a;
+            l += w.y * a;
+        }
+        l = wave_sum(l);
+        if ((tid & 63) == 0) sl[tid >> 6] = l;
+        __syncthreads();
+        l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+        const int k = tid / LP;
 #pragma unroll 4
-    for (int i = k; i < n; i += NS) o += po[((size_t)i << p.cshift) * LP] * al[i];
-    so[k][c] = o;
-    __syncthreads();
-    if (k) return;
+        for (int i = k; i < n; i += NS) o += po[((size_t)i << p.cshift) * LP] * al[i];
+        so[k][c] = o;
+        __syncthreads();
+        if (k) return;
 #pragma unroll
-    for (int i = 1; i < NS; ++i) o += so[i][c];
+        for (int i = 1; i < NS; ++i) o += so[i][c];
+    }
     float f[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = l == 0.f ? 0.f : o[e] / l;
-    store4((T*)p.out + (s.r0 + qi) * p.ldo + head * HD + 4 * c, f);
+    for (int q = 0; q < 4; ++q) f[q] = l == 0.f ? 0.f : o[q] / l;
+    store4((T*)p.out + (s.r0 + qc / p.group) * p.ldo + (sg.hk * p.group + qc % p.group) * HD + 4 * c, f);
 }
 
 // How a call is run: column tiles of 16 (this file) or 256 (kv_attention_rows.hip), and the workgroups that share the work
@@ -390,7 +376,7 @@ struct Way {
 Way way_of(int dtype, int B, int max_new, int kv, int group, int hd, int width, int pshift, int causal, int window) {
     Way w;
     const int64_t cols = (int64_t)max_new * group;
-    w.cshift = dtype != PGT_F32 && cols >= 64 ? (hd == 64 ? 8 : 7) : 4;
+    w.cshift = dtype != PGT_F32 && cols >= 64 ? 8 : 4;
     w.segs = (size_t)B * kv * ((cols + (1 << w.cshift) - 1) >> w.cshift);
     int64_t tiles = (((int64_t)width << pshift) + 63) / 64;
     if (causal && window) {      // from the first query's first token to the last one's last
@@ -398,8 +384,8 @@ Way way_of(int dtype, int B, int max_new, int kv, int group, int hd, int width, 
         if (n < tiles) tiles = n;
     }
     if (w.cshift != 4) {
-        w.wgs = 512;
-        if (w.segs >= 192 || tiles <= MIN_SHARE) w.wgs = 0;
+        w.wgs = 256;
+        if (w.segs >= 4096 || tiles <= MIN_SHARE) w.wgs = 0;
     } else {
         // as many as run at once (hd 64: 3 per CU, 128: 2), or one per column tile, without a join, where no sequence can be longer than
         // 16 tiles or there are so many column tiles that the chip is full anyway
@@ -453,8 +439,9 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     p.cshift = w.cshift;
     p.nct = (max_new * p.group + (1 << w.cshift) - 1) >> w.cshift;
     p.wgs = w.wgs;
-    const size_t wgs = w.wgs ? w.wgs : w.segs, rws = (size_t)B * max_new * heads;
-    PGT_CHECK(w.segs < (1ULL << 31) && rws < (1ULL << 31), "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
+    p.jrows = w.cshift == 4 && max_new * p.group < 16 ? max_new * p.group : 1 << w.cshift;
+    const size_t wgs = w.wgs ? w.wgs : w.segs;
+    PGT_CHECK(w.segs < (1ULL << 31), "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
     if (w.wgs) {
         PGT_CHECK((double)w.segs * (((int64_t)width << p.pshift) / 64 + 1) < 2147483648.0,
                   "kv_attention: %d sequences of up to %d pages of %d tokens exceed one launch", B, width, page);
@@ -472,7 +459,8 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
         if (w.cshift != 4) {}                                                                                         \
         else if (p.nct == 1) hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, true>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p); \
         else hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, false>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);      \
-        if (p.wgs) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)rws), dim3(64 * NW), 0, st, p);   \
+        if (p.wgs && w.cshift == 4) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_, 1>), dim3((unsigned)(w.segs * p.jrows)), dim3(256), 0, st, p); \
+        else if (p.wgs) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_, 1024 / HD_>), dim3((unsigned)(w.segs * (HD_ / 4))), dim3(256), 0, st, p); \
     } while (0)
 #define ATTN_HD(TT)                                                                                                   \
     do {                                                                                                              \

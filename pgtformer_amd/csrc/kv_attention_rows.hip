@@ -1,11 +1,12 @@
 // Attention over the paged 8-bit cache for many query rows (a prompt's chunk, whole frames): kv_attention.hip has the mathematics.
 //
-// 32x32x16 MFMA, swapped (S^T = K Q^T, O^T += V^T P^T); a wave holds 64 query columns, a workgroup of 4 waves 256.  Per tile of 64 tokens the
-// workgroup turns the codes into 16-bit operands ONCE, into LDS: 256 columns share one conversion, and every 1 KiB operand read feeds two
-// matrix instructions (read per wave from the cache, conversion and loads cost as many cycles as the products).  The images are in operand
-// order - K: 8 dims x 64 tokens, the tokens permuted so that a lane's 16 scores belong to one 16-token block (one scale) and are the 16
-// tokens its V operand holds; V: 8 tokens x hd dims - all reads and writes are 16 bytes per lane without conflicts.  Three stages: the
-// scores of the next 32 tokens are multiplied while the softmax of the current ones runs, across the tile boundary, one barrier per tile.
+// 32x32x16 MFMA, swapped (S^T = K Q^T, O^T += V^T P^T); a wave holds 32 query columns, a workgroup of 8 waves 256.  What bounds it is the
+// vector work beside the products (per 32 x 32 scores: 512 cycles of products at hd 128, 16 exponentials with their scaling, sums and
+// conversions per lane), so everything else is kept away from the waves: per tile of 64 tokens the workgroup turns the codes into 16-bit
+// operands ONCE, into LDS, for all its columns.  The images are in operand order - K: 8 dims x 64 tokens, the tokens permuted so that a
+// lane's 16 scores belong to one 16-token block (one scale) and are the 16 tokens its V operand holds; V: 8 tokens x hd dims - all reads
+// and writes are 16 bytes per lane.  Three stages: the scores of the next 32 tokens are multiplied while the softmax of the current ones
+// runs, across the tile boundary, one barrier per tile; every product has a slice of vector work behind it, fixed by hand.
 #include "kv_attention.h"
 
 #include "pgt_internal.h"
@@ -24,375 +25,292 @@ __device__ __forceinline__ float max_of_halves(float v) {
     return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
 }
 
-template <typename T, int HD, int NQ, int NW> __global__ __launch_bounds__(64 * NW, 2) void kv_attn_rows_kernel(const AttnP p) {
+constexpr int NW = 8, TH = 64 * NW, CT = 32 * NW;      // waves, threads and columns of a workgroup
+
+template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_rows_kernel(const AttnP p) {
     constexpr bool HQ = __is_same(T, half_t);
-    constexpr int KS = HD / 16, ND = HD / 32;              // k-steps of S^T, row blocks of O^T
-    constexpr int CW = 32 * NQ, TH = 64 * NW, CT = CW * NW;      // columns of a wave; threads and columns of the workgroup
-    constexpr int UN = HD / 64;                            // 16-byte units per thread of K (and of V) per tile
-    static_assert(NW == 4, "a wave stages one of the four blocks of a tile");
-    constexpr int KB = 64 * HD * 2, STAGE = 2 * KB;        // bytes of a K image; of a stage
-    __shared__ __attribute__((aligned(16))) char smem[2 * STAGE];
-    __shared__ float2 sscale[2][4];                        // per 16-token block: score factor (negative: no page), log2 of the V scale
-    __shared__ int nans;                                   // a V code in the range stands for NaN
+    constexpr int KS = HD / 16, ND = HD / 32, NV = 2 * ND;      // products of S^T; row blocks of O^T, its products
+    constexpr int KB = 64 * HD * 2, STAGE = 2 * KB;             // bytes of a K image; of a stage
+    __shared__ __attribute__((aligned(16))) char smem[3 * STAGE];
+    __shared__ float4 sscale[3][4];                             // per 16-token block: score factor (negative: no page), log2 vs, 1 / vs
     __shared__ int red[2 * NW];
+    __shared__ int nans;                                        // a V code in the range stands for NaN
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
     const int page = 1 << p.pshift;
     const size_t page_bytes = (size_t)page * HD, stride = (size_t)p.kv * page_bytes;
 
-    int b, before = 0, pos = 0, pos_end = 0, id = 0;
-    if (p.wgs == 0) {
-        // column tiles of one (sequence, kv head) read the same pages: a contiguous run of ids per XCD (dispatch is round-robin over 8)
-        const int nblk = gridDim.x, xcd = blockIdx.x & 7, q8 = nblk >> 3, r8 = nblk & 7;
-        id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
-        b = id / (p.nct * p.kv);
-    } else {
+    // segments of one (sequence, kv head) read the same pages: a contiguous run of them per XCD (dispatch is round-robin over 8)
+    const int nblk = gridDim.x, xcd = blockIdx.x & 7, q8 = nblk >> 3, r8 = nblk & 7;
+    const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
+    int e = id, before = 0, pos = 0, pos_end = 0;
+    if (p.wgs) {
         const Line line = line_of<NW>(p, 0, before, red);
-        pos = blockIdx.x * line.share;
+        pos = id * line.share;
         pos_end = min(pos + line.share, line.total);
         if (pos >= pos_end) return;
-        locate<NW>(p, pos, b, before, red);
+        locate<NW>(p, pos, e, before, red);
     }
-    for (;;) {
-        const Seq s = seq_of(p, b);
-        const int cols = s.n * p.group;
-        int ct, hk, t0, te, slot = 0, units = 0;
-        if (p.wgs == 0) {
-            ct = p.nct - 1 - id % p.nct;      // the later queries see more: first
-            hk = id / p.nct % p.kv;
-            t0 = te = 0;
-            if (ct * CT >= cols) return;
-        } else {
-            int nct, first;
-            const int tiles = seq_tiles(p, s, first, nct);
-            units = tiles * nct * p.kv;
-            if (units == 0) { ++b; continue; }
-            const int i = (pos - before) / tiles, off = pos - before - i * tiles;
-            ct = i % nct;
-            hk = i / nct;
-            t0 = first + off;
-            te = first + min(off + pos_end - pos, tiles);
-            slot = blockIdx.x + (b * p.kv + hk) * p.nct + ct;
-        }
-        const int shift = s.len - s.n;
-        if (p.wgs == 0) {
-            int lo, hi, dummy;
-            sees(p, s.len, shift + ct * CT / p.group, lo, dummy);
-            sees(p, s.len, shift + min(ct * CT + CT - 1, cols - 1) / p.group, dummy, hi);
-            t0 = lo >> 6;
-            te = (hi + 63) >> 6;
-        }
+    for (;;) {      // the segments that this workgroup's part of the line touches
+        const Segment sg = uni(segment_of(p, e));
+        if (p.wgs && sg.tiles == 0) { ++e; continue; }
+        const int b = sg.b, hk = sg.hk, ct = sg.ct;
+        const Seq s = uni(seq_of(p, b));
+        const int cols = s.n * p.group, shift = s.len - s.n;
+        if (ct * CT >= cols) return;
+        const int t0 = sg.first + (p.wgs ? pos - before : 0), te = p.wgs ? sg.first + min(pos_end - before, sg.tiles) : sg.first + sg.tiles;
+        const bool whole = te - t0 == sg.tiles;
         // this wave's columns: what every one of them sees, and what any of them does
-        const int cw = ct * CT + wave * CW;
+        const int cw = ct * CT + wave * 32;
         int lo_a = 0, hi_a = 0, lo_z = 0, hi_z = 0;      // a wave without columns sees nothing
         if (cw < cols) {
-            sees(p, s.len, shift + cw / p.group, lo_a, hi_a);
-            sees(p, s.len, shift + min(cw + CW - 1, cols - 1) / p.group, lo_z, hi_z);
+            sees_uni(p, s.len, shift + cw / p.group, lo_a, hi_a);
+            sees_uni(p, s.len, shift + min(cw + 31, cols - 1) / p.group, lo_z, hi_z);
         }
-        uint4 qf[NQ][KS];
-        int lo[NQ], hi[NQ];
-        const uint32_t flip = p.c < 0.f ? 0x80008000u : 0u;      // a negative scale goes into q: the largest score stays the largest weight
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const int qc = min(cw + n * 32 + r, cols - 1), qi = qc / p.group;
-            sees(p, s.len, shift + qi, lo[n], hi[n]);
-            const T* qp = (const T*)p.q + (s.r0 + qi) * p.ldq + (hk * p.group + qc % p.group) * HD + 8 * h;
+        int all_lo, all_hi, dummy;                       // what all columns of the workgroup see
+        sees_uni(p, s.len, shift + ct * CT / p.group, dummy, all_hi);
+        sees_uni(p, s.len, shift + min(ct * CT + CT - 1, cols - 1) / p.group, all_lo, dummy);
+        const int qc = min(cw + r, cols - 1);
+        int lo, hi;
+        sees(p, s.len, shift + qc / p.group, lo, hi);
+        uint4 qf[KS];
+        {
+            const uint32_t flip = p.c < 0.f ? 0x80008000u : 0u;      // a negative scale goes into q: the largest score stays the largest weight
+            const T* qp = (const T*)p.q + (s.r0 + qc / p.group) * p.ldq + (hk * p.group + qc % p.group) * HD + 8 * h;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
                 uint4 w = *reinterpret_cast<const uint4*>(qp + 16 * k);
                 w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
-                qf[n][k] = w;
+                qf[k] = w;
             }
         }
-        f32x16 o[NQ][ND];
-        float m[NQ], l[NQ];
+        f32x16 o[ND];
+        float m = NEVER, l = 0.f;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            m[n] = -INFINITY;
-            l[n] = 0.f;
-#pragma unroll
-            for (int d = 0; d < ND; ++d)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[n][d][e] = 0.f;
-        }
+        for (int d = 0; d < ND; ++d) o[d] = zero16();
 
-        // Staging: wave w brings block w (16 tokens) of a tile, so page and scales are the wave's: lane -> K (token lane & 15, chunks lane / 16
-        // + 4 i), V (dims lane + 64 i).  Page numbers run one tile ahead of the loads, the loads one tile ahead of the conversion.
+        // Staging: a unit is 64 lanes x 16 bytes of one block (16 tokens): K 4 chunks of 16 dims (lane -> token lane & 15, chunk lane / 16), V 64 dims.
+        // hd 128: wave w brings unit w / 4 of K and of V of block w & 3; hd 64: waves 0-3 bring K, 4-7 V.  Page numbers run one tile ahead of
+        // the loads, the loads one tile ahead of the conversion.
+        constexpr bool BOTH = HD == 128;
+        const int blk = wave & 3, part = wave >> 2;
         const int32_t* tab = p.table + (size_t)b * p.ldt;
-        uint4 rk[UN], rv[UN];
+        uint4 rk, rv;
         int rpage, nextpage;
         float rsk, rsv;
-        auto page_at = [&](int t, int blk) {
-            const int i = (t * 64 + 16 * blk) >> p.pshift;
+        auto page_at = [&](int t, int k) {
+            const int i = (t * 64 + 16 * k) >> p.pshift;
             return t < te && i < p.width ? tab[i] : -1;
         };
         auto ok = [&](int i) { return i >= 0 && i < p.pages; };
-        const uint32_t k_at = (uint32_t)((lane >> 4) * page + (lane & 15)) * 16, k_step = (uint32_t)page * 64, v_at = (uint32_t)lane * 16;
+        const uint32_t k_at = (uint32_t)((lane >> 4) * page + (lane & 15)) * 16 + (BOTH ? (uint32_t)(part * 4 * page * 16) : 0u);
+        const uint32_t v_at = (uint32_t)(lane + (BOTH ? 64 * part : 0)) * 16;
         auto load_raw = [&](int t) {      // of page nextpage
             rpage = __builtin_amdgcn_readfirstlane(nextpage);
-            const int id = ok(rpage) ? rpage : 0;
-            const int tok = (t * 64 + 16 * wave) & (page - 1);
-            const uint8_t *kb = p.kp + id * stride + hk * page_bytes + tok * 16, *vb = p.vp + id * stride + hk * page_bytes + (size_t)tok * HD;
-#pragma unroll
-            for (int i = 0; i < UN; ++i) rk[i] = *reinterpret_cast<const uint4*>(kb + (k_at + k_step * i));
-#pragma unroll
-            for (int i = 0; i < UN; ++i) rv[i] = *reinterpret_cast<const uint4*>(vb + (v_at + 1024u * i));
-            rsk = p.ks[(size_t)id * p.kv + hk];
-            rsv = p.vs[(size_t)id * p.kv + hk];
+            const int pg = ok(rpage) ? rpage : 0;
+            const int tok = (t * 64 + 16 * blk) & (page - 1);
+            const size_t at = pg * stride + hk * page_bytes;
+            if (BOTH || part == 0) rk = *reinterpret_cast<const uint4*>(p.kp + at + tok * 16 + k_at);
+            if (BOTH || part == 1) rv = *reinterpret_cast<const uint4*>(p.vp + at + (size_t)tok * HD + v_at);
+            rsk = p.ks[(size_t)pg * p.kv + hk];
+            rsv = p.vs[(size_t)pg * p.kv + hk];
         };
         // token 16 hh + e of a 32-token half -> the row of S^T whose score ends up in register e of lane half hh
-        const int k_to = (((lane >> 4) * 2) * 64 + 32 * (wave >> 1) + (lane & 3) + 8 * ((lane & 15) >> 2) + 4 * (wave & 1)) * 16;
-        const int v_to = KB + (wave * 2 * HD + lane) * 16;
-        auto store = [&](int st) {
+        const int k_to = (((lane >> 4) + (BOTH ? 4 * part : 0)) * 128 + 32 * (blk >> 1) + (lane & 3) + 8 * ((lane & 15) >> 2) + 4 * (blk & 1)) * 16;
+        const int v_to = KB + (blk * 2 * HD + lane + (BOTH ? 64 * part : 0)) * 16;
+        auto store = [&](int st, int t) {
             char* d = smem + st * STAGE;
-#pragma unroll
-            for (int i = 0; i < UN; ++i) {      // (opaque: or the compiler regroups the registers right behind the loads, and waits for them there)
-                x3_opaque(rk[i]);
-                x3_opaque(rv[i]);
+            x3_opaque(rk);      // (or the compiler regroups the registers right behind the loads, and waits for them there)
+            x3_opaque(rv);
+            if (BOTH || part == 0) {
+                *reinterpret_cast<uint4*>(d + k_to) = HQ ? half8(rk.x, rk.y) : bfloat8(rk.x, rk.y);
+                *reinterpret_cast<uint4*>(d + k_to + 1024) = HQ ? half8(rk.z, rk.w) : bfloat8(rk.z, rk.w);
             }
-#pragma unroll
-            for (int i = 0; i < UN; ++i) {
-                const uint4 w = rk[i];
-                *reinterpret_cast<uint4*>(d + k_to + i * 8192) = HQ ? half8(w.x, w.y) : bfloat8(w.x, w.y);
-                *reinterpret_cast<uint4*>(d + k_to + i * 8192 + 1024) = HQ ? half8(w.z, w.w) : bfloat8(w.z, w.w);
-            }
-#pragma unroll
-            for (int i = 0; i < UN; ++i) {
-                const uint4 w = rv[i];
-                *reinterpret_cast<uint4*>(d + v_to + i * 1024) = half8(w.x, w.y);
-                *reinterpret_cast<uint4*>(d + v_to + i * 1024 + HD * 16) = half8(w.z, w.w);
-            }
-            uint32_t bad = 0;
-#pragma unroll
-            for (int i = 0; i < UN; ++i) bad |= nan_bytes(rv[i].x) | nan_bytes(rv[i].y) | nan_bytes(rv[i].z) | nan_bytes(rv[i].w);
-            if (__any(bad != 0)) {      // NaN times the weight 0 of a query that does not see the token: zeros here, see the end
-                nans = 1;
-#pragma unroll
-                for (int i = 0; i < UN; ++i) {
-                    const uint4 w = rv[i];
-                    auto clean = [](uint32_t v) { return v & ~((nan_bytes(v) >> 7) * 255u); };
-                    *reinterpret_cast<uint4*>(d + v_to + i * 1024) = half8(clean(w.x), clean(w.y));
-                    *reinterpret_cast<uint4*>(d + v_to + i * 1024 + HD * 16) = half8(clean(w.z), clean(w.w));
+            if (BOTH || part == 1) {
+                uint4 w = rv;
+                if ((t * 64 < all_lo) | (t * 64 + 64 > all_hi)) {
+                    // NaN times the weight 0 of a query that does not see the token: zeros here, see the end
+                    const uint4 n = make_uint4(nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w));
+                    if (__any((n.x | n.y | n.z | n.w) != 0)) nans = 1;
+                    w.x &= ~((n.x >> 7) * 255u); w.y &= ~((n.y >> 7) * 255u); w.z &= ~((n.z >> 7) * 255u); w.w &= ~((n.w >> 7) * 255u);
                 }
+                *reinterpret_cast<uint4*>(d + v_to) = half8(w.x, w.y);
+                *reinterpret_cast<uint4*>(d + v_to + HD * 16) = half8(w.z, w.w);
             }
-            if (lane == 0)      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
-                sscale[st][wave] = make_float2(ok(rpage) ? fmaxf(fabsf(p.c) * rsk, 1e-30f) : -1.f, (float)((int)((__float_as_uint(rsv) >> 23) & 255) - 127));
+            if (lane == 0 && part == 0) {      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
+                const int ev = (int)((__float_as_uint(rsv) >> 23) & 255) - 127;
+                sscale[st][blk] = make_float4(ok(rpage) ? fmaxf(fabsf(p.c) * rsk, 1e-30f) : -1.f, (float)ev, __uint_as_float((uint32_t)(127 - ev) << 23), 0.f);
+            }
         };
         auto k_operand = [&](int st, int sb, int k) {
-            return *reinterpret_cast<const uint4*>(smem + st * STAGE + (sb * 32 + r + 64 * h) * 16 + k * 2 * 64 * 16);
+            return *reinterpret_cast<const uint4*>(smem + st * STAGE + (sb * 32 + r + 64 * h) * 16 + k * 2048);
         };
         auto v_operand = [&](int st, int sb, int i) {      // i = k-step * ND + row block
             return *reinterpret_cast<const uint4*>(smem + st * STAGE + KB + ((sb * 2 + h) * 2 * HD + r) * 16 + ((i / ND) * HD + (i % ND) * 32) * 16);
         };
-        float2 sc = make_float2(1.f, 0.f);      // of the current scores: factor and log2 of the V scale of this lane's 16 tokens
-        float tm[NQ];                           // largest of a query's current scores, in units of the exponent
-        auto top = [&](const f32x16 (&x)[NQ], int n) {
-            float mx = x[n][0];
+        float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);      // of the current scores: sscale of this lane's 16 tokens
+        float tm = NEVER;                                 // the largest of them, in units of the exponent
+        auto top = [&](const f32x16& x) {
+            float mx = x[0];
 #pragma unroll
-            for (int e = 1; e < 16; ++e) mx = fmaxf(mx, x[n][e]);
+            for (int k = 1; k < 16; ++k) mx = fmaxf(mx, x[k]);
             return max_of_halves(__builtin_fmaf(mx, fabsf(sc.x), sc.y));
         };
-        // the scores of half sb of stage st
-        auto scores = [&](int st, int sb, f32x16 (&x)[NQ]) {
+        auto scores = [&](int st, int sb, f32x16& x) {
 #pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const uint4 a = k_operand(st, sb, k);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) x[n] = mma16<T>(a, qf[n][k], k == 0 ? zero16() : x[n]);
-            }
+            for (int k = 0; k < KS; ++k) x = mma16<T>(k_operand(st, sb, k), qf[k], k == 0 ? zero16() : x);
             sc = sscale[st][sb * 2 + h];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) tm[n] = top(x, n);
+            tm = top(x);
         };
-        // softmax of the scores x of half sb of tile t (stage st) and their product with V; xn = the scores of half nsb of stage nst (behind
-        // the last tile: of whatever is there, unused).  The order is fixed by hand (nothing moves over a SLICE): behind every product a slice of
-        // vector work that takes about as long, operands read four products ahead.
+        // softmax of the scores x of half sb of tile t (stage st) and their product with V; xn = the scores of half nsb of stage nst (behind the
+        // last tile: of whatever is there, unused).  Nothing moves over a SLICE; operands are read four products ahead.
 #define SLICE() __builtin_amdgcn_sched_barrier(0)
-        auto step = [&](int t, int st, int sb, int nst, int nsb, f32x16 (&x)[NQ], f32x16 (&xn)[NQ]) {
+        auto step = [&](int t, int st, int sb, int nst, int nsb, f32x16& x, f32x16& xn) {
             const int tok = t * 64 + sb * 32;
             if (tok >= hi_z || tok + 32 <= lo_a) {
-                scores(nst, nsb, xn);
+                if (cw < cols) scores(nst, nsb, xn);
                 return;
             }
-            const float ck = fabsf(sc.x), ev = sc.y;
-            const int missing = __any(sc.x < 0.f);
-            if ((tok < lo_z) | (tok + 32 > hi_a) | (missing != 0)) {
+            const float ck = fabsf(sc.x), ev = sc.y, back = sc.z;
+            if ((tok < lo_z) | (tok + 32 > hi_a) | (__any(sc.x < 0.f) != 0)) {
+                const uint32_t span = sc.x < 0.f ? 0u : (uint32_t)(hi - lo);
+                const int at = tok + 16 * h - lo;
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    const uint32_t span = sc.x < 0.f ? 0u : (uint32_t)(hi[n] - lo[n]);
-                    const int at = tok + 16 * h - lo[n];
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) x[n][e] = (uint32_t)(at + e) < span ? x[n][e] : -INFINITY;
-                    tm[n] = top(x, n);
-                }
+                for (int k = 0; k < 16; ++k) x[k] = (uint32_t)(at + k) < span ? x[k] : -INFINITY;
+                tm = top(x);
             }
-            bool up = false;
+            if (__any(tm > m + 15.f)) {
+                const float mn = tm > m + 15.f ? tm - 7.f : m;      // each query by itself: its result does not depend on its neighbours
+                const float al = exp2_(m - mn);
+                l *= al;
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) up |= tm[n] > m[n] + 15.f;
-            if (__any(up)) {
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    const float mn = tm[n] > m[n] + 15.f ? tm[n] - 7.f : m[n];
-                    const float al = m[n] == -INFINITY ? 0.f : exp2_(m[n] - mn);
-                    l[n] *= al;
-#pragma unroll
-                    for (int d = 0; d < ND; ++d) o[n][d] *= al;
-                    m[n] = mn;
-                }
+                for (int d = 0; d < ND; ++d) o[d] *= al;
+                m = mn;
             }
-            const float back = __uint_as_float((uint32_t)(127 - (int)ev) << 23);      // 1 / vs
-            float em[NQ], ls[NQ];
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                em[n] = ev - (m[n] == -INFINITY ? 0.f : m[n]);
-                ls[n] = 0.f;
-            }
-            uint32_t pw[NQ][8];
-            auto weight2 = [&](int n, int i) {      // weights 2 i, 2 i + 1 of query block n
-                const float a = exp2_(__builtin_fmaf(x[n][2 * i], ck, em[n])), b = exp2_(__builtin_fmaf(x[n][2 * i + 1], ck, em[n]));
-                ls[n] += a;
-                ls[n] += b;
-                pw[n][i] = f2h2_nosat(a, b);
+            const float em = ev - m;
+            float ls = 0.f;
+            uint32_t pw[8];
+            const halfx2 ones = {(_Float16)1.f, (_Float16)1.f};
+            auto weight2 = [&](int i) {      // weights 2 i, 2 i + 1; their sum is that of the rounded ones, as the product's
+                pw[i] = f2h2_nosat(exp2_(__builtin_fmaf(x[2 * i], ck, em)), exp2_(__builtin_fmaf(x[2 * i + 1], ck, em)));
+                ls = __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, pw[i]), ones, ls, false);
             };
             uint4 f[4];      // operands in flight
 #pragma unroll
             for (int k = 0; k < 4; ++k) f[k] = k_operand(nst, nsb, k);
-            const float2 scn = sscale[nst][nsb * 2 + h];
+            const float4 scn = sscale[nst][nsb * 2 + h];
             SLICE();
-            // S^T of the next half; the weights of query block 0
 #pragma unroll
-            for (int i = 0; i < NQ * KS; ++i) {
-                const int k = i / NQ, n = i % NQ;
-                xn[n] = mma16<T>(f[k % 4], qf[n][k], k == 0 ? zero16() : xn[n]);
-                if (n == NQ - 1) {
-                    if (k + 4 < KS) f[k % 4] = k_operand(nst, nsb, k + 4);
-                    else f[k % 4] = v_operand(st, sb, k + 4 - KS);
-                }
-                weight2(0, i);
+            for (int k = 0; k < KS; ++k) {      // S^T of the next half, the weights
+                xn = mma16<T>(f[k % 4], qf[k], k == 0 ? zero16() : xn);
+                if (k + 4 < KS) f[k % 4] = k_operand(nst, nsb, k + 4);
+                else f[k % 4] = v_operand(st, sb, k + 4 - KS);
+#pragma unroll
+                for (int i = 0; i < 8 / KS; ++i) weight2(k * (8 / KS) + i);
                 SLICE();
             }
             sc = scn;
-            // O^T; the weights of query block 1, the largest of the next scores
-            float mx[NQ];
-            constexpr int NV = 2 * ND;      // products per query block
+            float mx = 0.f;
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
+            for (int i = 0; i < NV; ++i) {      // O^T, the largest of the next scores
+                const int k = i / ND, d = i % ND;
+                o[d] = mma16<half_t>(f[i % 4], make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]), o[d]);
+                if (i + 4 < NV) f[i % 4] = v_operand(st, sb, i + 4);
+                if (i == 0) mx = fmaxf(xn[0], xn[1]);
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    const int k = i / ND, d = i % ND;
-                    o[n][d] = mma16<half_t>(f[i % 4], make_uint4(pw[n][4 * k], pw[n][4 * k + 1], pw[n][4 * k + 2], pw[n][4 * k + 3]), o[n][d]);
-                    if (i + 4 < NV) f[i % 4] = v_operand(st, sb, i + 4);
-                    if (NQ == 2 && n == 0) {
-                        weight2(NQ - 1, 2 * i);
-                        weight2(NQ - 1, 2 * i + 1);
-                    } else {
-                        constexpr int PER = 16 / NV;
-#pragma unroll
-                        for (int q = 0; q < NQ; ++q) {
-                            if (i == 0) mx[q] = xn[q][0];
-#pragma unroll
-                            for (int e = 0; e < PER; ++e) mx[q] = fmaxf(mx[q], xn[q][PER * i + e]);
-                        }
-                    }
-                    SLICE();
-                }
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                l[n] = __builtin_fmaf(ls[n], back, l[n]);
-                tm[n] = max_of_halves(__builtin_fmaf(mx[n], fabsf(sc.x), sc.y));
+                for (int q = i == 0 ? 2 : 16 / NV * i; q < 16 / NV * (i + 1); ++q) mx = fmaxf(mx, xn[q]);
+                SLICE();
             }
+            l = __builtin_fmaf(ls, back, l);
+            tm = max_of_halves(__builtin_fmaf(mx, fabsf(sc.x), sc.y));
         };
 #undef SLICE
 
-        __syncthreads();      // the stages of the column tile before
+        __syncthreads();      // the stages of the segment before
         if (tid == 0) nans = 0;
         __syncthreads();
         if (t0 < te) {
-            nextpage = page_at(t0, wave);
+            nextpage = page_at(t0, blk);
             load_raw(t0);
-            nextpage = page_at(t0 + 1, wave);
-            store(0);
+            nextpage = page_at(t0 + 1, blk);
+            store(0, t0);
             if (t0 + 1 < te) load_raw(t0 + 1);
-            nextpage = page_at(t0 + 2, wave);
+            nextpage = page_at(t0 + 2, blk);
             __syncthreads();
-            f32x16 xa[NQ], xb[NQ];
-            scores(0, 0, xa);
+            f32x16 xa, xb;
+            if (cw < cols) scores(0, 0, xa);
             int st = 0;
-            for (int t = t0; t < te; ++t, st ^= 1) {
-                const bool more = t + 1 < te;
+            for (int t = t0; t < te; ++t) {
+                const int nst = st == 2 ? 0 : st + 1;
                 step(t, st, 0, st, 1, xa, xb);
-                __syncthreads();      // every wave is through with the other stage
-                if (more) {
-                    store(st ^ 1);
+                if (t + 1 < te) {      // (the stage was last read in tile t - 2, which every wave left before the last barrier)
+                    store(nst, t + 1);
                     if (t + 2 < te) load_raw(t + 2);
-                    nextpage = page_at(t + 3, wave);
+                    nextpage = page_at(t + 3, blk);
                 }
                 __syncthreads();
-                step(t, st, 1, st ^ 1, 0, xb, xa);
+                step(t, st, 1, nst, 0, xb, xa);
+                st = nst;
             }
         }
 
-        // columns cw + 32 n + r: rows 32 d + 8 q + 4 h + 0..3 of O^T are in registers 4 q .. 4 q + 3
+        // column cw + r: rows 32 d + 8 q + 4 h + 0..3 of O^T are in registers 4 q .. 4 q + 3
+        {
+            const float lt = l + __shfl_xor(l, 32, 64);
+            const int c = cw + r;
+            if (c < cols && whole) {
+                const float inv = lt == 0.f ? 0.f : 1.f / lt;      // a row that sees nothing is zero
+                T* op = (T*)p.out + (s.r0 + c / p.group) * p.ldo + (hk * p.group + c % p.group) * HD + 4 * h;
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            const float lt = l[n] + __shfl_xor(l[n], 32, 64);
-            const int qc = cw + n * 32 + r;
-            if (qc < cols) {
-                if (p.wgs == 0) {
-                    const float inv = lt == 0.f ? 0.f : 1.f / lt;
-                    T* op = (T*)p.out + (s.r0 + qc / p.group) * p.ldo + (hk * p.group + qc % p.group) * HD + 4 * h;
+                for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
+                    for (int q = 0; q < 4; ++q) {
+                        float f[4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            float f[4];
+                        for (int k = 0; k < 4; ++k) f[k] = lt == 0.f ? 0.f : o[d][4 * q + k] * inv;
+                        store4(op + 32 * d + 8 * q, f);
+                    }
+            } else if (c < cols) {
+                const size_t at = ((size_t)id + e) * CT + (c & (CT - 1));
+                float* w = p.po + at * HD + 4 * h;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) f[e] = lt == 0.f ? 0.f : o[n][d][4 * q + e] * inv;
-                            store4(op + 32 * d + 8 * q, f);
-                        }
-                } else {
-                    const size_t at = (size_t)slot * CT + (qc & (CT - 1));
-                    float* w = p.po + at * HD + 4 * h;
+                for (int d = 0; d < ND; ++d)
 #pragma unroll
-                    for (int d = 0; d < ND; ++d)
+                    for (int q = 0; q < 4; ++q) {
+                        float f[4];
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            float f[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) f[e] = o[n][d][4 * q + e];
-                            store4(w + 32 * d + 8 * q, f);
-                        }
-                    if (h == 0) store2(p.pml + at * 2, m[n], lt);
-                }
+                        for (int k = 0; k < 4; ++k) f[k] = o[d][4 * q + k];
+                        store4(w + 32 * d + 8 * q, f);
+                    }
+                if (h == 0) store2(p.pml + at * 2, m, lt);
             }
         }
-        // A V code that stands for NaN makes the outputs of exactly the queries that see its token NaN (and none by 0 * NaN)
-        __threadfence();
-        __syncthreads();
-        if (nans) {
-            for (int t = t0; t < te; ++t)
+        // A V code that stands for NaN, in a tile that not every column sees whole, makes the outputs of exactly the queries that see its token NaN
+        if (nans) {      // (the same in every thread: last written before the last barrier of the tiles)
+            __threadfence_block();
+            __syncthreads();
+            for (int t = t0; t < te; ++t) {
+                if (t * 64 >= all_lo && t * 64 + 64 <= all_hi) continue;
                 for (int u = tid; u < 4 * HD; u += TH) {
-                    const int blk = u / HD, dim = u % HD, tok = t * 64 + blk * 16, pg = page_at(t, blk);
+                    const int k = u / HD, dim = u % HD, tok = t * 64 + k * 16, pg = page_at(t, k);
                     if (!ok(pg)) continue;
                     const uint8_t* c = p.vp + pg * stride + hk * page_bytes + ((size_t)((tok & (page - 1)) >> 4) * HD + dim) * 16;
-                    for (int e = 0; e < 16; ++e) {
-                        if ((c[e] & 0x7f) != 0x7f) continue;
-                        for (int qc = ct * CT; qc < min(ct * CT + CT, cols); ++qc) {
+                    for (int i = 0; i < 16; ++i) {
+                        if ((c[i] & 0x7f) != 0x7f) continue;
+                        for (int q = ct * CT; q < min(ct * CT + CT, cols); ++q) {
                             int lq, hq;
-                            sees(p, s.len, shift + qc / p.group, lq, hq);
-                            if (tok + e < lq || tok + e >= hq) continue;
-                            if (p.wgs == 0) store_nan((T*)p.out + (s.r0 + qc / p.group) * p.ldo + (hk * p.group + qc % p.group) * HD + dim);
-                            else p.po[((size_t)slot * CT + (qc & (CT - 1))) * HD + dim] = __builtin_nanf("");
+                            sees(p, s.len, shift + q / p.group, lq, hq);
+                            if (tok + i < lq || tok + i >= hq) continue;
+                            if (whole) store_nan((T*)p.out + (s.r0 + q / p.group) * p.ldo + (hk * p.group + q % p.group) * HD + dim);
+                            else p.po[(((size_t)id + e) * CT + (q & (CT - 1))) * HD + dim] = __builtin_nanf("");
                         }
                     }
                 }
+            }
         }
-        if (p.wgs == 0) return;
         pos += te - t0;
         if (pos >= pos_end) return;
-        if (pos - before >= units) {
-            before += units;
-            ++b;
-        }
+        before += sg.tiles;
+        ++e;
     }
 }
 
@@ -400,8 +318,7 @@ template <typename T, int HD, int NQ, int NW> __global__ __launch_bounds__(64 * 
 
 int pgt_kv_attention_rows_launch(const void* pp, int bf16, int hd, unsigned groups, hipStream_t st) {
     const AttnP& p = *(const AttnP*)pp;
-#define ROWS_GO(TT, HD_)                                                                                                          \
-    hipLaunchKernelGGL((kv_attn_rows_kernel<TT, HD_, HD_ == 64 ? 2 : 1, 4>), dim3(groups), dim3(256), 0, st, p)
+#define ROWS_GO(TT, HD_) hipLaunchKernelGGL((kv_attn_rows_kernel<TT, HD_>), dim3(groups), dim3(TH), 0, st, p)
     if (bf16) {
         if (hd == 64) ROWS_GO(bf16_t, 64);
         else ROWS_GO(bf16_t, 128);
