@@ -42,6 +42,7 @@ struct AttnP {
     const float *ks, *vs;
     const int32_t *table, *lens, *cu;
     float *po, *pml;                  // partial results: (slot, columns, hd), (slot, columns, {m, l})
+    int2* ends;                       // per segment: the workgroups that hold its first and its last piece
     int64_t ldq, ldo;
     int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, cshift, nct, wgs, jrows, causal, window;      // column tiles of 2^cshift; wgs: workgroups that share the work, 0 = one per
                                       // column tile; jrows: rows of a column tile that the join looks at
@@ -124,31 +125,19 @@ __device__ __forceinline__ int wave_sum_i(int v) {
 struct Line {
     int total, share;
 };
-// the whole line, and the part of it before segment e (all 64 * W threads; red: 2 * W ints)
-template <int W> __device__ __forceinline__ Line line_of(const AttnP& p, int e, int& before, int* red) {
+// the whole line (all 64 * W threads; red: 2 * W ints)
+template <int W> __device__ __forceinline__ Line line_of(const AttnP& p, int* red) {
     const int segs = p.B * p.kv * p.nct;
-    int all = 0, pre = 0;
-    for (int i = threadIdx.x; i < segs; i += 64 * W) {
-        const int u = segment_of(p, i).tiles;
-        all += u;
-        if (i < e) pre += u;
-    }
+    int all = 0;
+    for (int i = threadIdx.x; i < segs; i += 64 * W) all += segment_of(p, i).tiles;
     all = wave_sum_i(all);
-    pre = wave_sum_i(pre);
-    if ((threadIdx.x & 63) == 0) {
-        red[threadIdx.x >> 6] = all;
-        red[W + (threadIdx.x >> 6)] = pre;
-    }
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = all;
     __syncthreads();
     Line l;
-    l.total = before = 0;
+    l.total = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) {
-        l.total += red[w];
-        before += red[W + w];
-    }
+    for (int w = 0; w < W; ++w) l.total += red[w];
     l.total = uni(l.total);
-    before = uni(before);
     l.share = uni(max((l.total + p.wgs - 1) / p.wgs, MIN_SHARE));
     return l;
 }

@@ -33,7 +33,7 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     __shared__ __attribute__((aligned(16))) float so[NW][16][HD + 4];
     int e = blockIdx.x, before = 0, pos = 0, pos_end = 0;
     if (p.wgs) {
-        const Line line = line_of<NW>(p, 0, before, red);
+        const Line line = line_of<NW>(p, red);
         pos = blockIdx.x * line.share;
         pos_end = min(pos + line.share, line.total);
         if (pos >= pos_end) return;
@@ -294,6 +294,10 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
             store2(p.pml + at * 2, mm2, lt);
         }
     }
+    if (p.wgs && tid == 0) {
+        if (t0 == sg.first) p.ends[e].x = blockIdx.x;
+        if (te == sg.first + sg.tiles) p.ends[e].y = blockIdx.x;
+    }
     pos += te - t0;
     if (pos >= pos_end) return;
     before += sg.tiles;
@@ -308,16 +312,14 @@ constexpr int MAX_WGS = 768;
 template <typename T, int HD, int ROWS> __global__ __launch_bounds__(256) void kv_attn_join_kernel(const AttnP p) {
     constexpr int LP = HD / 4, NS = 256 / (LP * ROWS);
     static_assert(LP * ROWS * NS == 256 && (NS == 1 || ROWS == 1), "either rows or pieces side by side");
-    __shared__ int red[8];
     const int tid = threadIdx.x, chunks = p.jrows / ROWS;
     const int e = blockIdx.x / chunks, r0 = blockIdx.x % chunks * ROWS;
     const Segment sg = segment_of(p, e);
     const Seq s = seq_of(p, sg.b);
     const int c0 = (sg.ct << p.cshift) + r0, cols = s.n * p.group;
     if (c0 >= cols) return;
-    int before;
-    const Line line = line_of<4>(p, e, before, red);
-    const int w0 = before / line.share, n = sg.tiles > 0 ? (before + sg.tiles - 1) / line.share - w0 + 1 : 0;
+    const int2 ends = sg.tiles > 0 ? p.ends[e] : make_int2(0, -1);
+    const int w0 = ends.x, n = ends.y - w0 + 1;
     if (n == 1) return;
     const int c = tid % LP, row = ROWS > 1 ? tid / LP : 0, qc = c0 + row;
     const size_t at = (((size_t)w0 + e) << p.cshift) + r0 + row;      // the next piece is in the next slot
@@ -385,7 +387,7 @@ Way way_of(int dtype, int B, int max_new, int kv, int group, int hd, int width, 
     }
     if (w.cshift != 4) {
         w.wgs = 256;
-        if (w.segs >= 4096 || tiles <= MIN_SHARE) w.wgs = 0;
+        if (w.segs >= 1024 || tiles <= MIN_SHARE) w.wgs = 0;
     } else {
         // as many as run at once (hd 64: 3 per CU, 128: 2), or one per column tile, without a join, where no sequence can be longer than
         // 16 tiles or there are so many column tiles that the chip is full anyway
@@ -395,6 +397,7 @@ Way way_of(int dtype, int B, int max_new, int kv, int group, int hd, int width, 
     w.slots = w.wgs ? w.wgs + w.segs : 0;
     return w;
 }
+size_t bytes_of(const Way& w, int hd) { return w.wgs ? ((w.slots << w.cshift) * (hd + 2) + w.segs * 2) * 4 : 0; }
 
 }  // namespace
 
@@ -402,7 +405,7 @@ extern "C" size_t pgt_kv_attention_workspace_bytes(int32_t dtype, int32_t B, int
                                                    int32_t page, int32_t causal, int32_t window) {
     if (B <= 0 || max_new <= 0 || heads <= 0 || kv_heads <= 0 || hd <= 0 || width <= 0 || kv_page_shift(page) < 0 || heads % kv_heads || causal < 0 || window < 0) return 0;
     const Way w = way_of(dtype, B, max_new, kv_heads, heads / kv_heads, hd, width, kv_page_shift(page), causal, window);
-    return (w.slots << w.cshift) * (hd + 2) * sizeof(float);
+    return bytes_of(w, hd);
 }
 
 extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const void* k_pages, const void* v_pages, const float* k_scale,
@@ -445,11 +448,12 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     if (w.wgs) {
         PGT_CHECK((double)w.segs * (((int64_t)width << p.pshift) / 64 + 1) < 2147483648.0,
                   "kv_attention: %d sequences of up to %d pages of %d tokens exceed one launch", B, width, page);
-        const size_t need = (w.slots << w.cshift) * (hd + 2) * sizeof(float);
+        const size_t need = bytes_of(w, hd);
         PGT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
                   "kv_attention: workspace of %zu bytes, %zu needed", workspace_bytes, need);
         p.po = (float*)workspace;
         p.pml = p.po + (w.slots << w.cshift) * hd;
+        p.ends = (int2*)(p.pml + (w.slots << w.cshift) * 2);
     }
     hipStream_t st = (hipStream_t)stream;
     if (w.cshift != 4)

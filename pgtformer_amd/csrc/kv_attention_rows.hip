@@ -25,6 +25,8 @@ __device__ __forceinline__ float max_of_halves(float v) {
     return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
 constexpr int NW = 8, TH = 64 * NW, CT = 32 * NW;      // waves, threads and columns of a workgroup
 
 template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_rows_kernel(const AttnP p) {
@@ -32,7 +34,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
     constexpr int KS = HD / 16, ND = HD / 32, NV = 2 * ND;      // products of S^T; row blocks of O^T, its products
     constexpr int KB = 64 * HD * 2, STAGE = 2 * KB;             // bytes of a K image; of a stage
     __shared__ __attribute__((aligned(16))) char smem[3 * STAGE];
-    __shared__ float4 sscale[3][4];                             // per 16-token block: score factor (negative: no page), log2 vs, 1 / vs
+    __shared__ float2 sscale[3][4];                             // per 16-token block: score factor (negative: no page), log2 vs
     __shared__ int red[2 * NW];
     __shared__ int nans;                                        // a V code in the range stands for NaN
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
@@ -44,7 +46,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
     const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
     int e = id, before = 0, pos = 0, pos_end = 0;
     if (p.wgs) {
-        const Line line = line_of<NW>(p, 0, before, red);
+        const Line line = line_of<NW>(p, red);
         pos = id * line.share;
         pos_end = min(pos + line.share, line.total);
         if (pos >= pos_end) return;
@@ -89,44 +91,51 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         for (int d = 0; d < ND; ++d) o[d] = zero16();
 
         // Staging: a unit is 64 lanes x 16 bytes of one block (16 tokens): K 4 chunks of 16 dims (lane -> token lane & 15, chunk lane / 16), V 64 dims.
-        // hd 128: wave w brings unit w / 4 of K and of V of block w & 3; hd 64: waves 0-3 bring K, 4-7 V.  Page numbers run one tile ahead of
-        // the loads, the loads one tile ahead of the conversion.
+        // hd 128: wave w brings unit w / 4 of K and of V of block w & 3; hd 64: waves 0-3 bring K, 4-7 V.  The loads run two tiles
+        // ahead of the conversion (two sets of registers), page numbers a tile ahead of the loads and issued before them: loads return in order.
         constexpr bool BOTH = HD == 128;
         const int blk = wave & 3, part = wave >> 2;
         const int32_t* tab = p.table + (size_t)b * p.ldt;
-        uint4 rk, rv;
-        int rpage, nextpage;
-        float rsk, rsv;
+        struct Raw {
+            u32x4 a, b;      // hd 128: K, V; hd 64: a alone
+            float s;         // lane 0: K scale, lane 1: V scale
+            bool have;
+        };
+        Raw raw[2];
+        int nextpage;
+        auto page_index = [&](int t, int k) { return (t * 64 + 16 * k) >> p.pshift; };
         auto page_at = [&](int t, int k) {
-            const int i = (t * 64 + 16 * k) >> p.pshift;
+            const int i = page_index(t, k);
             return t < te && i < p.width ? tab[i] : -1;
         };
         auto ok = [&](int i) { return i >= 0 && i < p.pages; };
         const uint32_t k_at = (uint32_t)((lane >> 4) * page + (lane & 15)) * 16 + (BOTH ? (uint32_t)(part * 4 * page * 16) : 0u);
         const uint32_t v_at = (uint32_t)(lane + (BOTH ? 64 * part : 0)) * 16;
-        auto load_raw = [&](int t) {      // of page nextpage
-            rpage = __builtin_amdgcn_readfirstlane(nextpage);
-            const int pg = ok(rpage) ? rpage : 0;
+        auto load_raw = [&](Raw& w, int t) {      // of page nextpage; then the page of the tile behind
+            const int pg0 = __builtin_amdgcn_readfirstlane(nextpage);
+            w.have = ok(pg0) & (t < te) & (page_index(t, blk) < p.width);
+            nextpage = tab[min(page_index(t + 1, blk), p.width - 1)];      // (no branch around a load: a wait behind one would be for all of them)
+            const int pg = w.have ? pg0 : 0;
             const int tok = (t * 64 + 16 * blk) & (page - 1);
-            const size_t at = pg * stride + hk * page_bytes;
-            if (BOTH || part == 0) rk = *reinterpret_cast<const uint4*>(p.kp + at + tok * 16 + k_at);
-            if (BOTH || part == 1) rv = *reinterpret_cast<const uint4*>(p.vp + at + (size_t)tok * HD + v_at);
-            rsk = p.ks[(size_t)pg * p.kv + hk];
-            rsv = p.vs[(size_t)pg * p.kv + hk];
+            const size_t at = pg * stride + hk * page_bytes, k_off = at + tok * 16, v_off = at + (size_t)tok * HD;
+            w.a = *reinterpret_cast<const u32x4*>(BOTH || part == 0 ? p.kp + k_off + k_at : p.vp + v_off + v_at);
+            if constexpr (BOTH) w.b = *reinterpret_cast<const u32x4*>(p.vp + v_off + v_at);
+            w.s = (lane & 1 ? p.vs : p.ks)[(size_t)pg * p.kv + hk];
         };
         // token 16 hh + e of a 32-token half -> the row of S^T whose score ends up in register e of lane half hh
         const int k_to = (((lane >> 4) + (BOTH ? 4 * part : 0)) * 128 + 32 * (blk >> 1) + (lane & 3) + 8 * ((lane & 15) >> 2) + 4 * (blk & 1)) * 16;
         const int v_to = KB + (blk * 2 * HD + lane + (BOTH ? 64 * part : 0)) * 16;
-        auto store = [&](int st, int t) {
+        auto store = [&](Raw& a, int st, int t) {
             char* d = smem + st * STAGE;
-            x3_opaque(rk);      // (or the compiler regroups the registers right behind the loads, and waits for them there)
-            x3_opaque(rv);
+            // (opaque, as one register quadruple: or the compiler regroups the registers right behind the loads, and waits for them there)
+            asm volatile("" : "+v"(a.a));
+            if constexpr (BOTH) asm volatile("" : "+v"(a.b));
             if (BOTH || part == 0) {
-                *reinterpret_cast<uint4*>(d + k_to) = HQ ? half8(rk.x, rk.y) : bfloat8(rk.x, rk.y);
-                *reinterpret_cast<uint4*>(d + k_to + 1024) = HQ ? half8(rk.z, rk.w) : bfloat8(rk.z, rk.w);
+                *reinterpret_cast<uint4*>(d + k_to) = HQ ? half8(a.a.x, a.a.y) : bfloat8(a.a.x, a.a.y);
+                *reinterpret_cast<uint4*>(d + k_to + 1024) = HQ ? half8(a.a.z, a.a.w) : bfloat8(a.a.z, a.a.w);
             }
             if (BOTH || part == 1) {
-                uint4 w = rv;
+                uint4 w = __builtin_bit_cast(uint4, BOTH ? a.b : a.a);
                 if ((t * 64 < all_lo) | (t * 64 + 64 > all_hi)) {
                     // NaN times the weight 0 of a query that does not see the token: zeros here, see the end
                     const uint4 n = make_uint4(nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w));
@@ -136,9 +145,9 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 *reinterpret_cast<uint4*>(d + v_to) = half8(w.x, w.y);
                 *reinterpret_cast<uint4*>(d + v_to + HD * 16) = half8(w.z, w.w);
             }
-            if (lane == 0 && part == 0) {      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
-                const int ev = (int)((__float_as_uint(rsv) >> 23) & 255) - 127;
-                sscale[st][blk] = make_float4(ok(rpage) ? fmaxf(fabsf(p.c) * rsk, 1e-30f) : -1.f, (float)ev, __uint_as_float((uint32_t)(127 - ev) << 23), 0.f);
+            if (lane < 2 && part == 0) {      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
+                const float factor = a.have ? fmaxf(fabsf(p.c) * a.s, 1e-30f) : -1.f, ev = (float)((int)((__float_as_uint(a.s) >> 23) & 255) - 127);
+                reinterpret_cast<float*>(&sscale[st][blk])[lane] = lane ? ev : factor;
             }
         };
         auto k_operand = [&](int st, int sb, int k) {
@@ -147,8 +156,8 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         auto v_operand = [&](int st, int sb, int i) {      // i = k-step * ND + row block
             return *reinterpret_cast<const uint4*>(smem + st * STAGE + KB + ((sb * 2 + h) * 2 * HD + r) * 16 + ((i / ND) * HD + (i % ND) * 32) * 16);
         };
-        float4 sc = make_float4(1.f, 0.f, 1.f, 0.f);      // of the current scores: sscale of this lane's 16 tokens
-        float tm = NEVER;                                 // the largest of them, in units of the exponent
+        float2 sc = make_float2(1.f, 0.f);      // of the current scores: sscale of this lane's 16 tokens
+        float tm = NEVER;                       // the largest of them, in units of the exponent
         auto top = [&](const f32x16& x) {
             float mx = x[0];
 #pragma unroll
@@ -170,7 +179,8 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 if (cw < cols) scores(nst, nsb, xn);
                 return;
             }
-            const float ck = fabsf(sc.x), ev = sc.y, back = sc.z;
+            const float ck = fabsf(sc.x), ev = sc.y;
+            const float back = __uint_as_float((uint32_t)(127 - (int)ev) << 23);      // 1 / vs
             if ((tok < lo_z) | (tok + 32 > hi_a) | (__any(sc.x < 0.f) != 0)) {
                 const uint32_t span = sc.x < 0.f ? 0u : (uint32_t)(hi - lo);
                 const int at = tok + 16 * h - lo;
@@ -197,7 +207,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             uint4 f[4];      // operands in flight
 #pragma unroll
             for (int k = 0; k < 4; ++k) f[k] = k_operand(nst, nsb, k);
-            const float4 scn = sscale[nst][nsb * 2 + h];
+            const float2 scn = sscale[nst][nsb * 2 + h];
             SLICE();
 #pragma unroll
             for (int k = 0; k < KS; ++k) {      // S^T of the next half, the weights
@@ -229,27 +239,29 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         if (tid == 0) nans = 0;
         __syncthreads();
         if (t0 < te) {
-            nextpage = page_at(t0, blk);
-            load_raw(t0);
-            nextpage = page_at(t0 + 1, blk);
-            store(0, t0);
-            if (t0 + 1 < te) load_raw(t0 + 1);
-            nextpage = page_at(t0 + 2, blk);
+            nextpage = tab[min(page_index(t0, blk), p.width - 1)];
+            load_raw(raw[0], t0);
+            load_raw(raw[1], t0 + 1);
+            store(raw[0], 0, t0);
+            load_raw(raw[0], t0 + 2);
             __syncthreads();
             f32x16 xa, xb;
             if (cw < cols) scores(0, 0, xa);
             int st = 0;
-            for (int t = t0; t < te; ++t) {
+            auto tile = [&](int t, Raw& next) {      // next holds tile t + 1
                 const int nst = st == 2 ? 0 : st + 1;
                 step(t, st, 0, st, 1, xa, xb);
-                if (t + 1 < te) {      // (the stage was last read in tile t - 2, which every wave left before the last barrier)
-                    store(nst, t + 1);
-                    if (t + 2 < te) load_raw(t + 2);
-                    nextpage = page_at(t + 3, blk);
-                }
+                store(next, nst, t + 1);      // (the stage was last read in tile t - 2, which every wave left before the last barrier)
+                load_raw(next, t + 3);        // (behind the last tile: page 0, not looked at)
                 __syncthreads();
                 step(t, st, 1, nst, 0, xb, xa);
                 st = nst;
+            };
+            for (int t = t0;;) {
+                tile(t, raw[1]);
+                if (++t >= te) break;
+                tile(t, raw[0]);
+                if (++t >= te) break;
             }
         }
 
@@ -306,6 +318,10 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                     }
                 }
             }
+        }
+        if (p.wgs && tid == 0) {
+            if (t0 == sg.first) p.ends[e].x = id;
+            if (te == sg.first + sg.tiles) p.ends[e].y = id;
         }
         pos += te - t0;
         if (pos >= pos_end) return;
