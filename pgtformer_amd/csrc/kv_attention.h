@@ -71,7 +71,8 @@ __device__ __forceinline__ void sees(const AttnP& p, int len, int pos, int& lo, 
     lo = 0;
     hi = len;
     if (p.causal) {
-        const uint32_t end = ((uint32_t)max(pos, 0) / (uint32_t)p.causal + 1) * (uint32_t)p.causal;      // < 2^32: pos + causal at most
+        const uint32_t at = (uint32_t)max(pos, 0), c = (uint32_t)p.causal;
+        const uint32_t end = c == 1 ? at + 1 : (at / c + 1) * c;      // < 2^32: pos + causal at most
         hi = (int)min(end, (uint32_t)len);
         if (p.window) lo = (int)min(end > (uint32_t)p.window ? end - (uint32_t)p.window : 0u, (uint32_t)len);
     }

@@ -25,7 +25,18 @@ __device__ __forceinline__ float max_of_halves(float v) {
     return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
 }
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// loads that write LDS: 64 lanes x 16 (4) bytes from a pointer per lane to dst + lane * 16 (4), dst uniform; asynchronous, counted by vmcnt
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+__device__ __forceinline__ void lds_load16(const void* src, uint32_t dst) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(src), "s"(dst) : "memory");
+}
+__device__ __forceinline__ void lds_load4(const void* src, uint32_t dst) {
+    uint32_t m0;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
+                 : "=&s"(m0) : "v"(src), "s"(dst) : "memory");
+}
 
 constexpr int NW = 8, TH = 64 * NW, CT = 32 * NW;      // waves, threads and columns of a workgroup
 
@@ -34,6 +45,8 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
     constexpr int KS = HD / 16, ND = HD / 32, NV = 2 * ND;      // products of S^T; row blocks of O^T, its products
     constexpr int KB = 64 * HD * 2, STAGE = 2 * KB;             // bytes of a K image; of a stage
     __shared__ __attribute__((aligned(16))) char smem[3 * STAGE];
+    constexpr int SET = (HD == 128 ? 2048 : 1024) + 256;        // bytes of a set of raw units of one wave
+    __shared__ __attribute__((aligned(16))) char rings[NW * 3 * SET];
     __shared__ float2 sscale[3][4];                             // per 16-token block: score factor (negative: no page), log2 vs
     __shared__ int red[2 * NW];
     __shared__ int nans;                                        // a V code in the range stands for NaN
@@ -61,6 +74,48 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         if (ct * CT >= cols) return;
         const int t0 = sg.first + (p.wgs ? pos - before : 0), te = p.wgs ? sg.first + min(pos_end - before, sg.tiles) : sg.first + sg.tiles;
         const bool whole = te - t0 == sg.tiles;
+
+        // Staging: a unit is 64 lanes x 16 bytes of one block (16 tokens): K 4 chunks of 16 dims (lane -> token lane & 15, chunk lane / 16), V 64 dims.
+        // hd 128: wave w brings unit w / 4 of K and of V of block w & 3; hd 64: waves 0-3 bring K, 4-7 V.  The loads go straight to LDS, into a
+        // ring of three sets per wave, three tiles ahead of the conversion (in registers the compiler moved them, and waited for that); a set
+        // also brings the block's scales and the page number of the tile three later.  Waits are by hand: NL loads per set, in order.
+        constexpr bool BOTH = HD == 128;
+        constexpr int NL = BOTH ? 3 : 2;
+        const int blk = wave & 3, part = wave >> 2;
+        const int32_t* tab = p.table + (size_t)b * p.ldt;
+        auto page_index = [&](int t, int k) { return (t * 64 + 16 * k) >> p.pshift; };
+        auto ok = [&](int i) { return i >= 0 && i < p.pages; };
+        char* ring = rings + wave * 3 * SET;
+        const uint32_t k_at = (uint32_t)((lane >> 4) * page + (lane & 15)) * 16 + (BOTH ? (uint32_t)(part * 4 * page * 16) : 0u);
+        const uint32_t v_at = (uint32_t)(lane + (BOTH ? 64 * part : 0)) * 16;
+        auto fetch = [&](int slot, int t, int pg0) {      // block blk of tile t, in page pg0 (behind the last tile, or missing: page 0, not looked at)
+            const int pg = (ok(pg0) & (t < te)) ? pg0 : 0;
+            const int tok = (t * 64 + 16 * blk) & (page - 1);
+            const size_t at = pg * stride + hk * page_bytes, one = (size_t)pg * p.kv + hk;
+            const uint8_t *kb = p.kp + (at + tok * 16) + k_at, *vb = p.vp + (at + (size_t)tok * HD) + v_at;
+            const uint32_t to = lds_address(ring + slot * SET);
+            lds_load16(BOTH || part == 0 ? kb : vb, to);
+            if constexpr (BOTH) lds_load16(vb, to + 1024);
+            const void* w = lane == 0 ? (const void*)(p.ks + one) : (const void*)(p.vs + one);
+            if (lane == 2) w = tab + min(page_index(t + 3, blk), p.width - 1);
+            lds_load4(w, to + SET - 256);
+        };
+        bool have0 = false, have1 = false, have2 = false;      // whether the next three tiles have a page
+        if (t0 < te) {      // the first three tiles are on their way while the columns are set up
+            int pg[3];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                const int k = page_index(t0 + i, blk);
+                pg[i] = uni(tab[min(k, p.width - 1)]);
+                if (k >= p.width) pg[i] = -1;
+            }
+            have0 = ok(pg[0]);
+            have1 = ok(pg[1]) & (t0 + 1 < te);
+            have2 = ok(pg[2]) & (t0 + 2 < te);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) fetch(i, t0 + i, pg[i]);
+        }
+
         // this wave's columns: what every one of them sees, and what any of them does
         const int cw = ct * CT + wave * 32;
         int lo_a = 0, hi_a = 0, lo_z = 0, hi_z = 0;      // a wave without columns sees nothing
@@ -90,53 +145,23 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = zero16();
 
-        // Staging: a unit is 64 lanes x 16 bytes of one block (16 tokens): K 4 chunks of 16 dims (lane -> token lane & 15, chunk lane / 16), V 64 dims.
-        // hd 128: wave w brings unit w / 4 of K and of V of block w & 3; hd 64: waves 0-3 bring K, 4-7 V.  The loads run two tiles
-        // ahead of the conversion (two sets of registers), page numbers a tile ahead of the loads and issued before them: loads return in order.
-        constexpr bool BOTH = HD == 128;
-        const int blk = wave & 3, part = wave >> 2;
-        const int32_t* tab = p.table + (size_t)b * p.ldt;
-        struct Raw {
-            u32x4 a, b;      // hd 128: K, V; hd 64: a alone
-            float s;         // lane 0: K scale, lane 1: V scale
-            bool have;
-        };
-        Raw raw[2];
-        int nextpage;
-        auto page_index = [&](int t, int k) { return (t * 64 + 16 * k) >> p.pshift; };
-        auto page_at = [&](int t, int k) {
-            const int i = page_index(t, k);
-            return t < te && i < p.width ? tab[i] : -1;
-        };
-        auto ok = [&](int i) { return i >= 0 && i < p.pages; };
-        const uint32_t k_at = (uint32_t)((lane >> 4) * page + (lane & 15)) * 16 + (BOTH ? (uint32_t)(part * 4 * page * 16) : 0u);
-        const uint32_t v_at = (uint32_t)(lane + (BOTH ? 64 * part : 0)) * 16;
-        auto load_raw = [&](Raw& w, int t) {      // of page nextpage; then the page of the tile behind
-            const int pg0 = __builtin_amdgcn_readfirstlane(nextpage);
-            w.have = ok(pg0) & (t < te) & (page_index(t, blk) < p.width);
-            nextpage = tab[min(page_index(t + 1, blk), p.width - 1)];      // (no branch around a load: a wait behind one would be for all of them)
-            const int pg = w.have ? pg0 : 0;
-            const int tok = (t * 64 + 16 * blk) & (page - 1);
-            const size_t at = pg * stride + hk * page_bytes, k_off = at + tok * 16, v_off = at + (size_t)tok * HD;
-            w.a = *reinterpret_cast<const u32x4*>(BOTH || part == 0 ? p.kp + k_off + k_at : p.vp + v_off + v_at);
-            if constexpr (BOTH) w.b = *reinterpret_cast<const u32x4*>(p.vp + v_off + v_at);
-            w.s = (lane & 1 ? p.vs : p.ks)[(size_t)pg * p.kv + hk];
-        };
         // token 16 hh + e of a 32-token half -> the row of S^T whose score ends up in register e of lane half hh
         const int k_to = (((lane >> 4) + (BOTH ? 4 * part : 0)) * 128 + 32 * (blk >> 1) + (lane & 3) + 8 * ((lane & 15) >> 2) + 4 * (blk & 1)) * 16;
         const int v_to = KB + (blk * 2 * HD + lane + (BOTH ? 64 * part : 0)) * 16;
-        auto store = [&](Raw& a, int st, int t) {
+        auto convert = [&](int st, int t) {      // set st = tile t -> stage st; then the set is fetched again, for tile t + 3
             char* d = smem + st * STAGE;
-            // (opaque, as one register quadruple: or the compiler regroups the registers right behind the loads, and waits for them there)
-            asm volatile("" : "+v"(a.a));
-            if constexpr (BOTH) asm volatile("" : "+v"(a.b));
+            const char* in = ring + st * SET;
+            const uint4 a = *reinterpret_cast<const uint4*>(in + lane * 16);
+            uint4 w = a;
+            if constexpr (BOTH) w = *reinterpret_cast<const uint4*>(in + 1024 + lane * 16);
+            const float scale = *reinterpret_cast<const float*>(in + SET - 256 + (lane & 1) * 4);
+            const int next = *reinterpret_cast<const int*>(in + SET - 256 + 8);
             if (BOTH || part == 0) {
-                *reinterpret_cast<uint4*>(d + k_to) = HQ ? half8(a.a.x, a.a.y) : bfloat8(a.a.x, a.a.y);
-                *reinterpret_cast<uint4*>(d + k_to + 1024) = HQ ? half8(a.a.z, a.a.w) : bfloat8(a.a.z, a.a.w);
+                *reinterpret_cast<uint4*>(d + k_to) = HQ ? half8(a.x, a.y) : bfloat8(a.x, a.y);
+                *reinterpret_cast<uint4*>(d + k_to + 1024) = HQ ? half8(a.z, a.w) : bfloat8(a.z, a.w);
             }
             if (BOTH || part == 1) {
-                uint4 w = __builtin_bit_cast(uint4, BOTH ? a.b : a.a);
-                if ((t * 64 < all_lo) | (t * 64 + 64 > all_hi)) {
+                if (((t * 64 < all_lo) | (t * 64 + 64 > all_hi)) & (t < te)) {
                     // NaN times the weight 0 of a query that does not see the token: zeros here, see the end
                     const uint4 n = make_uint4(nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w));
                     if (__any((n.x | n.y | n.z | n.w) != 0)) nans = 1;
@@ -146,9 +171,16 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 *reinterpret_cast<uint4*>(d + v_to + HD * 16) = half8(w.z, w.w);
             }
             if (lane < 2 && part == 0) {      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
-                const float factor = a.have ? fmaxf(fabsf(p.c) * a.s, 1e-30f) : -1.f, ev = (float)((int)((__float_as_uint(a.s) >> 23) & 255) - 127);
+                const float factor = have0 ? fmaxf(fabsf(p.c) * scale, 1e-30f) : -1.f, ev = (float)((int)((__float_as_uint(scale) >> 23) & 255) - 127);
                 reinterpret_cast<float*>(&sscale[st][blk])[lane] = lane ? ev : factor;
             }
+            // pages of the tiles ahead, and whether they are there
+            const int pn = page_index(t + 3, blk) < p.width ? uni(next) : -1;
+            have0 = have1;
+            have1 = have2;
+            have2 = ok(pn) & (t + 3 < te);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the set is read
+            fetch(st, t + 3, pn);
         };
         auto k_operand = [&](int st, int sb, int k) {
             return *reinterpret_cast<const uint4*>(smem + st * STAGE + (sb * 32 + r + 64 * h) * 16 + k * 2048);
@@ -239,30 +271,22 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         if (tid == 0) nans = 0;
         __syncthreads();
         if (t0 < te) {
-            nextpage = tab[min(page_index(t0, blk), p.width - 1)];
-            load_raw(raw[0], t0);
-            load_raw(raw[1], t0 + 1);
-            store(raw[0], 0, t0);
-            load_raw(raw[0], t0 + 2);
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+            convert(0, t0);
             __syncthreads();
             f32x16 xa, xb;
             if (cw < cols) scores(0, 0, xa);
             int st = 0;
-            auto tile = [&](int t, Raw& next) {      // next holds tile t + 1
+            for (int t = t0; t < te; ++t) {
                 const int nst = st == 2 ? 0 : st + 1;
                 step(t, st, 0, st, 1, xa, xb);
-                store(next, nst, t + 1);      // (the stage was last read in tile t - 2, which every wave left before the last barrier)
-                load_raw(next, t + 3);        // (behind the last tile: page 0, not looked at)
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");      // the set of tile t + 1 is here, those of t + 2, t + 3 on the way
+                convert(nst, t + 1);      // (the stage was last read in tile t - 2, which every wave left before the last barrier)
                 __syncthreads();
                 step(t, st, 1, nst, 0, xb, xa);
                 st = nst;
-            };
-            for (int t = t0;;) {
-                tile(t, raw[1]);
-                if (++t >= te) break;
-                tile(t, raw[0]);
-                if (++t >= te) break;
             }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
 
         // column cw + r: rows 32 d + 8 q + 4 h + 0..3 of O^T are in registers 4 q .. 4 q + 3
@@ -303,7 +327,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             for (int t = t0; t < te; ++t) {
                 if (t * 64 >= all_lo && t * 64 + 64 <= all_hi) continue;
                 for (int u = tid; u < 4 * HD; u += TH) {
-                    const int k = u / HD, dim = u % HD, tok = t * 64 + k * 16, pg = page_at(t, k);
+                    const int k = u / HD, dim = u % HD, tok = t * 64 + k * 16, pi = page_index(t, k), pg = pi < p.width ? tab[pi] : -1;
                     if (!ok(pg)) continue;
                     const uint8_t* c = p.vp + pg * stride + hk * page_bytes + ((size_t)((tok & (page - 1)) >> 4) * HD + dim) * 16;
                     for (int i = 0; i < 16; ++i) {
