@@ -23,14 +23,6 @@ __device__ __forceinline__ f32x4 mma_h(const uint4& a, const uint4& b, const f32
 __device__ __forceinline__ f32x4 mma_b(const uint4& a, const uint4& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
-// 16 bytes of the cache.  ONCE: with the streaming policy (7.1 instead of 6.3 TB/s on a plain read of 2 GiB), for launches in which no other
-// workgroup reads them (with it, 1024 query rows over the same pages took 1.5 times as long)
-template <bool ONCE> __device__ __forceinline__ uint4 load16(const uint8_t* p) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    const u32x4* q = reinterpret_cast<const u32x4*>(p);
-    if constexpr (ONCE) return __builtin_bit_cast(uint4, __builtin_nontemporal_load(q));
-    else return __builtin_bit_cast(uint4, *q);
-}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // does any of the four codes stand for NaN (0x7f, 0xff)?
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
@@ -90,64 +82,70 @@ __device__ __forceinline__ void sees_uni(const AttnP& p, int len, int pos, int& 
 }
 
 constexpr float NEVER = -1e30f;      // reference of a query that has seen nothing (finite: differences and products stay numbers)
-constexpr int MIN_SHARE = 4;         // tiles of a piece: one per wave of a workgroup with few rows
+constexpr int MIN_SHARE = 4;         // tiles of a piece
 
-// Work sharing (wgs > 0).  The tiles of 64 tokens of all segments - (sequence, kv head, column tile), in this order - are one line that is cut
-// into wgs equal pieces, whatever the lengths: every workgroup does the same work, and as many run as fit the chip at once.  A segment that
-// is cut leaves a partial result per piece - workgroup w and segment e meet in slot w + e, which no other pair has - and the join adds
-// them; one that is not is finished where it was computed.  Lengths are only known on the device: each workgroup sums them up.
+// Work sharing (wgs > 0).  The tiles of 64 tokens of all segments - (sequence, column tile, kv head), in an order of the kernel's - are one line
+// that is cut into wgs equal pieces, whatever the lengths: every workgroup does the same work, and as many run as fit the chip at once.  A
+// segment that is cut leaves a partial result per piece - workgroup w and segment e meet in slot w + e, which no other pair has - and the
+// join adds them; one that is not is finished where it was computed.  Lengths are only known on the device: each workgroup sums them up.
+//   order 0: (sequence, kv head, column tile), neighbours read the same pages       order 1: (sequence, column tile, kv head), one look-up for all heads
 struct Segment {
     int b, hk, ct, first, tiles;      // first tile, tiles
 };
-__device__ __forceinline__ Segment segment_of(const AttnP& p, int e) {
+__device__ __forceinline__ Segment segment_of(const AttnP& p, int order, int e) {
     Segment g;
-    g.ct = e % p.nct;
-    e /= p.nct;
-    g.hk = e % p.kv;
-    g.b = e / p.kv;
+    if (order) {
+        g.hk = e % p.kv;
+        e /= p.kv;
+        g.ct = p.nct == 1 ? 0 : e % p.nct;
+        g.b = p.nct == 1 ? e : e / p.nct;
+    } else {
+        g.ct = p.nct == 1 ? 0 : e % p.nct;
+        e = p.nct == 1 ? e : e / p.nct;
+        g.hk = e % p.kv;
+        g.b = e / p.kv;
+    }
     const Seq s = seq_of(p, g.b);
     const int cols = s.n * p.group, c0 = g.ct << p.cshift, cz = min(c0 + (1 << p.cshift), cols) - 1;
     g.first = g.tiles = 0;
     if (c0 < cols) {
         int lo, hi, dummy;
-        sees(p, s.len, s.len - s.n + c0 / p.group, lo, dummy);
-        sees(p, s.len, s.len - s.n + cz / p.group, dummy, hi);
+        sees(p, s.len, s.len - s.n + (c0 == 0 ? 0 : c0 / p.group), lo, dummy);
+        sees(p, s.len, s.len - s.n + (cz == cols - 1 ? s.n - 1 : cz / p.group), dummy, hi);
         g.first = lo >> 6;
         g.tiles = max(((hi + 63) >> 6) - g.first, 0);
     }
     return g;
 }
 __device__ __forceinline__ Segment uni(const Segment& g) { return {uni(g.b), uni(g.hk), uni(g.ct), uni(g.first), uni(g.tiles)}; }
-__device__ __forceinline__ int wave_sum_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
 struct Line {
     int total, share;
 };
-// the whole line (all 64 * W threads; red: 2 * W ints)
-template <int W> __device__ __forceinline__ Line line_of(const AttnP& p, int* red) {
-    const int segs = p.B * p.kv * p.nct;
-    int all = 0;
-    for (int i = threadIdx.x; i < segs; i += 64 * W) all += segment_of(p, i).tiles;
-    all = wave_sum_i(all);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = all;
-    __syncthreads();
-    Line l;
-    l.total = 0;
+// This workgroup's part [pos, end) of the line, the segment e that pos lies in and the line before that; false: nothing (all 64 * W threads;
+// red: W + 2 ints).  In order 1 the kv heads of a column tile are counted at once.
+template <int W, int ORDER>
+__device__ __forceinline__ bool part_of(const AttnP& p, int wg, int& pos, int& end, int& e, int& before, int* red) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int entries = p.B * p.nct * (ORDER ? 1 : p.kv), mul = ORDER ? p.kv : 1;
+    auto units = [&](int i) { return i < entries ? segment_of(p, ORDER, i * mul).tiles * mul : 0; };
+    const int mine = units(tid);      // (up to 64 * W entries: looked up once)
+    int all = mine;
+    for (int i = tid + 64 * W; i < entries; i += 64 * W) all += units(i);
 #pragma unroll
-    for (int w = 0; w < W; ++w) l.total += red[w];
-    l.total = uni(l.total);
-    l.share = uni(max((l.total + p.wgs - 1) / p.wgs, MIN_SHARE));
-    return l;
-}
-// the segment that place `pos` of the line lies in, and the line before it
-template <int W> __device__ __forceinline__ void locate(const AttnP& p, int pos, int& e, int& before, int* red) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, segs = p.B * p.kv * p.nct;
+    for (int o = 32; o > 0; o >>= 1) all += __shfl_xor(all, o, 64);
+    if (lane == 0) red[wave] = all;
+    __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) total += red[w];
+    total = uni(total);
+    const int share = uni(max((total + p.wgs - 1) / p.wgs, MIN_SHARE));
+    pos = wg * share;
+    end = min(pos + share, total);
+    if (pos >= end) return false;
     int run = 0;
-    for (int c = 0; c < segs; c += 64 * W) {
-        const int u = c + tid < segs ? segment_of(p, c + tid).tiles : 0;
+    for (int c = 0; c < entries; c += 64 * W) {
+        const int u = c == 0 ? mine : units(c + tid);
         int v = u;
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
@@ -168,9 +166,10 @@ template <int W> __device__ __forceinline__ void locate(const AttnP& p, int pos,
         if (run > pos) break;
     }
     __syncthreads();
-    e = uni(red[W]);
+    e = uni(red[W]) * mul;
     before = uni(red[W + 1]);
     __syncthreads();
+    return true;
 }
 
 }  // namespace

@@ -26,37 +26,51 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     constexpr int QP = F32 ? 3 : 1;          // planes of q
     constexpr int KS = HD / 32;              // k-steps of S^T
     constexpr int ND = HD / 16;              // row tiles of O^T
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
-    __shared__ int red[8];
+    __shared__ int red[NW + 2];
     __shared__ float sm[NW][16], sl[NW][16];
-    __shared__ __attribute__((aligned(16))) float so[NW][16][HD + 4];
+    // per wave a tile: K (chunk of 16 dims, 64 slots, 16 bytes), V (dims / 16, 4 blocks, 16 dims, 16 bytes), and 64 words: the four blocks'
+    // K scales, V scales, and pages of the next tile; afterwards the waves' results
+    constexpr int KB = HD * 64, SET = 2 * KB + 256, NK = HD / 16;
+    __shared__ __attribute__((aligned(16))) char rings[NW * SET];
+    static_assert(16 * (HD + 4) * 4 <= SET, "the results fit");
+    float (*so)[16][HD + 4] = reinterpret_cast<float (*)[16][HD + 4]>(rings);
     int e = blockIdx.x, before = 0, pos = 0, pos_end = 0;
-    if (p.wgs) {
-        const Line line = line_of<NW>(p, red);
-        pos = blockIdx.x * line.share;
-        pos_end = min(pos + line.share, line.total);
-        if (pos >= pos_end) return;
-        locate<NW>(p, pos, e, before, red);
-    }
-    for (;;) {      // the segments that this workgroup's part of the line touches
-    const Segment sg = uni(segment_of(p, e));
-    if (p.wgs && sg.tiles == 0) { ++e; continue; }
-    const int b = sg.b, hk = sg.hk, ct = sg.ct;
-    const Seq s = uni(seq_of(p, b));
-    const int cols = s.n * p.group;
+    if (p.wgs && !part_of<NW, 1>(p, blockIdx.x, pos, pos_end, e, before, red)) return;
+    for (;;) {      // the column tiles that this workgroup's part of the line touches
+    const Segment sg = uni(segment_of(p, 1, e));
+    const Seq s = uni(seq_of(p, sg.b));
+    const int cols = s.n * p.group, ct = sg.ct;
+    if (p.wgs && sg.tiles == 0) { e += p.kv; continue; }
     if (ct * 16 >= cols) return;
-    const int t0 = sg.first + (p.wgs ? pos - before : 0), te = p.wgs ? sg.first + min(pos_end - before, sg.tiles) : sg.first + sg.tiles;
-    const bool whole = te - t0 == sg.tiles;
-    const int qc = ct * 16 + col;
-    const int qi = min(qc, cols - 1) / p.group;
-    const int head = hk * p.group + min(qc, cols - 1) % p.group;
+    const int qc = min(ct * 16 + col, cols - 1), qi = qc / p.group, qg = qc - qi * p.group;
     int lo, hi;
     sees(p, s.len, s.len - s.n + qi, lo, hi);
-    // what the tile's first and last query see: the range to visit, and the part that every query sees
-    int lo_a, hi_a, lo_z, hi_z;
-    sees_uni(p, s.len, s.len - s.n + ct * 16 / p.group, lo_a, hi_a);
-    sees_uni(p, s.len, s.len - s.n + min(ct * 16 + 15, cols - 1) / p.group, lo_z, hi_z);
+    // what every query of the tile sees: from the last one's first token to the first one's last
+    int hi_a, lo_z, dummy;
+    sees_uni(p, s.len, s.len - s.n + ct * 16 / p.group, dummy, hi_a);
+    sees_uni(p, s.len, s.len - s.n + min(ct * 16 + 15, cols - 1) / p.group, lo_z, dummy);
+    int hk = sg.hk;
+    if (p.wgs) {      // (the look-up gives the first kv head)
+        hk = (pos - before) / sg.tiles;
+        e += hk;
+        before += hk * sg.tiles;
+    }
+    for (;;) {        // its kv heads
+    const int t0 = sg.first + (p.wgs ? pos - before : 0), te = p.wgs ? sg.first + min(pos_end - before, sg.tiles) : sg.first + sg.tiles;
+    const bool whole = te - t0 == sg.tiles;
+    const int head = hk * p.group + qg;
+
+    const int page = 1 << p.pshift, kblk = (lane >> 2) & 3;
+    const size_t page_bytes = (size_t)page * HD, head_off = (size_t)hk * page_bytes, stride = (size_t)p.kv * page_bytes;
+    const int32_t* tab = p.table + (size_t)sg.b * p.ldt;
+    auto valid = [&](int t, int i, int k) { return i >= 0 && i < p.pages && ((t * 64 + 16 * k) >> p.pshift) < p.width; };
+    auto page_slot = [&](int t, int k) { return tab + min((t * 64 + 16 * k) >> p.pshift, p.width - 1); };
+    const int steps = (te - t0 - wave + NW - 1) / NW;      // this wave's tiles t0 + wave, + NW, ...
+    // pages of the first tile: of the block whose K this lane brings, of the one whose scales it brings, and of its own (V, scores)
+    int pk = -1, pm = -1, pv = -1;
+    if (steps > 0) pk = *page_slot(t0 + wave, kblk), pm = *page_slot(t0 + wave, lane & 3), pv = *page_slot(t0 + wave, g);
 
     // Q^T operand: k-step 2 s + h covers dims 64 s + 16 g + 8 h .. + 7 of lane group g - the order of the K loads
     uint4 qf[QP][KS];
@@ -84,60 +98,69 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
             qf[0][st] = *reinterpret_cast<const uint4*>(qp);
         }
     }
+#pragma unroll
+    for (int pl = 0; pl < QP; ++pl)
+#pragma unroll
+        for (int st = 0; st < KS; ++st) x3_opaque(qf[pl][st]);      // here, or the wait for them stands in the loop and drains the tiles' loads
 
     f32x4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = NEVER, l = 0.f;
-    const int page = 1 << p.pshift, kblk = (lane >> 2) & 3;
-    const size_t page_bytes = (size_t)page * HD, head_off = (size_t)hk * page_bytes, stride = (size_t)p.kv * page_bytes;
-    const int32_t* tab = p.table + (size_t)b * p.ldt;
-
-    // Loads run one tile ahead: K of tile t + NW is issued when the scores of t are done, V when its product is, page numbers two tiles ahead
-    struct Page {
-        int k, v;      // page of the block whose K rows this lane loads, and of its own block (V, scales)
+    // Tiles come through LDS: the next K is asked for as soon as this one is in registers, the next V likewise, page numbers with the K of the
+    // tile before.  Slot 16 r + i of a K chunk holds token 16 (i / 4) + 4 r + i % 4: row i of S^T tile r.
+    char* ring = rings + wave * SET;
+    const int k_tok = 16 * kblk + 4 * g + (lane & 3);      // lane -> slot lane
+    // pages of tile t: of the block whose K this lane brings, and of its own block (V, scales, scores)
+    auto ask_k = [&](int t, int pk) {
+        const int id = valid(t, pk, kblk) ? pk : 0;
+        const uint8_t* kb = p.kp + id * stride + head_off + ((t * 64 + k_tok) & (page - 1)) * 16;
+        const uint32_t to = lds_address(ring);
+#pragma unroll
+        for (int c = 0; c < NK; ++c) lds_load16<ONCE>(kb + (size_t)c * page * 16, to + c * 1024);
     };
-    auto pages_of = [&](int t) {
-        const int ik = (t * 64 + 16 * kblk) >> p.pshift, iv = (t * 64 + 16 * g) >> p.pshift;
-        return Page{t < te && ik < p.width ? tab[ik] : -1, t < te && iv < p.width ? tab[iv] : -1};
+    auto ask_v = [&](int t, int pv) {
+        const int id = valid(t, pv, g) ? pv : 0;
+        const uint8_t* vb = p.vp + id * stride + head_off + (size_t)(((t * 64 + 16 * g) & (page - 1)) >> 4) * (HD * 16) + col * 16;
+        const uint32_t to = lds_address(ring + KB);
+#pragma unroll
+        for (int d = 0; d < ND; ++d) lds_load16<ONCE>(vb + d * 256, to + d * 1024);
     };
-    uint4 kr[4][HD / 64], vr[ND];
-    float sk, sv;
-    bool have;
-    auto load_k = [&](int t, Page pg) {
-        have = pg.v >= 0 && pg.v < p.pages;
-        const int idv = have ? pg.v : 0, idk = pg.k >= 0 && pg.k < p.pages ? pg.k : 0;
-        sk = p.ks[(size_t)idv * p.kv + hk];
-        sv = p.vs[(size_t)idv * p.kv + hk];
-        const uint8_t* kb = p.kp + idk * stride + head_off + (((t * 64 + 16 * kblk) & (page - 1)) + (lane & 3)) * 16;
+    auto ask_m = [&](int t, int pm) {      // pm: the page of block lane & 3
+        const size_t one = (size_t)(valid(t, pm, lane & 3) ? pm : 0) * p.kv + hk;
+        const void* from = lane < 4 ? (const void*)(p.ks + one) : (const void*)(p.vs + one);
+        if (lane >= 8) from = page_slot(t + NW, lane & 3);
+        lds_load4(from, lds_address(ring + 2 * KB));
+    };
+    if (steps > 0) {
+        ask_m(t0 + wave, pm);
+        ask_k(t0 + wave, pk);
+        ask_v(t0 + wave, pv);
+    }
+    for (int i = 0; i < steps; ++i) {
+        const int t = t0 + wave + NW * i, tv = t * 64 + 16 * g;
+        const bool more = i + 1 < steps, here = valid(t, pv, g);
+        wait_loads<NK>();      // all but V
+        uint4 kr[NK];
 #pragma unroll
         for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int c = 0; c < HD / 64; ++c) kr[r][c] = load16<ONCE>(kb + (size_t)(4 * c + g) * page * 16 + r * 64);
-    };
-    auto load_v = [&](int t, Page pg) {
-        const int idv = pg.v >= 0 && pg.v < p.pages ? pg.v : 0;
-        const uint8_t* vb = p.vp + idv * stride + head_off + (size_t)(((t * 64 + 16 * g) & (page - 1)) >> 4) * (HD * 16) + col * 16;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) vr[d] = load16<ONCE>(vb + d * 256);
-    };
-    const Page pg = pages_of(t0 + wave);
-    Page pn = pages_of(t0 + wave + NW);
-    if (t0 + wave < te) {
-        load_k(t0 + wave, pg);
-        load_v(t0 + wave, pg);
-    }
-    for (int t = t0 + wave; t < te; t += NW) {
-        const int tv = t * 64 + 16 * g;
-        const bool more = t + NW < te;
-        const Page p2 = pages_of(t + 2 * NW);
+            for (int c = 0; c < HD / 64; ++c) kr[r * (HD / 64) + c] = *reinterpret_cast<const uint4*>(ring + ((4 * c + g) * 64 + 16 * r + col) * 16);
+        const int* words = reinterpret_cast<const int*>(ring + 2 * KB);
+        const float sk_t = __int_as_float(words[g]), sv_t = here ? __int_as_float(words[4 + g]) : 1.f;
+        pk = words[8 + kblk], pv = words[8 + g], pm = words[8 + (lane & 3)];
+        wait_lds();
+        if (more) {
+            ask_m(t + NW, pm);
+            ask_k(t + NW, pk);
+        }
         f32x4 x[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             x[r] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < HD / 64; ++c) {
-                const uint4 w = kr[r][c];
+                const uint4 w = kr[r * (HD / 64) + c];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint4 a = HQ ? half8(h ? w.z : w.x, h ? w.w : w.y) : bfloat8(h ? w.z : w.x, h ? w.w : w.y);
@@ -147,18 +170,15 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
                 }
             }
         }
-        const bool here = have;
-        const float sk_t = sk, sv_t = sv;
-        if (more) load_k(t + NW, pn);
         const float ev = (float)((int)((__float_as_uint(sv_t) >> 23) & 255) - 127), ck = p.c * sk_t;
-        const bool masked = t * 64 < lo_z || t * 64 + 64 > hi_a || __any(!here);
+        const bool masked = (t * 64 < lo_z) | (t * 64 + 64 > hi_a) | (__any(!here) != 0);
         float y[16], mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) y[e] = __builtin_fmaf(x[e >> 2][e & 3], ck, ev);
         if (masked) {
+            const uint32_t span = here ? (uint32_t)(hi - lo) : 0u;
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-                if (!here || tv + e < lo || tv + e >= hi) y[e] = -INFINITY;
+            for (int e = 0; e < 16; ++e) y[e] = (uint32_t)(tv + e - lo) < span ? y[e] : -INFINITY;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, y[e]);
@@ -198,6 +218,13 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
                 pl2[h] = make_uint4(r[0], r[1], r[2], r[3]);
             }
         }
+        if (more) wait_loads<NK + 1>();      // all but the next tile's words and K
+        else wait_loads<0>();
+        uint4 vr[ND];
+#pragma unroll
+        for (int d = 0; d < ND; ++d) vr[d] = *reinterpret_cast<const uint4*>(ring + KB + d * 1024 + lane * 16);
+        wait_lds();
+        if (more) ask_v(t + NW, pv);
         if (masked) {
             // 0 * NaN: a V code that stands for NaN must reach the queries that see its token, and only those
             uint32_t any = 0;
@@ -244,15 +271,13 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
             o[d] = mma_h(a0, pf[0], o[d]);
             o[d] = mma_h(a1, pf[1], o[d]);
         }
-        if (more) load_v(t + NW, pn);
-        pn = p2;
     }
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
 
     // join the waves: every one against the common reference
     if (g == 0) sm[wave][col] = m;
-    __syncthreads();
+    __syncthreads();      // (and every wave is through with its ring)
     float mm = sm[0][col];
 #pragma unroll
     for (int w = 1; w < NW; ++w) mm = fmaxf(mm, sm[w][col]);
@@ -263,9 +288,9 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
         *reinterpret_cast<f32x4*>(&so[wave][col][16 * d + 4 * g]) = o[d] * al;
     }
     __syncthreads();
-    // thread: column tid / 16, HD / 16 consecutive dims
-    constexpr int PD = HD / 16;
-    const int c2 = tid >> 4, d2 = (tid & 15) * PD, qc2 = ct * 16 + c2;
+    // thread: column tid / (4 NW), HD / (4 NW) consecutive dims
+    constexpr int PT = 4 * NW, PD = HD / PT;
+    const int c2 = tid / PT, d2 = (tid % PT) * PD, qc2 = ct * 16 + c2;
     float f[PD], lt = 0.f;
 #pragma unroll
     for (int e = 0; e < PD; ++e) f[e] = 0.f;
@@ -287,7 +312,7 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
         const size_t at = ((size_t)blockIdx.x + e) * 16 + c2;
 #pragma unroll
         for (int e2 = 0; e2 < PD; e2 += 4) store4(p.po + at * HD + d2 + e2, f + e2);
-        if ((tid & 15) == 0) {
+        if (tid % PT == 0) {
             float mm2 = sm[0][c2];
 #pragma unroll
             for (int k = 1; k < NW; ++k) mm2 = fmaxf(mm2, sm[k][c2]);
@@ -303,6 +328,8 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     before += sg.tiles;
     ++e;
     __syncthreads();
+    if (++hk == p.kv) break;
+    }
     }
 }
 
@@ -314,7 +341,7 @@ template <typename T, int HD, int ROWS> __global__ __launch_bounds__(256) void k
     static_assert(LP * ROWS * NS == 256 && (NS == 1 || ROWS == 1), "either rows or pieces side by side");
     const int tid = threadIdx.x, chunks = p.jrows / ROWS;
     const int e = blockIdx.x / chunks, r0 = blockIdx.x % chunks * ROWS;
-    const Segment sg = segment_of(p, e);
+    const Segment sg = segment_of(p, p.cshift == 4, e);
     const Seq s = seq_of(p, sg.b);
     const int c0 = (sg.ct << p.cshift) + r0, cols = s.n * p.group;
     if (c0 >= cols) return;

@@ -25,19 +25,6 @@ __device__ __forceinline__ float max_of_halves(float v) {
     return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
 }
 
-// loads that write LDS: 64 lanes x 16 (4) bytes from a pointer per lane to dst + lane * 16 (4), dst uniform; asynchronous, counted by vmcnt
-__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
-__device__ __forceinline__ void lds_load16(const void* src, uint32_t dst) {
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0) : "v"(src), "s"(dst) : "memory");
-}
-__device__ __forceinline__ void lds_load4(const void* src, uint32_t dst) {
-    uint32_t m0;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %1, off\n\ts_mov_b32 m0, %0"
-                 : "=&s"(m0) : "v"(src), "s"(dst) : "memory");
-}
-
 constexpr int NW = 8, TH = 64 * NW, CT = 32 * NW;      // waves, threads and columns of a workgroup
 
 template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_rows_kernel(const AttnP p) {
@@ -48,7 +35,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
     constexpr int SET = (HD == 128 ? 2048 : 1024) + 256;        // bytes of a set of raw units of one wave
     __shared__ __attribute__((aligned(16))) char rings[NW * 3 * SET];
     __shared__ float2 sscale[3][4];                             // per 16-token block: score factor (negative: no page), log2 vs
-    __shared__ int red[2 * NW];
+    __shared__ int red[NW + 2];
     __shared__ int nans;                                        // a V code in the range stands for NaN
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, r = lane & 31;
     const int page = 1 << p.pshift;
@@ -59,14 +46,10 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
     const int id = (xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8) + (blockIdx.x >> 3);
     int e = id, before = 0, pos = 0, pos_end = 0;
     if (p.wgs) {
-        const Line line = line_of<NW>(p, red);
-        pos = id * line.share;
-        pos_end = min(pos + line.share, line.total);
-        if (pos >= pos_end) return;
-        locate<NW>(p, pos, e, before, red);
+        if (!part_of<NW, 0>(p, id, pos, pos_end, e, before, red)) return;
     }
     for (;;) {      // the segments that this workgroup's part of the line touches
-        const Segment sg = uni(segment_of(p, e));
+        const Segment sg = uni(segment_of(p, 0, e));
         if (p.wgs && sg.tiles == 0) { ++e; continue; }
         const int b = sg.b, hk = sg.hk, ct = sg.ct;
         const Seq s = uni(seq_of(p, b));
@@ -179,7 +162,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             have0 = have1;
             have1 = have2;
             have2 = ok(pn) & (t + 3 < te);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");      // the set is read
+            wait_lds();      // the set is read
             fetch(st, t + 3, pn);
         };
         auto k_operand = [&](int st, int sb, int k) {
@@ -271,7 +254,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         if (tid == 0) nans = 0;
         __syncthreads();
         if (t0 < te) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");
+            wait_loads<2 * NL>();
             convert(0, t0);
             __syncthreads();
             f32x16 xa, xb;
@@ -280,13 +263,13 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             for (int t = t0; t < te; ++t) {
                 const int nst = st == 2 ? 0 : st + 1;
                 step(t, st, 0, st, 1, xa, xb);
-                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NL) : "memory");      // the set of tile t + 1 is here, those of t + 2, t + 3 on the way
+                wait_loads<2 * NL>();      // the set of tile t + 1 is here, those of t + 2, t + 3 on the way
                 convert(nst, t + 1);      // (the stage was last read in tile t - 2, which every wave left before the last barrier)
                 __syncthreads();
                 step(t, st, 1, nst, 0, xb, xa);
                 st = nst;
             }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            wait_loads<0>();
         }
 
         // column cw + r: rows 32 d + 8 q + 4 h + 0..3 of O^T are in registers 4 q .. 4 q + 3
