@@ -44,6 +44,27 @@ struct RopeP {
 
 constexpr int MAXTOK = 4;
 
+// sum over the N lanes of an aligned group, in all of them: lane exchanges that cost no instruction of their own
+template <int CTRL> __device__ __forceinline__ float add_dpp(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int N> __device__ __forceinline__ float group_sum(float v) {
+    static_assert(N == 4 || N == 8 || N == 16 || N == 32, "lanes of a head row");
+    v = add_dpp<0xb1>(v);                            // lane ^ 1
+    v = add_dpp<0x4e>(v);                            // lane ^ 2
+    if constexpr (N >= 8) v = add_dpp<0x141>(v);     // the other half of 8
+    if constexpr (N >= 16) v = add_dpp<0x140>(v);    // the other half of 16
+    if constexpr (N >= 32) v += __shfl_xor(v, 16, 64);
+    return v;
+}
+
+// 1 / sqrt(v) to an ulp; the instruction takes subnormals for zero
+__device__ __forceinline__ float rsqrt_(float v) {
+    const bool small = v < 0x1p-100f;
+    const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p60f : v);
+    return small ? r * 0x1p30f : r;
+}
+
 template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void qk_rope_kernel(const RopeP p) {
     constexpr int LPH = HD / 8, NG = 256 / LPH;      // lanes per head row, head rows in flight per workgroup
     __shared__ float2 turn[MAXTOK][HD / 2];
@@ -62,6 +83,8 @@ template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void q
         gk[e] = p.kg ? p.kg[d] : 1.f;
         sq[e] = sk[e] = 0.f;
     }
+    // the workgroup's head rows: those of q, then those of k, tokens outermost; a group of lanes takes every step-th
+    const int step = NG * gridDim.y, first = blockIdx.y * NG + grp;
     const int nblk = (p.rows + p.tok - 1) / p.tok;
     for (int blk = blockIdx.x; blk < nblk; blk += gridDim.x) {
         const int t0 = blk * p.tok, nt = min(p.tok, p.rows - t0);
@@ -73,68 +96,69 @@ template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void q
             turn[t][c] = make_float2(cs, s);
         }
         __syncthreads();
-        for (int task = blockIdx.y * NG + grp; task < nt * nh; task += NG * gridDim.y) {
-            const int t = task / nh, h = task - t * nh;
-            const bool isq = h < p.heads;
-            const int hh = isq ? h : h - p.heads;
-            const size_t row = t0 + t;
-            const T* x = (const T*)(isq ? p.q : p.k) + row * (isq ? p.ldq : p.ldk) + hh * HD;
-            float f[8], z[8];
-            ld4(x + lo, f);
-            ld4(x + hi, f + 4);
-            if constexpr (BWD) {
-                const T* dy = (const T*)(isq ? p.dq : p.dk) + row * (isq ? p.lddq : p.lddk) + hh * HD;
-                ld4(dy + lo, z);
-                ld4(dy + hi, z + 4);
-            }
-            float ss = 0.f;
+        auto rows_of = [&](const void* xp, int ldx, const void* dyp, int lddy, void* yp, int ldy, int heads, int from, const float* gain, float* sum) {
+            const int dt = step / heads, dh = step - dt * heads;
+            int t = from / heads, h = from - t * heads;
+            for (; t < nt;) {
+                const size_t row = t0 + t;
+                const T* x = (const T*)xp + row * ldx + h * HD;
+                float f[8], z[8];
+                ld4(x + lo, f);
+                ld4(x + hi, f + 4);
+                if constexpr (BWD) {
+                    const T* dy = (const T*)dyp + row * lddy + h * HD;
+                    ld4(dy + lo, z);
+                    ld4(dy + hi, z + 4);
+                }
+                float ss = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+                for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+                const float r = rsqrt_(group_sum<LPH>(ss) * (1.f / HD) + p.eps);
+                float* v = BWD ? z : f;
+                if constexpr (!BWD) {
 #pragma unroll
-            for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o, 64);
-            const float r = 1.f / sqrtf(ss * (1.f / HD) + p.eps);
-            float* v = BWD ? z : f;
-            if constexpr (!BWD) {
+                    for (int e = 0; e < 8; ++e) f[e] = f[e] * r * gain[e];
+                }
+                if (turned) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = f[e] * r * (isq ? gq[e] : gk[e]);
-            }
-            if (turned) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 cs = turn[t][pr + e];
-                    const float s = BWD ? -cs.y : cs.y;
-                    if (p.inter) {
-                        const float a = v[2 * e], b = v[2 * e + 1];
-                        v[2 * e] = a * cs.x - b * s;
-                        v[2 * e + 1] = b * cs.x + a * s;
-                    } else {
-                        const float a = v[e], b = v[4 + e];
-                        v[e] = a * cs.x - b * s;
-                        v[4 + e] = b * cs.x + a * s;
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 cs = turn[t][pr + e];
+                        const float s = BWD ? -cs.y : cs.y;
+                        if (p.inter) {
+                            const float a = v[2 * e], b = v[2 * e + 1];
+                            v[2 * e] = a * cs.x - b * s;
+                            v[2 * e + 1] = b * cs.x + a * s;
+                        } else {
+                            const float a = v[e], b = v[4 + e];
+                            v[e] = a * cs.x - b * s;
+                            v[4 + e] = b * cs.x + a * s;
+                        }
                     }
                 }
-            }
-            if constexpr (BWD) {
-                float dot = 0.f;
+                if constexpr (BWD) {
+                    float dot = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    f[e] *= r;
-                    const float w = z[e] * f[e];
-                    if (isq) sq[e] += w;
-                    else sk[e] += w;
-                    z[e] *= isq ? gq[e] : gk[e];
-                    dot += f[e] * z[e];
+                    for (int e = 0; e < 8; ++e) {
+                        f[e] *= r;
+                        sum[e] += z[e] * f[e];
+                        z[e] *= gain[e];
+                        dot += f[e] * z[e];
+                    }
+                    dot = group_sum<LPH>(dot) * (1.f / HD);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z[e] = r * (z[e] - f[e] * dot);
                 }
-#pragma unroll
-                for (int o = LPH / 2; o > 0; o >>= 1) dot += __shfl_xor(dot, o, 64);
-                dot *= 1.f / HD;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) z[e] = r * (z[e] - f[e] * dot);
+                T* y = (T*)yp + row * ldy + h * HD;
+                store4(y + lo, v);
+                store4(y + hi, v + 4);
+                t += dt;
+                h += dh;
+                if (h >= heads) h -= heads, ++t;
             }
-            T* y = (T*)(isq ? p.qo : p.ko) + row * (isq ? p.ldqo : p.ldko) + hh * HD;
-            store4(y + lo, v);
-            store4(y + hi, v + 4);
-        }
+        };
+        if (p.heads) rows_of(p.q, p.ldq, p.dq, p.lddq, p.qo, p.ldqo, p.heads, first, gq, sq);
+        const int past = nt * p.heads - first;      // the head rows of q behind this group's first, to the next multiple of step
+        if (p.kv_heads) rows_of(p.k, p.ldk, p.dk, p.lddk, p.ko, p.ldko, p.kv_heads, past > 0 ? (past + step - 1) / step * step - past : -past, gk, sk);
         __syncthreads();
     }
     if constexpr (BWD) {      // the workgroup's share of dg: head rows in flight added in order
@@ -155,17 +179,27 @@ template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void q
     }
 }
 
-// dg[i] = sum over the n workgroups of part[w][i], in a fixed order (fp64: up to 1024 terms); 16 outputs per workgroup
-__global__ __launch_bounds__(256) void qk_rope_gain_kernel(const float* __restrict__ part, int n, int hd, float* __restrict__ dqg,
-                                                           float* __restrict__ dkg) {
-    __shared__ double red[16][17];
+// dg[i] = sum over the n workgroups of part[w][i], in a fixed order (fp64: up to 1024 terms).  16 outputs per workgroup, 64 threads each, so
+// that a thread's share of the terms is loaded at once.
+__global__ __launch_bounds__(1024) void qk_rope_gain_kernel(const float* __restrict__ part, int n, int hd, float* __restrict__ dqg,
+                                                            float* __restrict__ dkg) {
+    __shared__ double red[64][17];
     const int c = threadIdx.x & 15, s = threadIdx.x >> 4, i = blockIdx.x * 16 + c;
     double a = 0;
-    for (int w = s; w < n; w += 16) a += part[(size_t)w * (2 * hd) + i];
+    for (int w = s; w < n; w += 64 * 8) {
+        float f[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] = part[(size_t)min(w + 64 * k, n - 1) * (2 * hd) + i];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) a += w + 64 * k < n ? f[k] : 0.f;
+    }
     red[s][c] = a;
-    __syncthreads();
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        __syncthreads();
+        if (s < o) red[s][c] = a += red[s + o][c];
+    }
     if (s == 0) {
-        for (int w = 1; w < 16; ++w) a += red[w][c];
         float* out = i < hd ? dqg : dkg;
         if (out) out[i < hd ? i : i - hd] = (float)a;
     }
@@ -262,7 +296,7 @@ extern "C" int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t 
     if (rows) launch<true>(dtype, hd, p, dim3(groups), st);
     PGT_LAUNCH_CHECK();
     if (dq_gain || dk_gain)
-        hipLaunchKernelGGL(qk_rope_gain_kernel, dim3(2 * hd / 16), dim3(256), 0, st, p.part, groups, hd, dq_gain, dk_gain);
+        hipLaunchKernelGGL(qk_rope_gain_kernel, dim3(2 * hd / 16), dim3(1024), 0, st, p.part, groups, hd, dq_gain, dk_gain);
     PGT_LAUNCH_CHECK();
     return 0;
 }
