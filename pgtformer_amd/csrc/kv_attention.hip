@@ -397,7 +397,17 @@ template <typename T, int HD, int ROWS> __global__ __launch_bounds__(256) void k
     store4((T*)p.out + (s.r0 + qc / p.group) * p.ldo + (sg.hk * p.group + qc % p.group) * HD + 4 * c, f);
 }
 
-// How a call is run: column tiles of 16 (this file) or 256 (kv_attention_rows.hip), and the workgroups that share the work
+// How a call is run: column tiles of 16 (this file) or 256 (kv_attention_rows.hip), and the workgroups that share the work (0: one per column
+// tile, no join).  Lengths are only known on the device; the table's width bounds them.
+//
+// 256 columns, in units of a tile's time (2.2 us at hd 128, 1.6 at 64): one workgroup per column tile takes ceil(segs / 256) * tiles + 4, of
+// ragged lengths some 1.25 times that; shared, segs * tiles / 256 + 16 for the look-up, second segments and the join.  Shared against not, us: 8
+// segments of 64 tiles 32 / 101 (hd 64), 40 / 126 (128); 64 of 8: 36 / 20, 48 / 26; 256 of 32: 80 / 59, 107 / 79; 256 of 160 and 512 of 128,
+// ragged: 172 / 230, 437 / 559.  From 1024 segments on the dispatch evens lengths out by itself: 16 tiles 139 / 125, 202 / 163, 128 tiles 798 /
+// 784, 1163 / 1110.
+// 16 columns: the whole chip does a tile of 1024 segments in about that unit.  16 columns against 256, us: 1 sequence of 65536, 64 columns 52 / 67
+// (hd 64), 49 / 77 (128), 128 columns 92 / 71, 79 / 81; 16 of 8192, 128 columns 160 / 94, 169 / 119; 64 of 1024, 64 columns 34 / 60, 54 / 79,
+// 128 columns 63 / 64, 100 / 86, 256 columns 116 / 80, 194 / 110; 4 of 700, 256 columns 10 / 30, 13 / 39.
 struct Way {
     int cshift, wgs;
     size_t segs, slots;      // column tiles of the launch; slots of partial results
@@ -405,21 +415,26 @@ struct Way {
 Way way_of(int dtype, int B, int max_new, int kv, int group, int hd, int width, int pshift, int causal, int window) {
     Way w;
     const int64_t cols = (int64_t)max_new * group;
-    w.cshift = dtype != PGT_F32 && cols >= 64 ? 8 : 4;
-    w.segs = (size_t)B * kv * ((cols + (1 << w.cshift) - 1) >> w.cshift);
     int64_t tiles = (((int64_t)width << pshift) + 63) / 64;
     if (causal && window) {      // from the first query's first token to the last one's last
         const int64_t n = ((int64_t)window + causal + max_new + 63) / 64 + 1;
         if (n < tiles) tiles = n;
     }
-    if (w.cshift != 4) {
-        w.wgs = 256;
-        if (w.segs >= 1024 || tiles <= MIN_SHARE) w.wgs = 0;
+    const int64_t few = (int64_t)B * kv * ((cols + 15) >> 4), many = (int64_t)B * kv * ((cols + 255) >> 8);
+    const double alone = 1.25 * ((many + 255) / 256) * tiles + 4, shared = (double)many * tiles / 256 + 16;
+    const bool share = many < 1024 && shared < alone;
+    if (dtype != PGT_F32 && (double)few * tiles / 1024 > (share ? shared : alone)) {
+        w.cshift = 8;
+        w.segs = many;
+        w.wgs = share ? 256 : 0;
     } else {
-        // as many as run at once (hd 64: 3 per CU, 128: 2), or one per column tile, without a join, where no sequence can be longer than
-        // 16 tiles or there are so many column tiles that the chip is full anyway
+        // Shared by as many as run at once (hd 64: 3 per CU, 128: 2), unless sequences are short or there are enough segments to even their
+        // lengths out.  Shared against not, us: 8 segments of 16 tiles 12 / 8.5 (hd 64), 12 / 10 (128), of 64: 12 / 21, 13 / 27; 128 of 32: 20 / 13,
+        // 19 / 17; 512 of 64: 54 / 43, 87 / 82, ragged 384 of 128: 95 / 106; 2048 of 32: 102 / 83, 180 / 165.
+        w.cshift = 4;
+        w.segs = few;
         w.wgs = hd == 64 ? 768 : 512;
-        if (tiles <= 4 * NW || w.segs == 0 || w.segs >= 4096) w.wgs = 0;
+        if (tiles <= (few >= 128 ? 32 : 16) || few >= 2048 || few == 0) w.wgs = 0;
     }
     w.slots = w.wgs ? w.wgs + w.segs : 0;
     return w;
@@ -473,7 +488,7 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     const size_t wgs = w.wgs ? w.wgs : w.segs;
     PGT_CHECK(w.segs < (1ULL << 31), "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
     if (w.wgs) {
-        PGT_CHECK((double)w.segs * (((int64_t)width << p.pshift) / 64 + 1) < 2147483648.0,
+        PGT_CHECK((double)w.segs * (((int64_t)width << p.pshift) / 64 + 1) < 1073741824.0,
                   "kv_attention: %d sequences of up to %d pages of %d tokens exceed one launch", B, width, page);
         const size_t need = bytes_of(w, hd);
         PGT_CHECK(workspace && workspace_bytes >= need && ((uintptr_t)workspace & 15) == 0,
