@@ -333,68 +333,98 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     }
 }
 
-// out = the pieces' results against their common reference, for the segments that were cut (and zeros where nothing is seen).  A workgroup
-// takes ROWS rows of a segment: HD / 4 threads hold a row, and with ROWS = 1 the rest take other pieces, four loads in flight each.
+// out = the pieces' results against their common reference, for the segments that were cut (and zeros where nothing is seen).  HD / 4 threads
+// hold a row.  Few pieces, many rows (the 256-column kernel: a segment is cut once or twice): a thread adds up ROWS rows at once, so that their
+// loads are in flight together (one at a time: 30 us, four 18, eight 20 for 512 segments of 256 rows, hd 128).
 constexpr int MAX_WGS = 768;
-template <typename T, int HD, int ROWS> __global__ __launch_bounds__(256) void kv_attn_join_kernel(const AttnP p) {
-    constexpr int LP = HD / 4, NS = 256 / (LP * ROWS);
-    static_assert(LP * ROWS * NS == 256 && (NS == 1 || ROWS == 1), "either rows or pieces side by side");
-    const int tid = threadIdx.x, chunks = p.jrows / ROWS;
-    const int e = blockIdx.x / chunks, r0 = blockIdx.x % chunks * ROWS;
-    const Segment sg = segment_of(p, p.cshift == 4, e);
+template <typename T, int HD> __device__ __forceinline__ void store_row(const AttnP& p, const Segment& sg, const Seq& s, int qc, int c, const f32x4& o, float l) {
+    float f[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f[q] = l == 0.f ? 0.f : o[q] / l;
+    store4((T*)p.out + (s.r0 + qc / p.group) * p.ldo + (sg.hk * p.group + qc % p.group) * HD + 4 * c, f);
+}
+template <typename T, int HD, int ROWS> __global__ __launch_bounds__(256) void kv_attn_join_rows_kernel(const AttnP p) {
+    constexpr int LP = HD / 4, SIDE = 256 / LP, WG_ROWS = SIDE * ROWS;      // rows side by side, rows of a workgroup
+    const int chunks = (1 << p.cshift) / WG_ROWS;
+    const int e = blockIdx.x / chunks, r0 = blockIdx.x % chunks * WG_ROWS;
+    const Segment sg = segment_of(p, 0, e);
     const Seq s = seq_of(p, sg.b);
     const int c0 = (sg.ct << p.cshift) + r0, cols = s.n * p.group;
     if (c0 >= cols) return;
     const int2 ends = sg.tiles > 0 ? p.ends[e] : make_int2(0, -1);
     const int w0 = ends.x, n = ends.y - w0 + 1;
     if (n == 1) return;
-    const int c = tid % LP, row = ROWS > 1 ? tid / LP : 0, qc = c0 + row;
-    const size_t at = (((size_t)w0 + e) << p.cshift) + r0 + row;      // the next piece is in the next slot
+    const int c = threadIdx.x % LP, row = threadIdx.x / LP;
+    size_t at = (((size_t)w0 + e) << p.cshift) + r0 + row;      // the next piece is in the next slot
+    float l[ROWS], m[ROWS];
+    f32x4 o[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) l[k] = 0.f, m[k] = NEVER, o[k] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < n; ++i, at += (size_t)1 << p.cshift) {
+        float2 w[ROWS];
+        f32x4 x[ROWS];
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {      // (rows behind the last are slots nobody wrote: not stored)
+            w[k] = reinterpret_cast<const float2*>(p.pml)[at + SIDE * k];
+            x[k] = reinterpret_cast<const f32x4*>(p.po)[(at + SIDE * k) * LP + c];
+        }
+#pragma unroll
+        for (int k = 0; k < ROWS; ++k) {
+            const float mn = fmaxf(m[k], w[k].x), a = exp2_(m[k] - mn), b = exp2_(w[k].x - mn);
+            l[k] = l[k] * a + w[k].y * b;
+            o[k] = o[k] * a + x[k] * b;
+            m[k] = mn;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+        const int qc = c0 + row + SIDE * k;
+        if (qc < cols) store_row<T, HD>(p, sg, s, qc, c, o[k], l[k]);
+    }
+}
+// Many pieces, few rows: a workgroup per row, the pieces side by side, four loads in flight each.
+template <typename T, int HD> __global__ __launch_bounds__(256) void kv_attn_join_kernel(const AttnP p) {
+    constexpr int LP = HD / 4, NS = 256 / LP;
+    const int tid = threadIdx.x, e = blockIdx.x / p.jrows, r0 = blockIdx.x % p.jrows;
+    const Segment sg = segment_of(p, 1, e);
+    const Seq s = seq_of(p, sg.b);
+    const int qc = (sg.ct << 4) + r0;
+    if (qc >= s.n * p.group) return;
+    const int2 ends = sg.tiles > 0 ? p.ends[e] : make_int2(0, -1);
+    const int w0 = ends.x, n = ends.y - w0 + 1;
+    if (n == 1) return;
+    const int c = tid % LP, k = tid / LP;
+    const size_t at = (((size_t)w0 + e) << 4) + r0;
     const float2* ml = reinterpret_cast<const float2*>(p.pml) + at;
     const f32x4* po = reinterpret_cast<const f32x4*>(p.po + at * HD) + c;
     float l = 0.f, m = NEVER;
     f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-    if constexpr (ROWS > 1) {
-        if (qc >= cols) return;
-        for (int i = 0; i < n; ++i) m = fmaxf(m, ml[(size_t)i << p.cshift].x);
-        for (int i = 0; i < n; ++i) {
-            const float2 w = ml[(size_t)i << p.cshift];
-            const float a = exp2_(w.x - m);
-            l += w.y * a;
-            o += po[((size_t)i << p.cshift) * LP] * a;
-        }
-    } else {
-        __shared__ float al[MAX_WGS];
-        __shared__ f32x4 so[NS][LP];
-        __shared__ float sm[4], sl[4];
-        for (int i = tid; i < n; i += 256) m = fmaxf(m, ml[(size_t)i << p.cshift].x);
-        m = wave_max(m);
-        if ((tid & 63) == 0) sm[tid >> 6] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-        for (int i = tid; i < n; i += 256) {
-            const float2 w = ml[(size_t)i << p.cshift];
-            const float a = exp2_(w.x - m);
-            al[i] = a;
-            l += w.y * a;
-        }
-        l = wave_sum(l);
-        if ((tid & 63) == 0) sl[tid >> 6] = l;
-        __syncthreads();
-        l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
-        const int k = tid / LP;
-#pragma unroll 4
-        for (int i = k; i < n; i += NS) o += po[((size_t)i << p.cshift) * LP] * al[i];
-        so[k][c] = o;
-        __syncthreads();
-        if (k) return;
-#pragma unroll
-        for (int i = 1; i < NS; ++i) o += so[i][c];
+    __shared__ float al[MAX_WGS];
+    __shared__ f32x4 so[NS][LP];
+    __shared__ float sm[4], sl[4];
+    for (int i = tid; i < n; i += 256) m = fmaxf(m, ml[(size_t)i << 4].x);
+    m = wave_max(m);
+    if ((tid & 63) == 0) sm[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+    for (int i = tid; i < n; i += 256) {
+        const float2 w = ml[(size_t)i << 4];
+        const float a = exp2_(w.x - m);
+        al[i] = a;
+        l += w.y * a;
     }
-    float f[4];
+    l = wave_sum(l);
+    if ((tid & 63) == 0) sl[tid >> 6] = l;
+    __syncthreads();
+    l = (sl[0] + sl[1]) + (sl[2] + sl[3]);
+#pragma unroll 4
+    for (int i = k; i < n; i += NS) o += po[((size_t)i << 4) * LP] * al[i];
+    so[k][c] = o;
+    __syncthreads();
+    if (k) return;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) f[q] = l == 0.f ? 0.f : o[q] / l;
-    store4((T*)p.out + (s.r0 + qc / p.group) * p.ldo + (sg.hk * p.group + qc % p.group) * HD + 4 * c, f);
+    for (int i = 1; i < NS; ++i) o += so[i][c];
+    store_row<T, HD>(p, sg, s, qc, c, o, l);
 }
 
 // How a call is run: column tiles of 16 (this file) or 256 (kv_attention_rows.hip), and the workgroups that share the work (0: one per column
@@ -500,13 +530,14 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     hipStream_t st = (hipStream_t)stream;
     if (w.cshift != 4)
         if (const int rc = pgt_kv_attention_rows_launch(&p, dtype == PGT_BF16, hd, (unsigned)wgs, st)) return rc;
+    constexpr int JR = 4;
 #define ATTN_GO(TT, HD_)                                                                                              \
     do {                                                                                                              \
         if (w.cshift != 4) {}                                                                                         \
         else if (p.nct == 1) hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, true>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p); \
         else hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, false>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);      \
-        if (p.wgs && w.cshift == 4) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_, 1>), dim3((unsigned)(w.segs * p.jrows)), dim3(256), 0, st, p); \
-        else if (p.wgs) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_, 1024 / HD_>), dim3((unsigned)(w.segs * (HD_ / 4))), dim3(256), 0, st, p); \
+        if (p.wgs && w.cshift == 4) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)(w.segs * p.jrows)), dim3(256), 0, st, p); \
+        else if (p.wgs) hipLaunchKernelGGL((kv_attn_join_rows_kernel<TT, HD_, JR>), dim3((unsigned)(w.segs * (HD_ / 4 / JR))), dim3(256), 0, st, p); \
     } while (0)
 #define ATTN_HD(TT)                                                                                                   \
     do {                                                                                                              \
