@@ -69,34 +69,36 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         auto page_index = [&](int t, int k) { return (t * 64 + 16 * k) >> p.pshift; };
         auto ok = [&](int i) { return i >= 0 && i < p.pages; };
         char* ring = rings + wave * 3 * SET;
+        // where this lane's bytes of K, V and of the scales / the table (lanes 0, 1 / 2) lie in a page
         const uint32_t k_at = (uint32_t)((lane >> 4) * page + (lane & 15)) * 16 + (BOTH ? (uint32_t)(part * 4 * page * 16) : 0u);
         const uint32_t v_at = (uint32_t)(lane + (BOTH ? 64 * part : 0)) * 16;
-        auto fetch = [&](int slot, int t, int pg0) {      // block blk of tile t, in page pg0 (behind the last tile, or missing: page 0, not looked at)
-            const int pg = (ok(pg0) & (t < te)) ? pg0 : 0;
-            const int tok = (t * 64 + 16 * blk) & (page - 1);
-            const size_t at = pg * stride + hk * page_bytes, one = (size_t)pg * p.kv + hk;
-            const uint8_t *kb = p.kp + (at + tok * 16) + k_at, *vb = p.vp + (at + (size_t)tok * HD) + v_at;
+        const uint8_t *kb = p.kp + hk * page_bytes + k_at, *vb = p.vp + hk * page_bytes + v_at;
+        const uint8_t* base = BOTH || part == 0 ? kb : vb;
+        const uint8_t* word = (const uint8_t*)((lane == 0 ? p.ks : p.vs) + hk);
+        uint32_t word_step = (uint32_t)p.kv * 4;
+        if (lane == 2) word = (const uint8_t*)tab, word_step = 4;
+        auto fetch = [&](int slot, int t, int pg0, bool here) {      // block blk of tile t, in page pg0 (not here: page 0, not looked at)
+            const uint32_t pg = here ? (uint32_t)pg0 : 0u;
+            const uint32_t tok = (uint32_t)((t * 64 + 16 * blk) & (page - 1));
             const uint32_t to = lds_address(ring + slot * SET);
-            lds_load16(BOTH || part == 0 ? kb : vb, to);
-            if constexpr (BOTH) lds_load16(vb, to + 1024);
-            const void* w = lane == 0 ? (const void*)(p.ks + one) : (const void*)(p.vs + one);
-            if (lane == 2) w = tab + min(page_index(t + 3, blk), p.width - 1);
-            lds_load4(w, to + SET - 256);
+            const uint32_t k_off = tok * 16, v_off = tok * HD;
+            lds_load16(base + (uint64_t)pg * (uint32_t)stride + (BOTH || part == 0 ? k_off : v_off), to);
+            if constexpr (BOTH) lds_load16(vb + (uint64_t)pg * (uint32_t)stride + v_off, to + 1024);
+            const uint32_t i = lane == 2 ? (uint32_t)min(page_index(t + 3, blk), p.width - 1) : pg;
+            lds_load4(word + (uint64_t)i * word_step, to + SET - 256);
         };
         bool have0 = false, have1 = false, have2 = false;      // whether the next three tiles have a page
         if (t0 < te) {      // the first three tiles are on their way while the columns are set up
             int pg[3];
 #pragma unroll
-            for (int i = 0; i < 3; ++i) {
-                const int k = page_index(t0 + i, blk);
-                pg[i] = uni(tab[min(k, p.width - 1)]);
-                if (k >= p.width) pg[i] = -1;
-            }
-            have0 = ok(pg[0]);
-            have1 = ok(pg[1]) & (t0 + 1 < te);
-            have2 = ok(pg[2]) & (t0 + 2 < te);
-#pragma unroll
-            for (int i = 0; i < 3; ++i) fetch(i, t0 + i, pg[i]);
+            for (int i = 0; i < 3; ++i) pg[i] = tab[min(page_index(t0 + i, blk), p.width - 1)];
+            auto there = [&](int i) { return ok(pg[i]) & (t0 + i < te) & (page_index(t0 + i, blk) < p.width); };
+            have0 = there(0);
+            have1 = there(1);
+            have2 = there(2);
+            fetch(0, t0, pg[0], have0);
+            fetch(1, t0 + 1, pg[1], have1);
+            fetch(2, t0 + 2, pg[2], have2);
         }
 
         // this wave's columns: what every one of them sees, and what any of them does
@@ -131,19 +133,24 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         // token 16 hh + e of a 32-token half -> the row of S^T whose score ends up in register e of lane half hh
         const int k_to = (((lane >> 4) + (BOTH ? 4 * part : 0)) * 128 + 32 * (blk >> 1) + (lane & 3) + 8 * ((lane & 15) >> 2) + 4 * (blk & 1)) * 16;
         const int v_to = KB + (blk * 2 * HD + lane + (BOTH ? 64 * part : 0)) * 16;
-        auto convert = [&](int st, int t) {      // set st = tile t -> stage st; then the set is fetched again, for tile t + 3
+        uint4 ra, rb;      // a set, read before the product that hides its way
+        float rscale;
+        int rnext;
+        auto take = [&](int set) {
+            const char* in = ring + set * SET;
+            ra = *reinterpret_cast<const uint4*>(in + lane * 16);
+            if constexpr (BOTH) rb = *reinterpret_cast<const uint4*>(in + 1024 + lane * 16);
+            rscale = *reinterpret_cast<const float*>(in + SET - 256 + (lane & 1) * 4);
+            rnext = *reinterpret_cast<const int*>(in + SET - 256 + 8);
+        };
+        auto convert = [&](int st, int t) {      // the set taken, of tile t -> stage st; then the set is fetched again, for tile t + 3
             char* d = smem + st * STAGE;
-            const char* in = ring + st * SET;
-            const uint4 a = *reinterpret_cast<const uint4*>(in + lane * 16);
-            uint4 w = a;
-            if constexpr (BOTH) w = *reinterpret_cast<const uint4*>(in + 1024 + lane * 16);
-            const float scale = *reinterpret_cast<const float*>(in + SET - 256 + (lane & 1) * 4);
-            const int next = *reinterpret_cast<const int*>(in + SET - 256 + 8);
             if (BOTH || part == 0) {
-                *reinterpret_cast<uint4*>(d + k_to) = HQ ? half8(a.x, a.y) : bfloat8(a.x, a.y);
-                *reinterpret_cast<uint4*>(d + k_to + 1024) = HQ ? half8(a.z, a.w) : bfloat8(a.z, a.w);
+                *reinterpret_cast<uint4*>(d + k_to) = HQ ? half8(ra.x, ra.y) : bfloat8(ra.x, ra.y);
+                *reinterpret_cast<uint4*>(d + k_to + 1024) = HQ ? half8(ra.z, ra.w) : bfloat8(ra.z, ra.w);
             }
             if (BOTH || part == 1) {
+                uint4 w = BOTH ? rb : ra;
                 if (((t * 64 < all_lo) | (t * 64 + 64 > all_hi)) & (t < te)) {
                     // NaN times the weight 0 of a query that does not see the token: zeros here, see the end
                     const uint4 n = make_uint4(nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w));
@@ -154,16 +161,14 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 *reinterpret_cast<uint4*>(d + v_to + HD * 16) = half8(w.z, w.w);
             }
             if (lane < 2 && part == 0) {      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
-                const float factor = have0 ? fmaxf(fabsf(p.c) * scale, 1e-30f) : -1.f, ev = (float)((int)((__float_as_uint(scale) >> 23) & 255) - 127);
+                const float factor = have0 ? fmaxf(fabsf(p.c) * rscale, 1e-30f) : -1.f, ev = (float)((int)((__float_as_uint(rscale) >> 23) & 255) - 127);
                 reinterpret_cast<float*>(&sscale[st][blk])[lane] = lane ? ev : factor;
             }
             // pages of the tiles ahead, and whether they are there
-            const int pn = page_index(t + 3, blk) < p.width ? uni(next) : -1;
             have0 = have1;
             have1 = have2;
-            have2 = ok(pn) & (t + 3 < te);
-            wait_lds();      // the set is read
-            fetch(st, t + 3, pn);
+            have2 = ok(rnext) & (t + 3 < te) & (page_index(t + 3, blk) < p.width);
+            fetch(st, t + 3, rnext, have2);      // (the set is in registers: what is above needed them)
         };
         auto k_operand = [&](int st, int sb, int k) {
             return *reinterpret_cast<const uint4*>(smem + st * STAGE + (sb * 32 + r + 64 * h) * 16 + k * 2048);
@@ -186,12 +191,20 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             tm = top(x);
         };
         // softmax of the scores x of half sb of tile t (stage st) and their product with V; xn = the scores of half nsb of stage nst (behind the
-        // last tile: of whatever is there, unused).  Nothing moves over a SLICE; operands are read four products ahead.
+        // last tile: of whatever is there, unused); half fsb of stage fst is what the step after this one begins with.  Nothing moves over a SLICE;
+        // operands are read four products ahead, from one step into the next.  The barrier of a tile stands in the middle of its first step.
 #define SLICE() __builtin_amdgcn_sched_barrier(0)
-        auto step = [&](int t, int st, int sb, int nst, int nsb, f32x16& x, f32x16& xn) {
+        uint4 f[4];      // operands in flight: the first of the step's S^T at its start
+        auto ahead = [&](int st, int sb) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = k_operand(st, sb, k);
+        };
+        auto step = [&](int t, int st, int sb, int nst, int nsb, int fst, int fsb, f32x16& x, f32x16& xn) {
             const int tok = t * 64 + sb * 32;
             if (tok >= hi_z || tok + 32 <= lo_a) {
                 if (cw < cols) scores(nst, nsb, xn);
+                if (sb == 0) __syncthreads();
+                ahead(fst, fsb);
                 return;
             }
             const float ck = fabsf(sc.x), ev = sc.y;
@@ -219,9 +232,6 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 pw[i] = f2h2_nosat(exp2_(__builtin_fmaf(x[2 * i], ck, em)), exp2_(__builtin_fmaf(x[2 * i + 1], ck, em)));
                 ls = __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, pw[i]), ones, ls, false);
             };
-            uint4 f[4];      // operands in flight
-#pragma unroll
-            for (int k = 0; k < 4; ++k) f[k] = k_operand(nst, nsb, k);
             const float2 scn = sscale[nst][nsb * 2 + h];
             SLICE();
 #pragma unroll
@@ -233,13 +243,14 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 for (int i = 0; i < 8 / KS; ++i) weight2(k * (8 / KS) + i);
                 SLICE();
             }
+            if (sb == 0) __syncthreads();      // the next tile's stage is written
             sc = scn;
             float mx = 0.f;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {      // O^T, the largest of the next scores
                 const int k = i / ND, d = i % ND;
                 o[d] = mma16<half_t>(f[i % 4], make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]), o[d]);
-                if (i + 4 < NV) f[i % 4] = v_operand(st, sb, i + 4);
+                f[i % 4] = i + 4 < NV ? v_operand(st, sb, i + 4) : k_operand(fst, fsb, i + 4 - NV);
                 if (i == 0) mx = fmaxf(xn[0], xn[1]);
 #pragma unroll
                 for (int q = i == 0 ? 2 : 16 / NV * i; q < 16 / NV * (i + 1); ++q) mx = fmaxf(mx, xn[q]);
@@ -255,18 +266,22 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         __syncthreads();
         if (t0 < te) {
             wait_loads<2 * NL>();
+            take(0);
             convert(0, t0);
+            wait_loads<2 * NL>();
+            take(1);
             __syncthreads();
             f32x16 xa, xb;
             if (cw < cols) scores(0, 0, xa);
+            ahead(0, 1);
             int st = 0;
             for (int t = t0; t < te; ++t) {
                 const int nst = st == 2 ? 0 : st + 1;
-                step(t, st, 0, st, 1, xa, xb);
-                wait_loads<2 * NL>();      // the set of tile t + 1 is here, those of t + 2, t + 3 on the way
                 convert(nst, t + 1);      // (the stage was last read in tile t - 2, which every wave left before the last barrier)
-                __syncthreads();
-                step(t, st, 1, nst, 0, xb, xa);
+                step(t, st, 0, st, 1, nst, 0, xa, xb);
+                wait_loads<2 * NL>();      // the set of tile t + 2 is here, those of t + 3, t + 4 on the way
+                take(nst == 2 ? 0 : nst + 1);
+                step(t, st, 1, nst, 0, nst, 1, xb, xa);
                 st = nst;
             }
             wait_loads<0>();
