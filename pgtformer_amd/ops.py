@@ -1054,14 +1054,10 @@ def _pointers(*ts):
     dev = ts[0].get_device()
     if dev < 0 or dev != torch._C._cuda_getDevice():
         _dev(ts[0])
-    out = []
     for t in ts:
-        if t is None:
-            out.append(None)
-        elif t.get_device() != dev:
+        if t is not None and t.get_device() != dev:
             raise hip.PgtError("pgtformer_amd ops run on one GPU: tensors on %s and %s" % (ts[0].device, _dev(t).device))
-        else:
-            out.append(t.data_ptr())
+    out = [None if t is None else t.data_ptr() for t in ts]
     out.append(torch._C._cuda_getCurrentRawStream(dev))
     return out
 
@@ -1124,7 +1120,7 @@ def _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, wha
     _f32_vec(q_gain, hd, what + ": q_gain")
     _f32_vec(k_gain, hd, what + ": k_gain")
     if out is None:
-        qo, ko = (torch.empty((rows, n * hd), device=q.device, dtype=q.dtype) for n in (heads, kv_heads))
+        qo, ko = q.new_empty((rows, cols)), q.new_empty((rows, kv_heads * hd))
         return rows, hd, rot, qo, ko, ldq, ldk, cols, kv_heads * hd
     qo, ko = out
     _need(qo.dtype is q.dtype and ko.dtype is q.dtype and qo.shape[0] == rows and ko.shape[0] == rows, "%s: outputs of another type or length", what)
@@ -1154,10 +1150,10 @@ def qk_norm_rope_backward(dq, dk, q, k, positions, freqs, q_gain=None, k_gain=No
     lddq, lddk = _rows(dq, heads * hd, what + ": dq"), _rows(dk, kv_heads * hd, what + ": dk")
     if out is not None:
         _apart((qo, ko), (dq, dk, q, k), what)
-    gains = torch.empty((2, hd), device=q.device, dtype=torch.float32)
+    gains = q.new_empty((2, hd), dtype=torch.float32)
     L = hip.lib()
     nbytes = L.pgt_qk_norm_rope_backward_workspace_bytes(rows, hd)
-    ws = torch.empty(nbytes // 4, device=q.device, dtype=torch.float32)
+    ws = q.new_empty(nbytes // 4, dtype=torch.float32)
     gq, gk = gains.unbind(0)
     pdq, pdk, pq, pk, pp, pf, pqg, pkg, pqo, pko, pgq, pgk, pws, st = _pointers(dq, dk, q, k, positions, freqs, q_gain, k_gain, qo, ko, gq, gk, ws)
     with _profiled("qk_norm_rope_backward", 17.0 * rows * (heads + kv_heads) * hd, dq, dk, q, k, qo, ko):
@@ -1173,13 +1169,17 @@ class KvCache:
     __slots__ = ("k_pages", "v_pages", "k_scale", "v_scale", "pages", "page", "kv_heads", "hd")
 
     def __init__(self, k_pages, v_pages, k_scale, v_scale):
-        _need(k_pages.dim() == 5 and k_pages.shape[4] == 16, "KvCache: k_pages %s, (pages, kv_heads, hd / 16, page, 16) wanted", tuple(k_pages.shape))
-        n, kv, c, page, _ = k_pages.shape
-        _need(v_pages.shape == (n, kv, page // 16, 16 * c, 16), "KvCache: v_pages %s do not belong to k_pages %s", tuple(v_pages.shape),
-              tuple(k_pages.shape))
-        _need(k_scale.shape == (n, kv) and v_scale.shape == (n, kv), "KvCache: one scale per page and kv head wanted")
-        for t, want in ((k_pages, torch.uint8), (v_pages, torch.uint8), (k_scale, torch.float32), (v_scale, torch.float32)):
-            _need(t.dtype == want and t.is_contiguous(), "KvCache: contiguous uint8 pages and float32 scales wanted")
+        shape = k_pages.shape
+        if len(shape) != 5 or shape[4] != 16:
+            raise hip.PgtError("KvCache: k_pages %s, (pages, kv_heads, hd / 16, page, 16) wanted" % (tuple(shape),))
+        n, kv, c, page, _ = shape
+        if v_pages.shape != (n, kv, page // 16, 16 * c, 16):
+            raise hip.PgtError("KvCache: v_pages %s do not belong to k_pages %s" % (tuple(v_pages.shape), tuple(shape)))
+        if k_scale.shape != (n, kv) or v_scale.shape != (n, kv):
+            raise hip.PgtError("KvCache: one scale per page and kv head wanted")
+        if not (k_pages.dtype is v_pages.dtype is torch.uint8 and k_scale.dtype is v_scale.dtype is torch.float32 and k_pages.is_contiguous() and
+                v_pages.is_contiguous() and k_scale.is_contiguous() and v_scale.is_contiguous()):
+            raise hip.PgtError("KvCache: contiguous uint8 pages and float32 scales wanted")
         self.k_pages, self.v_pages, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
         self.pages, self.page, self.kv_heads, self.hd = n, page, kv, 16 * c
 
@@ -1218,7 +1218,8 @@ def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
     rows = k.shape[0]
     B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_append")
     n = cache.kv_heads * cache.hd
-    _need(k.dtype == v.dtype and v.shape[0] == rows, "kv_append: k %s %s, v %s %s", tuple(k.shape), k.dtype, tuple(v.shape), v.dtype)
+    if k.dtype is not v.dtype or v.shape[0] != rows:
+        raise hip.PgtError("kv_append: k %s %s, v %s %s" % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
     ldk, ldv = _rows(k, n, "kv_append: k"), _rows(v, n, "kv_append: v")
     pk, pv, kp, vp, ks, vs, pt, pl, pc, st = _pointers(k, v, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, lens, cu)
     with _profiled("kv_append", 8.0 * rows * n, k, v, more=2 * rows * n):
@@ -1232,7 +1233,7 @@ def kv_read(cache, table, start, rows, dtype, cu=None, *, max_rows=None, out=Non
     n = cache.kv_heads * cache.hd
     B, width, ldt, most = _seq_args(table, start, cu, rows, max_rows, "kv_read")
     if out is None:
-        ko, vo = (torch.empty((rows, n), device=cache.k_pages.device, dtype=dtype) for _ in range(2))
+        ko, vo = (cache.k_pages.new_empty((rows, n), dtype=dtype) for _ in range(2))
         ldk = ldv = n
     else:
         ko, vo = out
@@ -1255,7 +1256,7 @@ def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=
     B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_attention")
     ldq = _rows(q, heads * hd, "kv_attention: q")
     if out is None:
-        out, ldo = torch.empty((rows, heads * hd), device=q.device, dtype=q.dtype), heads * hd
+        out, ldo = q.new_empty((rows, heads * hd)), heads * hd
     else:
         _need(out.dtype == q.dtype and out.shape[0] == rows, "kv_attention: output of another type or length")
         ldo = _rows(out, heads * hd, "kv_attention: out")
