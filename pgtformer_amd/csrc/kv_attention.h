@@ -23,6 +23,24 @@ __device__ __forceinline__ f32x4 mma_h(const uint4& a, const uint4& b, const f32
 __device__ __forceinline__ f32x4 mma_b(const uint4& a, const uint4& b, const f32x4& c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
+// 8 floats as three bf16 planes: hi + mid + lo is the float but for 2^-25 of it
+__device__ __forceinline__ void split3(const float* p, uint4& hi, uint4& mid, uint4& lo) {
+    float f[8];
+    *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(p);
+    *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(p + 4);
+#pragma unroll
+    for (int pl = 0; pl < 3; ++pl) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            w[e] = f2bf2(f[2 * e], f[2 * e + 1]);
+            x3_opaque(w[e]);
+            f[2 * e] -= __uint_as_float(w[e] << 16);
+            f[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+        }
+        (pl == 0 ? hi : pl == 1 ? mid : lo) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // does any of the four codes stand for NaN (0x7f, 0xff)?
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
@@ -174,5 +192,5 @@ __device__ __forceinline__ bool part_of(const AttnP& p, int wg, int& pos, int& e
 
 }  // namespace
 
-// kv_attention_rows.hip: bf16 / half, column tiles of 256; p is an AttnP
-int pgt_kv_attention_rows_launch(const void* p, int bf16, int hd, unsigned groups, hipStream_t st);
+// kv_attention_rows.hip: column tiles of 256, fp32 at hd 64 only; p is an AttnP
+int pgt_kv_attention_rows_launch(const void* p, int dtype, int hd, unsigned groups, hipStream_t st);

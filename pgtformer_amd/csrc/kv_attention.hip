@@ -79,21 +79,7 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
         const int d = 64 * (st >> 1) + 16 * g + 8 * (st & 1);
         const T* qp = (const T*)p.q + (s.r0 + qi) * p.ldq + head * HD + d;
         if constexpr (F32) {
-            float f[8];
-            *reinterpret_cast<float4*>(f) = *reinterpret_cast<const float4*>(qp);
-            *reinterpret_cast<float4*>(f + 4) = *reinterpret_cast<const float4*>(qp + 4);
-#pragma unroll
-            for (int pl = 0; pl < 3; ++pl) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    w[e] = f2bf2(f[2 * e], f[2 * e + 1]);
-                    x3_opaque(w[e]);
-                    f[2 * e] -= __uint_as_float(w[e] << 16);
-                    f[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
-                }
-                qf[pl][st] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            split3(qp, qf[0][st], qf[1][st], qf[2][st]);
         } else {
             qf[0][st] = *reinterpret_cast<const uint4*>(qp);
         }
@@ -437,7 +423,9 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void kv_attn_joi
 // 784, 1163 / 1110.
 // 16 columns: the whole chip does a tile of 1024 segments in about that unit.  16 columns against 256, us: 1 sequence of 65536, 64 columns 52 / 67
 // (hd 64), 49 / 77 (128), 128 columns 92 / 71, 79 / 81; 16 of 8192, 128 columns 160 / 94, 169 / 119; 64 of 1024, 64 columns 34 / 60, 54 / 79,
-// 128 columns 63 / 64, 100 / 86, 256 columns 116 / 80, 194 / 110; 4 of 700, 256 columns 10 / 30, 13 / 39.
+// 128 columns 63 / 64, 100 / 86, 256 columns 116 / 80, 194 / 110; 4 of 700, 256 columns 10 / 30, 13 / 39.  fp32 (hd 64; at 128 its three planes
+// of q do not fit the registers of a wave of 32 columns): 2 of 8192, 8192 columns 764 / 552; 64 of 1024, 256 columns 170 / 96; 4 of 2048, 512
+// columns 38 / 47.
 struct Way {
     int cshift, wgs;
     size_t segs, slots;      // column tiles of the launch; slots of partial results
@@ -453,7 +441,7 @@ Way way_of(int dtype, int B, int max_new, int kv, int group, int hd, int width, 
     const int64_t few = (int64_t)B * kv * ((cols + 15) >> 4), many = (int64_t)B * kv * ((cols + 255) >> 8);
     const double alone = 1.25 * ((many + 255) / 256) * tiles + 4, shared = (double)many * tiles / 256 + 16;
     const bool share = many < 1024 && shared < alone;
-    if (dtype != PGT_F32 && (double)few * tiles / 1024 > (share ? shared : alone)) {
+    if ((dtype != PGT_F32 || hd == 64) && (double)few * tiles / 1024 > (share ? shared : alone)) {
         w.cshift = 8;
         w.segs = many;
         w.wgs = share ? 256 : 0;
@@ -529,7 +517,7 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     }
     hipStream_t st = (hipStream_t)stream;
     if (w.cshift != 4)
-        if (const int rc = pgt_kv_attention_rows_launch(&p, dtype == PGT_BF16, hd, (unsigned)wgs, st)) return rc;
+        if (const int rc = pgt_kv_attention_rows_launch(&p, dtype, hd, (unsigned)wgs, st)) return rc;
     constexpr int JR = 4;
 #define ATTN_GO(TT, HD_)                                                                                              \
     do {                                                                                                              \

@@ -27,9 +27,14 @@ __device__ __forceinline__ float max_of_halves(float v) {
 
 constexpr int NW = 8, TH = 64 * NW, CT = 32 * NW;      // waves, threads and columns of a workgroup
 
+template <typename T> struct QType { typedef T type; };
+template <> struct QType<float> { typedef bf16_t type; };
+
 template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_rows_kernel(const AttnP p) {
-    constexpr bool HQ = __is_same(T, half_t);
-    constexpr int KS = HD / 16, ND = HD / 32, NV = 2 * ND;      // products of S^T; row blocks of O^T, its products
+    constexpr bool HQ = __is_same(T, half_t), F32 = __is_same(T, float);
+    constexpr int QP = F32 ? 3 : 1;                             // planes of q: fp32 as three bf16
+    using Q = typename QType<T>::type;
+    constexpr int KS = HD / 16, ND = HD / 32, NV = 2 * ND;      // k-steps of S^T; row blocks of O^T, its products
     constexpr int KB = 64 * HD * 2, STAGE = 2 * KB;             // bytes of a K image; of a stage
     __shared__ __attribute__((aligned(16))) char smem[3 * STAGE];
     constexpr int SET = (HD == 128 ? 2048 : 1024) + 256;        // bytes of a set of raw units of one wave
@@ -114,17 +119,26 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         const int qc = min(cw + r, cols - 1);
         int lo, hi;
         sees(p, s.len, shift + qc / p.group, lo, hi);
-        uint4 qf[KS];
+        uint4 qf[QP][KS];
         {
             const uint32_t flip = p.c < 0.f ? 0x80008000u : 0u;      // a negative scale goes into q: the largest score stays the largest weight
             const T* qp = (const T*)p.q + (s.r0 + qc / p.group) * p.ldq + (hk * p.group + qc % p.group) * HD + 8 * h;
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                uint4 w = *reinterpret_cast<const uint4*>(qp + 16 * k);
-                w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
-                qf[k] = w;
+                if constexpr (F32) split3(qp + 16 * k, qf[0][k], qf[1][k], qf[2][k]);
+                else qf[0][k] = *reinterpret_cast<const uint4*>(qp + 16 * k);
+#pragma unroll
+                for (int pl = 0; pl < QP; ++pl) {
+                    uint4& w = qf[pl][k];
+                    w.x ^= flip; w.y ^= flip; w.z ^= flip; w.w ^= flip;
+                }
             }
         }
+        auto mma_s = [&](const uint4& a, int k, f32x16 x) {      // the smallest plane first
+#pragma unroll
+            for (int pl = QP - 1; pl >= 0; --pl) x = mma16<Q>(a, qf[pl][k], x);
+            return x;
+        };
         f32x16 o[ND];
         float m = NEVER, l = 0.f;
 #pragma unroll
@@ -186,7 +200,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         };
         auto scores = [&](int st, int sb, f32x16& x) {
 #pragma unroll
-            for (int k = 0; k < KS; ++k) x = mma16<T>(k_operand(st, sb, k), qf[k], k == 0 ? zero16() : x);
+            for (int k = 0; k < KS; ++k) x = mma_s(k_operand(st, sb, k), k, k == 0 ? zero16() : x);
             sc = sscale[st][sb * 2 + h];
             tm = top(x);
         };
@@ -226,17 +240,24 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             }
             const float em = ev - m;
             float ls = 0.f;
-            uint32_t pw[8];
+            uint32_t pw[8], pl[F32 ? 8 : 1];      // weights in half; fp32: what is left of them, in half
             const halfx2 ones = {(_Float16)1.f, (_Float16)1.f};
             auto weight2 = [&](int i) {      // weights 2 i, 2 i + 1; their sum is that of the rounded ones, as the product's
-                pw[i] = f2h2_nosat(exp2_(__builtin_fmaf(x[2 * i], ck, em)), exp2_(__builtin_fmaf(x[2 * i + 1], ck, em)));
+                const float a = exp2_(__builtin_fmaf(x[2 * i], ck, em)), b = exp2_(__builtin_fmaf(x[2 * i + 1], ck, em));
+                pw[i] = f2h2_nosat(a, b);
+                if constexpr (F32) {
+                    x3_opaque(pw[i]);
+                    const halfx2 w = __builtin_bit_cast(halfx2, pw[i]);
+                    pl[i] = f2h2_nosat(a - (float)w.x, b - (float)w.y);
+                    ls = __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, pl[i]), ones, ls, false);
+                }
                 ls = __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, pw[i]), ones, ls, false);
             };
             const float2 scn = sscale[nst][nsb * 2 + h];
             SLICE();
 #pragma unroll
             for (int k = 0; k < KS; ++k) {      // S^T of the next half, the weights
-                xn = mma16<T>(f[k % 4], qf[k], k == 0 ? zero16() : xn);
+                xn = mma_s(f[k % 4], k, k == 0 ? zero16() : xn);
                 if (k + 4 < KS) f[k % 4] = k_operand(nst, nsb, k + 4);
                 else f[k % 4] = v_operand(st, sb, k + 4 - KS);
 #pragma unroll
@@ -249,6 +270,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
 #pragma unroll
             for (int i = 0; i < NV; ++i) {      // O^T, the largest of the next scores
                 const int k = i / ND, d = i % ND;
+                if constexpr (F32) o[d] = mma16<half_t>(f[i % 4], make_uint4(pl[4 * k], pl[4 * k + 1], pl[4 * k + 2], pl[4 * k + 3]), o[d]);
                 o[d] = mma16<half_t>(f[i % 4], make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]), o[d]);
                 f[i % 4] = i + 4 < NV ? v_operand(st, sb, i + 4) : k_operand(fst, fsb, i + 4 - NV);
                 if (i == 0) mx = fmaxf(xn[0], xn[1]);
@@ -334,8 +356,10 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                             int lq, hq;
                             sees(p, s.len, shift + q / p.group, lq, hq);
                             if (tok + i < lq || tok + i >= hq) continue;
-                            if (whole) store_nan((T*)p.out + (s.r0 + q / p.group) * p.ldo + (hk * p.group + q % p.group) * HD + dim);
-                            else p.po[(((size_t)id + e) * CT + (q & (CT - 1))) * HD + dim] = __builtin_nanf("");
+                            T* op = (T*)p.out + (s.r0 + q / p.group) * p.ldo + (hk * p.group + q % p.group) * HD + dim;
+                            if constexpr (F32) { if (whole) *op = __builtin_nanf(""); }
+                            else if (whole) store_nan(op);
+                            if (!whole) p.po[(((size_t)id + e) * CT + (q & (CT - 1))) * HD + dim] = __builtin_nanf("");
                         }
                     }
                 }
@@ -354,10 +378,12 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
 
 }  // namespace
 
-int pgt_kv_attention_rows_launch(const void* pp, int bf16, int hd, unsigned groups, hipStream_t st) {
+int pgt_kv_attention_rows_launch(const void* pp, int dtype, int hd, unsigned groups, hipStream_t st) {
     const AttnP& p = *(const AttnP*)pp;
 #define ROWS_GO(TT, HD_) hipLaunchKernelGGL((kv_attn_rows_kernel<TT, HD_>), dim3(groups), dim3(TH), 0, st, p)
-    if (bf16) {
+    if (dtype == PGT_F32) {
+        ROWS_GO(float, 64);
+    } else if (dtype == PGT_BF16) {
         if (hd == 64) ROWS_GO(bf16_t, 64);
         else ROWS_GO(bf16_t, 128);
     } else {

@@ -102,6 +102,9 @@ MANY = [
     (1, 8, 32, 64, 64, 313, 100, 1, 0, 0.125, "f16"),        # one long sequence, its segments cut many times
     (2, 8, 64, 128, 32, 70, 300, 1, 0, 0.09, "bf16"),
     (5, 1, 8, 64, 128, 9, 1100, 7, 90, 0.3, "bf16"),         # 35 column tiles, a window in which most rows see two tiles
+    (64, 8, 32, 64, 32, 13, 41, 1, 0, 0.125, "f32"),
+    (33, 8, 32, 64, 64, 16, 63, 16, 600, -0.125, "f32"),
+    (64, 4, 20, 128, 128, 4, 37, 0, 0, 0.09, "f32"),         # (fp32 of 128 dims: 16 columns)
 ]
 
 
@@ -151,7 +154,7 @@ def test_the_cases_reach_both_ways_of_sharing():
     """workspaces tell: some of the cases above run a workgroup per column tile (none), some in pieces (one)"""
     f = hip.lib().pgt_kv_attention_workspace_bytes
     size = [f(ops._dt(torch.empty(0, dtype=DT[c[10]])), c[0], c[6], c[2], c[1], c[3], c[5], c[4], c[7], c[8]) for c in MANY]
-    assert [s > 0 for s in size] == [False, False, False, True, True, False, True, True, True, False], size
+    assert [s > 0 for s in size] == [False, False, False, True, True, False, True, True, True, False, False, True, False], size
 
 
 def test_many_segments_of_few_rows():
