@@ -352,8 +352,9 @@ int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const
  * h / (heads / kv_heads)).  lens: tokens INCLUDING the rows' own: row i of n of sequence b is at position p = lens[b] - n + i.
  *   causal == 0: sees tokens < lens[b].   causal = c >= 1: tokens < e = (p / c + 1) * c (and < lens[b]): c = 1 token by token, c = 1024 the whole
  *   frames of 1024 tokens up to its own.  window = w > 0 (with causal): of these the tokens >= e - w.
- * A row that sees no token is zero.  Deterministic.  workspace: pgt_kv_attention_workspace_bytes(...) bytes (0: may be NULL),
- * scratch of one call - calls that may run concurrently need their own. */
+ * A row that sees no token is zero.  Deterministic for one shape of call (B, max_new, width, window choose how the work is split, and with it
+ * the order of the sums).  width * page <= 2^31 - 2^16.  workspace: pgt_kv_attention_workspace_bytes(...) bytes (0: may be NULL), scratch
+ * of one call - calls that may run concurrently need their own. */
 int pgt_kv_append(int32_t dtype, const void* k, int32_t ldk, const void* v, int32_t ldv, void* k_pages, void* v_pages,
                   float* k_scale, float* v_scale, int32_t pages, int32_t page, int32_t kv_heads, int32_t hd, const int32_t* table,
                   int32_t ld_table, int32_t width, const int32_t* lens, const int32_t* cu, int32_t B, int32_t rows,

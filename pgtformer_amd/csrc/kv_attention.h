@@ -72,8 +72,7 @@ __device__ __forceinline__ Seq seq_of(const AttnP& p, int b) {
         s.r0 = b * p.max_new;
         s.n = p.max_new;
     }
-    const int64_t cap = min((int64_t)p.width << p.pshift, (int64_t)0x7fffff00);
-    s.len = (int)min((int64_t)max(p.lens[b], 0), cap);
+    s.len = min(max(p.lens[b], 0), p.width << p.pshift);
     return s;
 }
 // tokens [lo, hi) that the query at position pos (of a sequence of len tokens) sees

@@ -133,7 +133,8 @@ def test_c_entry_points_refuse():
                                       dict(rows=-1), dict(n=5), dict(width=-1), dict(ldt=1), dict(causal=-1), dict(window=-1), dict(causal=0, window=3),
                                       dict(scale=math.inf), dict(scale=math.nan), dict(kp=None), dict(ks=None), dict(vp=P + 4), dict(q=None),
                                       dict(out=None), dict(lens=None), dict(table=None), dict(ldq=500), dict(ldo=514), dict(out=P + 8),
-                                      dict(width=4000, ldt=4000, ws=None), dict(width=4000, ldt=4000, nb=64), dict(width=4000, ldt=4000, ws=P + 8)])
+                                      dict(width=4000, ldt=4000, ws=None), dict(width=4000, ldt=4000, nb=64), dict(width=4000, ldt=4000, ws=P + 8),
+                                      dict(width=1 << 27, ldt=1 << 27), dict(width=(1 << 27) - 1, ldt=1 << 27), dict(width=1 << 24, ldt=1 << 24, page=128)])
     # nothing to do is not an error (and launches nothing)
     assert entry("pgt_qk_norm_rope", rope, rows=0)[0] == 0
     for name, base in (("pgt_kv_append", kv), ("pgt_kv_read", kv), ("pgt_kv_attention", att)):
