@@ -31,10 +31,10 @@ __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
     return a <= FLT_MAX ? a : 0.f;
 }
-__device__ __forceinline__ float clamp448(float v) { return v > 448.f ? 448.f : (v < -448.f ? -448.f : v); }      // NaN passes
+__device__ __forceinline__ float clamp_to(float v, float top) { return v > top ? top : (v < -top ? -top : v); }      // NaN passes
 __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) {
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(clamp448(a), clamp448(b), 0, false);
-    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamp448(c), clamp448(d), w, true);
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ void value4(uint32_t w, float* f) {
@@ -128,7 +128,7 @@ __device__ __forceinline__ Spot find(const KvP& p) {
 }
 
 template <typename T> __global__ __launch_bounds__(512) void kv_append_kernel(const KvP p) {
-    __shared__ float wmax[8];
+    __shared__ uint32_t wmax[8];
     const Spot s = find(p);
     if (!s.any) return;
     const int tid = threadIdx.x, page = 1 << p.pshift, hd = p.hd, nch = hd >> 4, nthr = page * hd >> 5;
@@ -139,40 +139,54 @@ template <typename T> __global__ __launch_bounds__(512) void kv_append_kernel(co
     uint8_t* dst = (s.half ? p.vp : p.kp) + base;
     const T* src = (const T*)(s.half ? p.v : p.k) + s.head * hd;
     const int64_t ld = s.half ? p.ldv : p.ldk;
-    float f[32], am = 0.f;
+    float f[32];
+    uint32_t top = 0;      // bits of the largest |x|: not below infinity's if there is one, or a NaN
     // K: units tid, tid + nthr of (token, 16 dims); V: one unit of (16 tokens, 2 dims)
     const int blk = tid / (hd >> 1), d0 = 2 * (tid % (hd >> 1));
+#pragma unroll
+    for (int e = 0; e < 32; ++e) f[e] = 0.f;
     if (active && s.half == 0) {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int u = tid + i * nthr, t = u / nch, c = u % nch;
-            if (t >= s.t_lo && t < s.t_hi) {
-                ld16(src + (s.row0 + t - s.t_off) * ld + c * 16, f + 16 * i);
-#pragma unroll
-                for (int e = 0; e < 16; ++e) am = fmaxf(am, finite_abs(f[16 * i + e]));
-            }
+            if (t >= s.t_lo && t < s.t_hi) ld16(src + (s.row0 + t - s.t_off) * ld + c * 16, f + 16 * i);
         }
     } else if (active) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
             const int t = blk * 16 + e;
-            f[e] = f[16 + e] = 0.f;
-            if (t >= s.t_lo && t < s.t_hi) {
-                ld2(src + (s.row0 + t - s.t_off) * ld + d0, f[e], f[16 + e]);
-                am = fmaxf(am, fmaxf(finite_abs(f[e]), finite_abs(f[16 + e])));
-            }
+            if (t >= s.t_lo && t < s.t_hi) ld2(src + (s.row0 + t - s.t_off) * ld + d0, f[e], f[16 + e]);
         }
     }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) top = max(top, __float_as_uint(f[e]) & 0x7fffffffu);
     const float was = *scale;      // read before the barrier, written behind it
-    am = wave_max(am);
-    if ((tid & 63) == 0) wmax[tid >> 6] = am;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+    if ((tid & 63) == 0) wmax[tid >> 6] = top;
     __syncthreads();
-    for (int w = 0; w < ((int)blockDim.x + 63) >> 6; ++w) am = fmaxf(am, wmax[w]);
-    int e = scale_exponent(am);
+    for (int w = 0; w < ((int)blockDim.x + 63) >> 6; ++w) top = max(top, wmax[w]);
+    const bool rare = top > __float_as_uint(448.f * 0x1p32f);      // something saturates, is infinite or NaN
+    if (rare) {
+        float am = 0.f;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) am = fmaxf(am, finite_abs(f[e]));
+        am = wave_max(am);
+        __syncthreads();
+        if ((tid & 63) == 0) wmax[tid >> 6] = __float_as_uint(am);
+        __syncthreads();
+        top = 0;
+        for (int w = 0; w < ((int)blockDim.x + 63) >> 6; ++w) top = max(top, wmax[w]);
+    }
+    int e = scale_exponent(__uint_as_float(top));
     const int e_old = min(max((int)((__float_as_uint(was) >> 23) & 255) - 127, E_MIN), E_MAX);
     if (!fresh) e = max(e, e_old);
     const bool grew = !fresh && e > e_old;
     const float inv = pow2(-e), back = pow2(e_old - e);
+    if (rare) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) f[k] = clamp_to(f[k], 448.f * pow2(e));
+    }
     if (tid == 0 && (fresh || grew)) *scale = pow2(e);
     if (!active) return;
     if (s.half == 0) {
