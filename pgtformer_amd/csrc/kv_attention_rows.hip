@@ -1,7 +1,7 @@
 // Attention over the paged 8-bit cache for many query rows (a prompt's chunk, whole frames): kv_attention.hip has the mathematics.
 //
 // 32x32x16 MFMA, swapped (S^T = K Q^T, O^T += V^T P^T); a wave holds 32 query columns, a workgroup of 8 waves 256.  What bounds it is the
-// vector work beside the products (per 32 x 32 scores: 512 cycles of products at hd 128, 256 at 64, and 73 vector instructions, 16 of them
+// vector work beside the products (per 32 x 32 scores: 512 cycles of products at hd 128, 256 at 64, and 62 vector instructions, 16 of them
 // exponentials), so everything else is kept away from the waves: per tile of 64 tokens the workgroup turns the codes into 16-bit
 // operands ONCE, into LDS, for all its columns.  The images are in operand order - K: 8 dims x 64 tokens, the tokens permuted so that a
 // lane's 16 scores belong to one 16-token block (one scale) and are the 16 tokens its V operand holds; V: 8 tokens x hd dims - all reads
@@ -193,18 +193,10 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             return *reinterpret_cast<const uint4*>(smem + st * STAGE + KB + ((sb * 2 + h) * 2 * HD + r) * 16 + ((i / ND) * HD + (i % ND) * 32) * 16);
         };
         float2 sc = make_float2(1.f, 0.f);      // of the current scores: sscale of this lane's 16 tokens
-        float tm = NEVER;                       // the largest of them, in units of the exponent
-        auto top = [&](const f32x16& x) {
-            float mx = x[0];
-#pragma unroll
-            for (int k = 1; k < 16; ++k) mx = fmaxf(mx, x[k]);
-            return max_of_halves(__builtin_fmaf(mx, fabsf(sc.x), sc.y));
-        };
         auto scores = [&](int st, int sb, f32x16& x) {
 #pragma unroll
             for (int k = 0; k < KS; ++k) x = mma_s(k_operand(st, sb, k), k, k == 0 ? zero16() : x);
             sc = sscale[st][sb * 2 + h];
-            tm = top(x);
         };
         // softmax of the scores x of half sb of tile t (stage st) and their product with V; xn = the scores of half nsb of stage nst (behind the
         // last tile: of whatever is there, unused); half fsb of stage fst is what the step after this one begins with.  Nothing moves over a SLICE;
@@ -230,17 +222,8 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 const int at = tok + 16 * h - lo;
 #pragma unroll
                 for (int k = 0; k < 16; ++k) x[k] = (uint32_t)(at + k) < span ? x[k] : -INFINITY;
-                tm = top(x);
             }
-            if (__any(tm > m + 15.f)) {
-                const float mn = tm > m + 15.f ? tm - 7.f : m;      // each query by itself: its result does not depend on its neighbours
-                const float al = exp2_(m - mn);
-                l *= al;
-#pragma unroll
-                for (int d = 0; d < ND; ++d) o[d] *= al;
-                m = mn;
-            }
-            const float em = ev - m;
+            float em = ev - m;
             float ls = 0.f;
             uint32_t pw[8], pl[F32 ? 8 : 1];      // weights in half; fp32: what is left of them, in half
             const halfx2 ones = {(_Float16)1.f, (_Float16)1.f};
@@ -266,22 +249,37 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 for (int i = 0; i < 8 / KS; ++i) weight2(k * (8 / KS) + i);
                 SLICE();
             }
+            // A query whose weights passed 2^15 in sum (each fits half until then) takes a new reference, 7 under its largest score, and its weights
+            // again - each query by itself: its result does not depend on its neighbours.  A maximum ahead of the weights would cost 12
+            // instructions more, and its way from the products to the exponentials stands between the steps.
+            if (__any(!(ls <= 32768.f))) {
+                float mx = x[0];
+#pragma unroll
+                for (int k = 1; k < 16; ++k) mx = fmaxf(mx, x[k]);
+                const float tm = max_of_halves(__builtin_fmaf(mx, ck, ev));
+                const bool over = max_of_halves(ls <= 32768.f ? 0.f : 1.f) > 0.f;
+                const float mn = over && tm > m + 10.f ? tm - 7.f : m;
+                const float al = exp2_(m - mn);
+                l *= al;
+#pragma unroll
+                for (int d = 0; d < ND; ++d) o[d] *= al;
+                m = mn;
+                em = ev - m;
+                ls = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) weight2(i);
+            }
             if (sb == 0) __syncthreads();      // the next tile's stage is written
             sc = scn;
-            float mx = 0.f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {      // O^T, the largest of the next scores
+            for (int i = 0; i < NV; ++i) {      // O^T
                 const int k = i / ND, d = i % ND;
                 if constexpr (F32) o[d] = mma16<half_t>(f[i % 4], make_uint4(pl[4 * k], pl[4 * k + 1], pl[4 * k + 2], pl[4 * k + 3]), o[d]);
                 o[d] = mma16<half_t>(f[i % 4], make_uint4(pw[4 * k], pw[4 * k + 1], pw[4 * k + 2], pw[4 * k + 3]), o[d]);
                 f[i % 4] = i + 4 < NV ? v_operand(st, sb, i + 4) : k_operand(fst, fsb, i + 4 - NV);
-                if (i == 0) mx = fmaxf(xn[0], xn[1]);
-#pragma unroll
-                for (int q = i == 0 ? 2 : 16 / NV * i; q < 16 / NV * (i + 1); ++q) mx = fmaxf(mx, xn[q]);
                 SLICE();
             }
             l = __builtin_fmaf(ls, back, l);
-            tm = max_of_halves(__builtin_fmaf(mx, fabsf(sc.x), sc.y));
         };
 #undef SLICE
 
