@@ -6,7 +6,6 @@ and the pixel/row stride may exceed C (channel slices of a wider buffer are vali
 dtype torch.float32 selects the exact-f32 kernels, torch.bfloat16 / torch.float16 the 16-bit MFMA kernels (bf16: 8
 significand bits; IEEE half: 11 - the decoder-side type of the default precision mode).
 """
-import contextlib
 import ctypes as C
 import math
 
@@ -1034,7 +1033,7 @@ def _need(ok, what, *args):
         raise hip.PgtError(what % args if args else what)
 
 
-def _rows(t, cols, what):
+def _rows(t, cols, what, name):
     """row stride of a (rows, cols) matrix whose rows do not overlap"""
     shape, stride = t.shape, t.stride()
     if len(shape) == 2 and shape[1] == cols and stride[1] == 1:
@@ -1042,8 +1041,8 @@ def _rows(t, cols, what):
             return cols
         if stride[0] >= cols:
             return stride[0]
-    raise hip.PgtError("%s: shape %s, strides %s; (rows, %d) wanted, elements of a row adjacent, rows not overlapping" % (
-        what, tuple(shape), stride, cols))
+    raise hip.PgtError("%s: %s has shape %s, strides %s; (rows, %d) wanted, elements of a row adjacent, rows not overlapping" % (
+        what, name, tuple(shape), stride, cols))
 
 
 def _pointers(*ts):
@@ -1078,22 +1077,19 @@ def _apart(outs, ins, what):
             _need(o.stride(0) == x.stride(0) and d >= x.shape[1] and d + o.shape[1] <= ld, "%s: an output overlaps another tensor", what)
 
 
-def _index(t, n, what):
-    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
-        raise hip.PgtError("%s: %s %s, contiguous int32 (%d,) wanted" % (what, t.dtype, tuple(t.shape), n))
+def _vec(t, dtype, n, what, name):
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
+        raise hip.PgtError("%s: %s is %s %s, contiguous %s (%d,) wanted" % (what, name, t.dtype, tuple(t.shape), dtype, n))
 
 
-def _f32_vec(t, n, what):
-    if t is not None and (t.dtype is not torch.float32 or t.shape != (n,) or not t.is_contiguous()):
-        raise hip.PgtError("%s: contiguous float32 (%d,) wanted" % (what, n))
-
-
-def _profiled(kernel, flops, *tensors, more=0.0):
-    """_Prof of a launch, its bytes counted only if somebody records"""
-    return _NOT_PROFILED if PROFILE is None else _Prof(kernel, flops, _nb(*tensors) + more)
-
-
-_NOT_PROFILED = contextlib.nullcontext()
+def _launch(name, args, flops, tensors, more=0):
+    """pgt_<name>(*args), recorded if somebody records (flops, bytes of tensors + more: only then looked at)"""
+    if PROFILE is None:
+        rc = getattr(hip.lib(), "pgt_" + name)(*args)
+    else:
+        with _Prof(name, float(flops), _nb(*tensors) + more):
+            rc = getattr(hip.lib(), "pgt_" + name)(*args)
+    hip.check(rc, "pgt_" + name)
 
 
 def rope_freqs(rot, base=10000.0, device="cuda"):
@@ -1111,20 +1107,26 @@ def _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, wha
     hd = cols // heads
     if k.shape[0] != rows or k.dtype is not q.dtype:
         raise hip.PgtError("%s: k %s %s, q %s %s" % (what, tuple(k.shape), k.dtype, tuple(q.shape), q.dtype))
-    ldq, ldk = _rows(q, cols, what + ": q"), _rows(k, kv_heads * hd, what + ": k")
-    rot = 0 if freqs is None else 2 * freqs.numel()
-    if rot:
-        _need(freqs.dtype is torch.float64 and freqs.is_contiguous(), "%s: freqs must be contiguous float64 (ops.rope_freqs)", what)
-        _need(positions is not None, "%s: a rotation needs positions", what)
-        _index(positions, rows, what + ": positions")
-    _f32_vec(q_gain, hd, what + ": q_gain")
-    _f32_vec(k_gain, hd, what + ": k_gain")
+    ldq, ldk = _rows(q, cols, what, "q"), _rows(k, kv_heads * hd, what, "k")
+    rot = 0
+    if freqs is not None:
+        rot = 2 * freqs.numel()
+        if freqs.dtype is not torch.float64 or not freqs.is_contiguous():
+            raise hip.PgtError("%s: freqs must be contiguous float64 (ops.rope_freqs)" % what)
+        if rot:
+            if positions is None:
+                raise hip.PgtError("%s: a rotation needs positions" % what)
+            _vec(positions, torch.int32, rows, what, "positions")
+    if q_gain is not None:
+        _vec(q_gain, torch.float32, hd, what, "q_gain")
+    if k_gain is not None:
+        _vec(k_gain, torch.float32, hd, what, "k_gain")
     if out is None:
-        qo, ko = q.new_empty((rows, cols)), q.new_empty((rows, kv_heads * hd))
+        qo, ko = torch.empty_like(q), torch.empty_like(k)      # (rows that do not overlap, elements adjacent: what comes back is dense)
         return rows, hd, rot, qo, ko, ldq, ldk, cols, kv_heads * hd
     qo, ko = out
     _need(qo.dtype is q.dtype and ko.dtype is q.dtype and qo.shape[0] == rows and ko.shape[0] == rows, "%s: outputs of another type or length", what)
-    return rows, hd, rot, qo, ko, ldq, ldk, _rows(qo, cols, what + ": out"), _rows(ko, kv_heads * hd, what + ": out")
+    return rows, hd, rot, qo, ko, ldq, ldk, _rows(qo, cols, what, "out"), _rows(ko, kv_heads * hd, what, "out")
 
 
 def qk_norm_rope(q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_heads, eps=1e-6, interleaved=False, out=None):
@@ -1135,9 +1137,8 @@ def qk_norm_rope(q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_
     if out is not None:
         _apart((qo, ko), (q, k), "qk_norm_rope")
     pq, pk, pp, pf, pqg, pkg, pqo, pko, st = _pointers(q, k, positions, freqs, q_gain, k_gain, qo, ko)
-    with _profiled("qk_norm_rope", 9.0 * rows * (heads + kv_heads) * hd, q, k, qo, ko):
-        hip.check(hip.lib().pgt_qk_norm_rope(_dt(q), pq, ldq, pk, ldk, rows, heads, kv_heads, hd, pp, pf, rot, int(interleaved), pqg, pkg, eps,
-                                             pqo, ldqo, pko, ldko, st), "pgt_qk_norm_rope")
+    _launch("qk_norm_rope", (_dt(q), pq, ldq, pk, ldk, rows, heads, kv_heads, hd, pp, pf, rot, 1 if interleaved else 0, pqg, pkg, eps, pqo, ldqo, pko,
+                             ldko, st), 9 * rows * (heads + kv_heads) * hd, (q, k, qo, ko))
     return qo, ko
 
 
@@ -1147,7 +1148,7 @@ def qk_norm_rope_backward(dq, dk, q, k, positions, freqs, q_gain=None, k_gain=No
     what = "qk_norm_rope_backward"
     rows, hd, rot, qo, ko, ldq, ldk, ldqo, ldko = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, what)
     _need(dq.dtype is q.dtype and dk.dtype is q.dtype and dq.shape[0] == rows and dk.shape[0] == rows, "%s: gradients of another type or length", what)
-    lddq, lddk = _rows(dq, heads * hd, what + ": dq"), _rows(dk, kv_heads * hd, what + ": dk")
+    lddq, lddk = _rows(dq, heads * hd, what, "dq"), _rows(dk, kv_heads * hd, what, "dk")
     if out is not None:
         _apart((qo, ko), (dq, dk, q, k), what)
     gains = q.new_empty((2, hd), dtype=torch.float32)
@@ -1156,10 +1157,9 @@ def qk_norm_rope_backward(dq, dk, q, k, positions, freqs, q_gain=None, k_gain=No
     ws = q.new_empty(nbytes // 4, dtype=torch.float32)
     gq, gk = gains.unbind(0)
     pdq, pdk, pq, pk, pp, pf, pqg, pkg, pqo, pko, pgq, pgk, pws, st = _pointers(dq, dk, q, k, positions, freqs, q_gain, k_gain, qo, ko, gq, gk, ws)
-    with _profiled("qk_norm_rope_backward", 17.0 * rows * (heads + kv_heads) * hd, dq, dk, q, k, qo, ko):
-        hip.check(L.pgt_qk_norm_rope_backward(_dt(q), pdq, lddq, pdk, lddk, pq, ldq, pk, ldk, rows, heads, kv_heads, hd, pp, pf, rot,
-                                              int(interleaved), pqg, pkg, eps, pqo, ldqo, pko, ldko, pgq, pgk, pws, nbytes, st),
-                  "pgt_qk_norm_rope_backward")
+    _launch("qk_norm_rope_backward", (_dt(q), pdq, lddq, pdk, lddk, pq, ldq, pk, ldk, rows, heads, kv_heads, hd, pp, pf, rot, 1 if interleaved else 0,
+                                      pqg, pkg, eps, pqo, ldqo, pko, ldko, pgq, pgk, pws, nbytes, st),
+            17 * rows * (heads + kv_heads) * hd, (dq, dk, q, k, qo, ko))
     return qo, ko, gq, gk
 
 
@@ -1198,13 +1198,13 @@ def _seq_args(table, lens, cu, rows, most, what):
     if len(shape) != 2 or table.dtype is not torch.int32 or (shape[1] > 1 and stride[1] != 1) or (shape[0] > 1 and stride[0] < shape[1]):
         raise hip.PgtError("%s: int32 table (B, width) wanted, got %s %s" % (what, table.dtype, tuple(shape)))
     B, width = shape
-    _index(lens, B, what + ": lens")
+    _vec(lens, torch.int32, B, what, "lens")
     if cu is None:
         if B <= 0 or rows % B or (most is not None and most != rows // B):
             raise hip.PgtError("%s: %d rows over %d sequences, %s each (ragged: pass cu)" % (what, rows, B, most))
         most = rows // B
     else:
-        _index(cu, B + 1, what + ": cu")
+        _vec(cu, torch.int32, B + 1, what, "cu")
         most = rows if most is None else int(most)
         if not 0 <= most <= rows:
             raise hip.PgtError("%s: at most %d tokens per sequence of %d rows" % (what, most, rows))
@@ -1220,11 +1220,10 @@ def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
     n = cache.kv_heads * cache.hd
     if k.dtype is not v.dtype or v.shape[0] != rows:
         raise hip.PgtError("kv_append: k %s %s, v %s %s" % (tuple(k.shape), k.dtype, tuple(v.shape), v.dtype))
-    ldk, ldv = _rows(k, n, "kv_append: k"), _rows(v, n, "kv_append: v")
+    ldk, ldv = _rows(k, n, "kv_append", "k"), _rows(v, n, "kv_append", "v")
     pk, pv, kp, vp, ks, vs, pt, pl, pc, st = _pointers(k, v, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, lens, cu)
-    with _profiled("kv_append", 8.0 * rows * n, k, v, more=2 * rows * n):
-        hip.check(hip.lib().pgt_kv_append(_dt(k), pk, ldk, pv, ldv, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, cache.hd, pt, ldt,
-                                          width, pl, pc, B, rows, most, st), "pgt_kv_append")
+    _launch("kv_append", (_dt(k), pk, ldk, pv, ldv, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, cache.hd, pt, ldt, width, pl, pc, B, rows,
+                          most, st), 8 * rows * n, (k, v), 2 * rows * n)
 
 
 def kv_read(cache, table, start, rows, dtype, cu=None, *, max_rows=None, out=None):
@@ -1238,12 +1237,11 @@ def kv_read(cache, table, start, rows, dtype, cu=None, *, max_rows=None, out=Non
     else:
         ko, vo = out
         _need(ko.dtype is dtype and vo.dtype is dtype and ko.shape[0] == rows and vo.shape[0] == rows, "kv_read: outputs of another type or length")
-        ldk, ldv = _rows(ko, n, "kv_read: out"), _rows(vo, n, "kv_read: out")
+        ldk, ldv = _rows(ko, n, "kv_read", "out"), _rows(vo, n, "kv_read", "out")
         _apart((ko, vo), (), "kv_read")
     pk, pv, kp, vp, ks, vs, pt, pl, pc, st = _pointers(ko, vo, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, start, cu)
-    with _profiled("kv_read", 2.0 * rows * n, ko, vo, more=2 * rows * n):
-        hip.check(hip.lib().pgt_kv_read(_dt(ko), pk, ldk, pv, ldv, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, cache.hd, pt, ldt,
-                                        width, pl, pc, B, rows, most, st), "pgt_kv_read")
+    _launch("kv_read", (_dt(ko), pk, ldk, pv, ldv, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, cache.hd, pt, ldt, width, pl, pc, B, rows,
+                        most, st), 2 * rows * n, (ko, vo), 2 * rows * n)
     return ko, vo
 
 
@@ -1254,22 +1252,21 @@ def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=
     sees nothing is zero; rows that no sequence owns stay as they are in `out`.  scale: default hd ** -0.5."""
     rows, hd = q.shape[0], cache.hd
     B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_attention")
-    ldq = _rows(q, heads * hd, "kv_attention: q")
+    ldq = _rows(q, heads * hd, "kv_attention", "q")
     if out is None:
-        out, ldo = q.new_empty((rows, heads * hd)), heads * hd
+        out, ldo = torch.empty_like(q), heads * hd
     else:
         _need(out.dtype == q.dtype and out.shape[0] == rows, "kv_attention: output of another type or length")
-        ldo = _rows(out, heads * hd, "kv_attention: out")
+        ldo = _rows(out, heads * hd, "kv_attention", "out")
         _apart((out,), (q,), "kv_attention")
     L = hip.lib()
     nbytes = L.pgt_kv_attention_workspace_bytes(_dt(q), B, most, heads, cache.kv_heads, hd, width, cache.page, causal, window)
     ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
     tokens = width * cache.page
     pq, kp, vp, ks, vs, pt, pl, pc, po, pw, st = _pointers(q, cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, table, lens, cu, out, ws)
-    with _profiled("kv_attention", 4.0 * rows * tokens * heads * hd, q, out, more=2 * B * tokens * cache.kv_heads * hd):
-        hip.check(L.pgt_kv_attention(_dt(q), pq, ldq, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, hd, pt, ldt, width, pl, pc, B,
-                                     rows, most, heads, hd ** -0.5 if scale is None else scale, causal, window, po, ldo, pw, nbytes, st),
-                  "pgt_kv_attention")
+    _launch("kv_attention", (_dt(q), pq, ldq, kp, vp, ks, vs, cache.pages, cache.page, cache.kv_heads, hd, pt, ldt, width, pl, pc, B, rows, most, heads,
+                             hd ** -0.5 if scale is None else scale, causal, window, po, ldo, pw, nbytes, st),
+            4 * rows * tokens * heads * hd, (q, out), 2 * B * tokens * cache.kv_heads * hd)
     return out
 
 
