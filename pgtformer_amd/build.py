@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libpgt_hip.so")
+EXT = os.path.join(LIBDIR, "_pgt_ops.so")      # native launchers of ops.py (csrc/py): host code against torch's headers, calls into LIB
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 ARCH = "gfx950"
 FLAGS = ["--offload-arch=" + ARCH, "-O3", "-std=c++17", "-fPIC", "-I", INCLUDE, "-I", CSRC,
@@ -112,7 +113,32 @@ def _build_locked(force, verbose):
         if verbose:
             print("[pgt build]", " ".join(cmd), flush=True)
         subprocess.check_call(cmd)
+    _build_ext(objdir, force, verbose)
     return LIB
+
+
+def _build_ext(objdir, force, verbose):
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    src, header = os.path.join(CSRC, "py", "ops_ext.cpp"), os.path.join(INCLUDE, "pgt_hip.h")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI,
+           "-I", INCLUDE, "-I", sysconfig.get_paths()["include"]]
+    cmd += [a for d in cpp_extension.include_paths() for a in ("-isystem", d)] + [src, "-o", EXT]
+    cmd += ["-L" + d for d in cpp_extension.library_paths()] + ["-lc10", "-ltorch_cpu", "-ltorch_python"]
+    key = hashlib.sha256(open(src, "rb").read() + open(header, "rb").read() + (torch.__version__ + " ".join(cmd)).encode()).hexdigest()
+    stamp = os.path.join(objdir, "_pgt_ops.sha")
+    try:
+        have = open(stamp).read().strip()
+    except OSError:
+        have = ""
+    if force or not os.path.exists(EXT) or have != key:
+        if verbose:
+            print("[pgt build]", " ".join(cmd), flush=True)
+        subprocess.check_call(cmd)
+        with open(stamp, "w") as f:
+            f.write(key)
 
 
 if __name__ == "__main__":

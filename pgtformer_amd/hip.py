@@ -177,6 +177,29 @@ def lib():
     return _LIB
 
 
+_EXT = None
+_EXT_ENTRIES = ("pgt_qk_norm_rope", "pgt_qk_norm_rope_backward", "pgt_qk_norm_rope_backward_workspace_bytes", "pgt_kv_append", "pgt_kv_read",
+                "pgt_kv_attention", "pgt_kv_attention_workspace_bytes")      # in the order of csrc/py/ops_ext.cpp
+
+
+def ops_ext():
+    """Load (once) and return the native launchers of ops.py (csrc/py/ops_ext.cpp), bound to the library that lib() loaded."""
+    global _EXT
+    if _EXT is None:
+        import importlib.machinery
+        import importlib.util
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "_pgt_ops.so")
+        if not os.path.exists(path):
+            raise PgtError(f"{path} is missing: build it with `python -m pgtformer_amd.build`")
+        real = lib() if TRACE is None else lib()._real
+        loader = importlib.machinery.ExtensionFileLoader("_pgt_ops", path)
+        ext = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_pgt_ops", path, loader=loader))
+        loader.exec_module(ext)
+        ext.bind(*(C.cast(getattr(real, n), C.c_void_p).value for n in _EXT_ENTRIES))
+        _EXT = ext
+    return _EXT
+
+
 def check(rc, what):
     if rc != 0:
         msg = lib().pgt_last_error()

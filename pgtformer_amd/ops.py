@@ -1092,6 +1092,23 @@ def _launch(name, args, flops, tensors, more=0):
     hip.check(rc, "pgt_" + name)
 
 
+def _native(t):
+    """(native launchers, current device, its stream) for a call on the GPU that nobody records; else None.  What they decline - they return None -
+    goes the way below their call."""
+    if not t.is_cuda or PROFILE is not None or hip.TRACE is not None or hip.TRACE_TENSORS is not None:
+        return None
+    dev = torch._C._cuda_getDevice()
+    return hip.ops_ext(), dev, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _done(r, what):
+    """a result of the native launchers, or its status as an error"""
+    if type(r) is int:
+        hip.check(r, what)
+        return True
+    return r
+
+
 def rope_freqs(rot, base=10000.0, device="cuda"):
     """Rotation frequencies of qk_norm_rope in revolutions per position, fp64 (rot / 2,): base ** (-2 i / rot) / (2 pi)."""
     _need(rot >= 0 and rot % 8 == 0, "rope_freqs: %d rotated elements (a multiple of 8)", rot)
@@ -1133,6 +1150,10 @@ def qk_norm_rope(q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_
     """Per-head RMS norm (gains fp32 (hd,) or None) of q (rows, heads * hd) and k (rows, kv_heads * hd) and the rotation by their positions
     (int32 (rows,); freqs: rope_freqs(rot), None = no rotation) in one pass -> (q_out, k_out).  out: the two outputs, which may be q and
     k themselves.  interleaved: pairs (2i, 2i + 1) instead of (i, i + rot / 2)."""
+    if out is None and (nat := _native(q)) is not None:
+        r = nat[0].qk_norm_rope(nat[1], nat[2], q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, eps, True if interleaved else False)
+        if r is not None:
+            return _done(r, "pgt_qk_norm_rope")
     rows, hd, rot, qo, ko, ldq, ldk, ldqo, ldko = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, "qk_norm_rope")
     if out is not None:
         _apart((qo, ko), (q, k), "qk_norm_rope")
@@ -1146,6 +1167,10 @@ def qk_norm_rope_backward(dq, dk, q, k, positions, freqs, q_gain=None, k_gain=No
     """Gradients of qk_norm_rope: (dq, dk) of its outputs, its inputs q, k -> (gradient of q, of k, of q_gain, of k_gain; the gains' fp32
     (hd,)).  out: where the first two go (dq, dk themselves are allowed)."""
     what = "qk_norm_rope_backward"
+    if out is None and (nat := _native(q)) is not None:
+        r = nat[0].qk_norm_rope_backward(nat[1], nat[2], q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, eps, True if interleaved else False, dq, dk)
+        if r is not None:
+            return _done(r, "pgt_qk_norm_rope_backward")
     rows, hd, rot, qo, ko, ldq, ldk, ldqo, ldko = _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, what)
     _need(dq.dtype is q.dtype and dk.dtype is q.dtype and dq.shape[0] == rows and dk.shape[0] == rows, "%s: gradients of another type or length", what)
     lddq, lddk = _rows(dq, heads * hd, what, "dq"), _rows(dk, kv_heads * hd, what, "dk")
@@ -1215,6 +1240,11 @@ def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
     """Quantise the rows k, v (rows, kv_heads * hd) into the cache: sequence b's (rows cu[b] .. cu[b + 1] - 1; cu None: rows / B each) become
     its tokens lens[b] .. .  lens: int32 (B,), tokens BEFORE the call (the caller counts on).  max_new: most rows of one sequence - the
     launch covers so many (default with cu: all rows, correct but a larger launch)."""
+    if (nat := _native(k)) is not None:
+        r = nat[0].kv_append(nat[1], nat[2], cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, cache.pages, cache.page, cache.kv_heads, cache.hd,
+                             table, lens, cu, k, v, max_new)
+        if r is not None:
+            return hip.check(r, "pgt_kv_append")
     rows = k.shape[0]
     B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_append")
     n = cache.kv_heads * cache.hd
@@ -1229,6 +1259,11 @@ def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
 def kv_read(cache, table, start, rows, dtype, cu=None, *, max_rows=None, out=None):
     """The cache's values as (k, v), each (rows, kv_heads * hd) of dtype: the rows of sequence b (cu as in kv_append) are its tokens start[b] .. .
     Rows that no sequence owns stay as they are in `out`; tokens that no page holds are zeros."""
+    if out is None and (nat := _native(cache.k_pages)) is not None:
+        r = nat[0].kv_read(nat[1], nat[2], cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, cache.pages, cache.page, cache.kv_heads, cache.hd,
+                           table, start, cu, rows, max_rows, dtype)
+        if r is not None:
+            return _done(r, "pgt_kv_read")
     n = cache.kv_heads * cache.hd
     B, width, ldt, most = _seq_args(table, start, cu, rows, max_rows, "kv_read")
     if out is None:
@@ -1250,6 +1285,11 @@ def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=
     (int32) the tokens the cache holds INCLUDING these rows'.  causal: 0 = every token, c = those up to the end of the block of c tokens that
     the position lies in (1 = token by token, tokens per frame = whole frames); window > 0: only the last `window` of these.  A row that
     sees nothing is zero; rows that no sequence owns stay as they are in `out`.  scale: default hd ** -0.5."""
+    if out is None and (nat := _native(q)) is not None:
+        r = nat[0].kv_attention(nat[1], nat[2], cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, cache.pages, cache.page, cache.kv_heads, cache.hd,
+                                table, lens, cu, q, heads, max_new, causal, window, scale)
+        if r is not None:
+            return _done(r, "pgt_kv_attention")
     rows, hd = q.shape[0], cache.hd
     B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_attention")
     ldq = _rows(q, heads * hd, "kv_attention", "q")

@@ -597,6 +597,64 @@ def test_on_another_stream_and_two_at_once():
     assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
 
 
+def every_operator(typ, ragged):
+    """one call of each operator on inputs made anew: all outputs, the cache included"""
+    B, heads, kv, hd, page, width = 3, 8, 2, 64, 16, 6
+    g = torch.Generator().manual_seed(91)
+    new = [5, 0, 7] if ragged else [4, 4, 4]
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    rows = cu[-1]
+    cache = ops.KvCache.alloc(B * width, kv, page, hd, DEV)
+    table = scatter_table(B, width, B * width, 92).to(DEV)
+    wide = torch.randn((rows, (heads + 2 * kv) * hd + 8), generator=g).to(DT[typ]).to(DEV)
+    q, k, v = wide[:, :heads * hd], wide[:, heads * hd:(heads + kv) * hd], wide[:, (heads + kv) * hd:(heads + 2 * kv) * hd]
+    pos = torch.arange(rows, dtype=torch.int32, device=DEV)
+    gain = (1 + 0.1 * torch.randn(hd, generator=g)).to(DEV)
+    before = torch.tensor([0, 20, 9], dtype=torch.int32, device=DEV)
+    cud = torch.tensor(cu, dtype=torch.int32, device=DEV) if ragged else None
+    most = dict(max_new=max(new)) if ragged else {}
+    freqs = ops.rope_freqs(32, device=DEV)
+    outs = list(ops.qk_norm_rope(q, k, pos, freqs, gain, None, heads=heads, kv_heads=kv, interleaved=ragged))
+    outs += ops.qk_norm_rope(q, k, None, None, heads=heads, kv_heads=kv, eps=1e-3)
+    outs += ops.qk_norm_rope_backward(outs[0], outs[1], q, k, pos, freqs, gain, gain, heads=heads, kv_heads=kv)
+    ops.kv_append(cache, k, v, table, before, cud, **most)
+    outs += [cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale]
+    outs += ops.kv_read(cache, table, before, rows, torch.float16, cud)
+    lens = before + torch.tensor(new, dtype=torch.int32, device=DEV)
+    outs.append(ops.kv_attention(q, cache, table, lens, cud, heads=heads, window=9, **most))
+    outs.append(ops.kv_attention(q, cache, table, lens, cud, heads=heads, causal=0, scale=0.3))
+    return outs
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_native_launchers_and_the_python_ones_do_the_same(typ, ragged, monkeypatch):
+    taken = []
+
+    class Counted:
+        def __init__(self, ext):
+            self.ext = ext
+
+        def __getattr__(self, name):
+            def call(*a):
+                r = getattr(self.ext, name)(*a)
+                taken.append((name, r is not None))
+                return r
+            return call
+    real = ops._native
+    monkeypatch.setattr(ops, "_native", lambda t: (lambda n: n and (Counted(n[0]), *n[1:]))(real(t)))
+    a = every_operator(typ, ragged)
+    assert [n for n, ok in taken if ok] == ["qk_norm_rope", "qk_norm_rope", "qk_norm_rope_backward", "kv_append", "kv_read", "kv_attention", "kv_attention"], taken
+    monkeypatch.setattr(ops, "_native", lambda t: None)
+    b = every_operator(typ, ragged)
+    assert len(a) == len(b)
+    for i, (x, y) in enumerate(zip(a, b)):
+        assert x.dtype is y.dtype and x.shape == y.shape and x.is_contiguous() and not x.requires_grad, i
+        assert torch.equal(x, y), i
+
+
 def test_refusals_on_the_device():
     cache = ops.KvCache.alloc(4, 2, 16, 64, DEV)
     q, lens, table = torch.zeros((2, 8 * 64), device=DEV), torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros((2, 2), dtype=torch.int32, device=DEV)

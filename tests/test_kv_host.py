@@ -142,6 +142,25 @@ def test_c_entry_points_refuse():
             assert entry(name, base, **kw)[0] == 0, (name, kw)
 
 
+def test_native_launchers_decline_what_is_not_plainly_right():
+    """nothing is launched, nothing raised: ops.py then says what is wrong"""
+    e = hip.ops_ext()
+    q, k, lens, table = torch.zeros(4, 512), torch.zeros(4, 128), i32(2), i32(2, 3)
+    c = cache()
+    cc = (c.k_pages, c.v_pages, c.k_scale, c.v_scale, c.pages, c.page, c.kv_heads, c.hd)
+    for dev in (0, -1, 1 << 40, "cuda"):
+        assert e.qk_norm_rope(dev, 0, q, k, None, None, None, None, 8, 2, 1e-6, False) is None      # tensors of the host
+        assert e.qk_norm_rope_backward(dev, 0, q, k, None, None, None, None, 8, 2, 1e-6, False, q, k) is None
+        assert e.kv_append(dev, 0, *cc, table, lens, None, k, k, None) is None
+        assert e.kv_read(dev, 0, *cc, table, lens, None, 4, None, torch.float16) is None
+        assert e.kv_attention(dev, 0, *cc, table, lens, None, q, 8, None, 1, 0, None) is None
+    assert e.qk_norm_rope(0, 0, None, 3, "x", [], {}, (), 8.5, 1 << 70, "e", 1) is None
+    assert e.kv_read(0, 0, *cc, table, lens, None, -4, None, torch.float16) is None
+    for bad in (lambda: e.kv_append(0, 0), lambda: e.qk_norm_rope(), lambda: e.bind(1, 2)):
+        with pytest.raises(TypeError):
+            bad()
+
+
 def test_workspace_sizes():
     L = hip.lib()
     assert L.pgt_qk_norm_rope_backward_workspace_bytes(0, 64) == 0
