@@ -5,17 +5,17 @@
 //   (i, i + rot / 2), or (2i, 2i + 1) in the interleaved form; the elements behind `rot` are not turned.
 // gradient: z = R(-pos) dy, u = g * z, xh = x * r:   dx = r (u - xh * mean(xh * u)),   dg = sum over rows and heads of z * xh
 //
-// Memory bound: x is read once and y written once.  hd / 8 lanes hold a head row, 8 elements each, picked so that both halves of
-// every pair sit in one lane (a rotation needs no exchange; the mean is one shuffle reduction).  The angle is taken in fp64 and
+// Memory bound: x is read once and y written once.  hd / 8 (or hd / 16) lanes hold a head row, two runs of 4 (8) elements each, picked so that
+// both halves of every pair sit in one lane (a rotation needs no exchange; the mean is a few lane exchanges).  The angle is taken in fp64 and
 // reduced to a fraction of a turn before it is rounded to fp32 - exact for any int32 position - once per token and pair, into
-// LDS, for all heads of the token.  16411 tokens of 32 + 8 heads of 128 in bf16: 74 us, 4.5 TB/s (a copy: 5.1); the gradient of 8190: 49 us, 5.1
+// LDS, for all heads of the token.  16411 tokens of 32 + 8 heads of 128 in bf16: 65 us, 5.2 TB/s (a copy: 5.1); the gradient of 8190: 49 us, 5.1
 // TB/s, and 4.6 for the sums of the gain gradients.  Issue counts: a division per row, selects between q and k and an exact root cost 10 us.
 #include "kv_common.h"
 #include "pgt_internal.h"
 
 namespace {
 
-// 8 elements of one head row: two runs of 4 (16-bit: 8 bytes each, fp32: 16 bytes each).  ONCE: streaming loads, for the form that only reads
+// A run of 4 elements of a head row (16-bit: 8 bytes, fp32: 16 bytes).  ONCE: streaming loads, for the form that only reads
 // and writes once (16411 tokens of 40 heads of 128: 74 instead of 77 us; the gradient, with twice the loads in flight, gains nothing).
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 template <bool ONCE, typename T> __device__ __forceinline__ void ld4(const T* p, float* f) {
@@ -37,6 +37,22 @@ template <bool ONCE, typename T> __device__ __forceinline__ void ld4(const T* p,
     }
 }
 
+// R elements: 4, or 8 of a 16-bit type (16 bytes)
+template <int R, bool ONCE, typename T> __device__ __forceinline__ void ldr(const T* p, float* f) {
+    if constexpr (R == 4) {
+        ld4<ONCE>(p, f);
+    } else {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const u32x4* at = reinterpret_cast<const u32x4*>(p);
+        const u32x4 v = ONCE ? __builtin_nontemporal_load(at) : *at;
+        Vec16<T>::unpack(make_uint4(v.x, v.y, v.z, v.w), f);
+    }
+}
+template <int R, typename T> __device__ __forceinline__ void str(T* p, const float* f) {
+    if constexpr (R == 4) store4(p, f);
+    else *reinterpret_cast<uint4*>(p) = make_uint4(pair_of<T>(f[0], f[1]), pair_of<T>(f[2], f[3]), pair_of<T>(f[4], f[5]), pair_of<T>(f[6], f[7]));
+}
+
 struct RopeP {
     const void *q, *k, *dq, *dk;      // dq, dk: gradient form only
     void *qo, *ko;
@@ -45,7 +61,7 @@ struct RopeP {
     const float *qg, *kg;
     float* part;                      // gradient form: (workgroups, 2, hd) partial sums of dg
     int ldq, ldk, lddq, lddk, ldqo, ldko;
-    int rows, heads, kv_heads, rot, inter, tok;
+    int rows, heads, kv_heads, rot, inter, tok, run;
     float eps;
 };
 
@@ -56,9 +72,9 @@ template <int CTRL> __device__ __forceinline__ float add_dpp(float v) {
     return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
 template <int N> __device__ __forceinline__ float group_sum(float v) {
-    static_assert(N == 4 || N == 8 || N == 16 || N == 32, "lanes of a head row");
+    static_assert(N == 2 || N == 4 || N == 8 || N == 16 || N == 32, "lanes of a head row");
     v = add_dpp<0xb1>(v);                            // lane ^ 1
-    v = add_dpp<0x4e>(v);                            // lane ^ 2
+    if constexpr (N >= 4) v = add_dpp<0x4e>(v);      // lane ^ 2
     if constexpr (N >= 8) v = add_dpp<0x141>(v);     // the other half of 8
     if constexpr (N >= 16) v = add_dpp<0x140>(v);    // the other half of 16
     if constexpr (N >= 32) v += __shfl_xor(v, 16, 64);
@@ -72,20 +88,20 @@ __device__ __forceinline__ float rsqrt_(float v) {
     return small ? r * 0x1p30f : r;
 }
 
-template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void qk_rope_kernel(const RopeP p) {
-    constexpr int LPH = HD / 8, NG = 256 / LPH;      // lanes per head row, head rows in flight per workgroup
+template <typename T, int HD, bool BWD, int R> __global__ __launch_bounds__(256) void qk_rope_kernel(const RopeP p) {
+    constexpr int LPH = HD / (2 * R), NG = 256 / LPH;      // lanes per head row, head rows in flight per workgroup
     __shared__ float2 turn[MAXTOK][HD / 2];
     const int tid = threadIdx.x, j = tid % LPH, grp = tid / LPH;
     const int nh = p.heads + p.kv_heads, half = p.rot >> 1;
-    const bool turned = 8 * j < p.rot;
+    const bool turned = 2 * R * j < p.rot;
     // the two runs of 4 elements this lane holds, and its first pair (pairs pr .. pr + 3)
-    const int lo = turned && !p.inter ? 4 * j : 8 * j;
-    const int hi = turned && !p.inter ? half + 4 * j : 8 * j + 4;
-    const int pr = 4 * j;
-    float gq[8], gk[8], sq[8], sk[8];
+    const int lo = turned && !p.inter ? R * j : 2 * R * j;
+    const int hi = turned && !p.inter ? half + R * j : 2 * R * j + R;
+    const int pr = R * j;
+    float gq[2 * R], gk[2 * R], sq[2 * R], sk[2 * R];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int d = (e < 4 ? lo : hi - 4) + e;
+    for (int e = 0; e < 2 * R; ++e) {
+        const int d = (e < R ? lo : hi - R) + e;
         gq[e] = p.qg ? p.qg[d] : 1.f;
         gk[e] = p.kg ? p.kg[d] : 1.f;
         sq[e] = sk[e] = 0.f;
@@ -109,26 +125,26 @@ template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void q
             for (; t < nt;) {
                 const size_t row = t0 + t;
                 const T* x = (const T*)xp + row * ldx + h * HD;
-                float f[8], z[8];
-                ld4<!BWD>(x + lo, f);
-                ld4<!BWD>(x + hi, f + 4);
+                float f[2 * R], z[2 * R];
+                ldr<R, !BWD>(x + lo, f);
+                ldr<R, !BWD>(x + hi, f + R);
                 if constexpr (BWD) {
                     const T* dy = (const T*)dyp + row * lddy + h * HD;
-                    ld4<!BWD>(dy + lo, z);
-                    ld4<!BWD>(dy + hi, z + 4);
+                    ldr<R, !BWD>(dy + lo, z);
+                    ldr<R, !BWD>(dy + hi, z + R);
                 }
                 float ss = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) ss += f[e] * f[e];
+                for (int e = 0; e < 2 * R; ++e) ss += f[e] * f[e];
                 const float r = rsqrt_(group_sum<LPH>(ss) * (1.f / HD) + p.eps);
                 float* v = BWD ? z : f;
                 if constexpr (!BWD) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) f[e] = f[e] * r * gain[e];
+                    for (int e = 0; e < 2 * R; ++e) f[e] = f[e] * r * gain[e];
                 }
                 if (turned) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
+                    for (int e = 0; e < R; ++e) {
                         const float2 cs = turn[t][pr + e];
                         const float s = BWD ? -cs.y : cs.y;
                         if (p.inter) {
@@ -136,16 +152,16 @@ template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void q
                             v[2 * e] = a * cs.x - b * s;
                             v[2 * e + 1] = b * cs.x + a * s;
                         } else {
-                            const float a = v[e], b = v[4 + e];
+                            const float a = v[e], b = v[R + e];
                             v[e] = a * cs.x - b * s;
-                            v[4 + e] = b * cs.x + a * s;
+                            v[R + e] = b * cs.x + a * s;
                         }
                     }
                 }
                 if constexpr (BWD) {
                     float dot = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
+                    for (int e = 0; e < 2 * R; ++e) {
                         f[e] *= r;
                         sum[e] += z[e] * f[e];
                         z[e] *= gain[e];
@@ -153,11 +169,11 @@ template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void q
                     }
                     dot = group_sum<LPH>(dot) * (1.f / HD);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z[e] = r * (z[e] - f[e] * dot);
+                    for (int e = 0; e < 2 * R; ++e) z[e] = r * (z[e] - f[e] * dot);
                 }
                 T* y = (T*)yp + row * ldy + h * HD;
-                store4(y + lo, v);
-                store4(y + hi, v + 4);
+                str<R>(y + lo, v);
+                str<R>(y + hi, v + R);
                 t += dt;
                 h += dh;
                 if (h >= heads) h -= heads, ++t;
@@ -171,8 +187,8 @@ template <typename T, int HD, bool BWD> __global__ __launch_bounds__(256) void q
     if constexpr (BWD) {      // the workgroup's share of dg: head rows in flight added in order
         __shared__ float red[2][NG][HD];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int d = (e < 4 ? lo : hi - 4) + e;
+        for (int e = 0; e < 2 * R; ++e) {
+            const int d = (e < R ? lo : hi - R) + e;
             red[0][grp][d] = sq[e];
             red[1][grp][d] = sk[e];
         }
@@ -242,7 +258,16 @@ int check(int dtype, const RopeP& p, int hd, bool bwd) {
 }
 
 template <bool BWD> void launch(int dtype, int hd, const RopeP& p, dim3 grid, hipStream_t st) {
-#define ROPE_GO(TT, HD) hipLaunchKernelGGL((qk_rope_kernel<TT, HD, BWD>), grid, dim3(256), 0, st, p)
+#define ROPE_GO(TT, HD)                                                                                                   \
+    do {                                                                                                                  \
+        if constexpr (!BWD && !__is_same(TT, float)) {                                                                    \
+            if (p.run == 8) {                                                                                             \
+                hipLaunchKernelGGL((qk_rope_kernel<TT, HD, false, 8>), grid, dim3(256), 0, st, p);                        \
+                break;                                                                                                    \
+            }                                                                                                             \
+        }                                                                                                                 \
+        hipLaunchKernelGGL((qk_rope_kernel<TT, HD, BWD, 4>), grid, dim3(256), 0, st, p);                                  \
+    } while (0)
 #define ROPE_HD(TT)                                                                                                       \
     do {                                                                                                                  \
         if (hd == 32) ROPE_GO(TT, 32);                                                                                    \
@@ -270,7 +295,10 @@ extern "C" int pgt_qk_norm_rope(int32_t dtype, const void* q, int32_t ldq, const
     if (const int rc = check(dtype, p, hd, false)) return rc;
     if (rows == 0) return 0;
     p.tok = rope_tok(rows);
-    const int ng = 256 / (hd / 8), nh = heads + kv_heads;
+    // runs of 16 bytes of a 16-bit type where the pairs allow it: 16411 tokens 65 instead of 74 us; with a token per workgroup the longer way of a
+    // lane costs more (4 tokens: 4.7 instead of 3.9)
+    p.run = dtype != PGT_F32 && rot % 16 == 0 && p.tok > 1 ? 8 : 4;
+    const int ng = 256 / (hd / (2 * p.run)), nh = heads + kv_heads;
     const dim3 grid((rows + p.tok - 1) / p.tok, p.tok == 1 ? (nh + ng - 1) / ng : 1);
     PGT_CHECK(grid.y <= 65535, "qk_norm_rope: %d heads", nh);
     launch<false>(dtype, hd, p, grid, (hipStream_t)stream);
