@@ -108,9 +108,11 @@ struct Rope {
         if (a[3] != Py_None) {
             const at::Tensor& f = c.tensor(a[3]);
             rot = int32(2 * f.numel());
-            if (f.scalar_type() != at::kDouble || !f.is_contiguous() || rot == 0) throw No();
-            freqs = (const double*)f.data_ptr();
-            pos = c.vec<int32_t>(a[2], at::kInt, rows);
+            if (f.scalar_type() != at::kDouble || !f.is_contiguous()) throw No();
+            if (rot) {
+                freqs = (const double*)f.data_ptr();
+                pos = c.vec<int32_t>(a[2], at::kInt, rows);
+            }
         }
         qg = c.vec<float>(a[4], at::kFloat, hd, true);
         kg = c.vec<float>(a[5], at::kFloat, hd, true);

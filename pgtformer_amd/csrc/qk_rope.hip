@@ -228,8 +228,9 @@ __global__ __launch_bounds__(1024) void qk_rope_gain_kernel(const float* __restr
     }
 }
 
-// tokens per workgroup: 1 until the grid fills the chip, then 4 share one pass over the angles
-int rope_tok(int rows) { return rows >= 4096 ? MAXTOK : 1; }
+// Tokens per workgroup that share one pass over the angles.  1 / 2 / 4 of them, us: 128 tokens 3.7 / 5.0 / 6.4 (40 heads of 128, bf16), 3.1 / 3.1 / 3.9
+// (16 of 64, fp32); 1024: 9.6 / 6.9 / 8.1, 4.5 / 3.9 / 4.5; 4096: 32.7 / 18.5 / 16.6, 11.8 / 9.1 / 8.1; the gradient's are closer together.
+int rope_tok(int rows) { return rows >= 2500 ? MAXTOK : rows >= 512 ? 2 : 1; }
 int rope_bwd_groups(int rows) {
     const int n = (rows + rope_tok(rows) - 1) / rope_tok(rows);
     return n < 1024 ? n : 1024;

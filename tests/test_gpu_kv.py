@@ -27,6 +27,7 @@ ROPE = [  # rows, heads, kv, hd, rot, interleaved, type
     (129, 32, 8, 128, 128, False, "bf16"), (7, 3, 3, 256, 256, False, "f32"), (65, 2, 2, 256, 24, False, "f16"), (4097, 4, 2, 64, 64, False, "f16"),
     (4099, 3, 1, 32, 32, True, "f32"), (5, 8, 8, 64, 0, False, "bf16"), (2, 6, 2, 128, 40, True, "f32"), (4096, 3, 1, 32, 16, True, "bf16"),
     (4100, 2, 1, 256, 48, False, "f16"), (4101, 4, 2, 128, 0, False, "bf16"), (4097, 2, 2, 128, 24, False, "bf16"), (4098, 5, 1, 128, 128, True, "f16"),
+    (601, 8, 2, 64, 64, False, "bf16"), (2499, 3, 1, 64, 32, True, "f32"), (777, 3, 1, 32, 8, True, "f16"), (2501, 2, 2, 128, 64, True, "bf16"), (512, 1, 1, 256, 256, False, "f32"),
 ]
 
 
