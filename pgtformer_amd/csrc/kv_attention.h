@@ -108,6 +108,7 @@ constexpr int MIN_SHARE = 4;         // tiles of a piece
 //   order 0: (sequence, kv head, column tile), neighbours read the same pages       order 1: (sequence, column tile, kv head), one look-up for all heads
 struct Segment {
     int b, hk, ct, first, tiles;      // first tile, tiles
+    Seq s;
 };
 __device__ __forceinline__ Segment segment_of(const AttnP& p, int order, int e) {
     Segment g;
@@ -122,7 +123,7 @@ __device__ __forceinline__ Segment segment_of(const AttnP& p, int order, int e) 
         g.hk = e % p.kv;
         g.b = e / p.kv;
     }
-    const Seq s = seq_of(p, g.b);
+    const Seq s = g.s = seq_of(p, g.b);
     const int cols = s.n * p.group, c0 = g.ct << p.cshift, cz = min(c0 + (1 << p.cshift), cols) - 1;
     g.first = g.tiles = 0;
     if (c0 < cols) {
@@ -134,7 +135,7 @@ __device__ __forceinline__ Segment segment_of(const AttnP& p, int order, int e) 
     }
     return g;
 }
-__device__ __forceinline__ Segment uni(const Segment& g) { return {uni(g.b), uni(g.hk), uni(g.ct), uni(g.first), uni(g.tiles)}; }
+__device__ __forceinline__ Segment uni(const Segment& g) { return {uni(g.b), uni(g.hk), uni(g.ct), uni(g.first), uni(g.tiles), uni(g.s)}; }
 struct Line {
     int total, share;
 };

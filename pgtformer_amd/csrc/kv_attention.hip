@@ -45,7 +45,7 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     if (p.wgs && !part_of<NW, 1>(p, blockIdx.x, pos, pos_end, e, before, red)) return;
     for (;;) {      // the column tiles that this workgroup's part of the line touches
     const Segment sg = uni(segment_of(p, 1, e));
-    const Seq s = uni(seq_of(p, sg.b));
+    const Seq& s = sg.s;
     const int cols = s.n * p.group, ct = sg.ct;
     if (p.wgs && sg.tiles == 0) { e += p.kv; continue; }
     if (ct * 16 >= cols) return;
@@ -339,7 +339,7 @@ template <typename T, int HD, int ROWS> __global__ __launch_bounds__(256) void k
     const int chunks = (1 << p.cshift) / WG_ROWS;
     const int e = blockIdx.x / chunks, r0 = blockIdx.x % chunks * WG_ROWS;
     const Segment sg = segment_of(p, 0, e);
-    const Seq s = seq_of(p, sg.b);
+    const Seq& s = sg.s;
     const int c0 = (sg.ct << p.cshift) + r0, cols = s.n * p.group;
     if (c0 >= cols) return;
     const int2 ends = sg.tiles > 0 ? p.ends[e] : make_int2(0, -1);
@@ -378,7 +378,7 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void kv_attn_joi
     constexpr int LP = HD / 4, NS = 256 / LP;
     const int tid = threadIdx.x, e = blockIdx.x / p.jrows, r0 = blockIdx.x % p.jrows;
     const Segment sg = segment_of(p, 1, e);
-    const Seq s = seq_of(p, sg.b);
+    const Seq& s = sg.s;
     const int qc = (sg.ct << 4) + r0;
     if (qc >= s.n * p.group) return;
     const int2 ends = sg.tiles > 0 ? p.ends[e] : make_int2(0, -1);

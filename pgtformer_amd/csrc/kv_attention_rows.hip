@@ -59,7 +59,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         const Segment sg = uni(segment_of(p, 0, e));
         if (p.wgs && sg.tiles == 0) { ++e; continue; }
         const int b = sg.b, hk = sg.hk, ct = sg.ct;
-        const Seq s = uni(seq_of(p, b));
+        const Seq& s = sg.s;
         const int cols = s.n * p.group, shift = s.len - s.n;
         if (ct * CT >= cols) return;
         const int t0 = sg.first + (p.wgs ? pos - before : 0), te = p.wgs ? sg.first + min(pos_end - before, sg.tiles) : sg.first + sg.tiles;
