@@ -227,7 +227,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             float ls = 0.f;
             uint32_t pw[8], pl[F32 ? 8 : 1];      // weights in half; fp32: what is left of them, in half
             const halfx2 ones = {(_Float16)1.f, (_Float16)1.f};
-            auto weight2 = [&](int i) {      // weights 2 i, 2 i + 1; their sum is that of the rounded ones, as the product's
+            auto weight2 = [&](int i) {      // weights 2 i, 2 i + 1; their sum is that of the rounded ones
                 const float a = exp2_(__builtin_fmaf(x[2 * i], ck, em)), b = exp2_(__builtin_fmaf(x[2 * i + 1], ck, em));
                 pw[i] = f2h2_nosat(a, b);
                 if constexpr (F32) {
@@ -268,6 +268,14 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 ls = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) weight2(i);
+            }
+            // The sum of rounded weights is off by 16 x 2^-25 / vs at most, 2^-21 of l while 1 / vs <= l.  Where it is not - at first, and in pages whose
+            // values are by far smaller than those the reference comes from, down to nothing but zeros - the unrounded ones are added up.
+            if (__any(back > l)) {
+                float exact = 0.f;
+#pragma unroll
+                for (int k = 0; k < 16; ++k) exact += exp2_(__builtin_fmaf(x[k], ck, em));
+                ls = back > l ? exact : ls;
             }
             if (sb == 0) __syncthreads();      // the next tile's stage is written
             sc = scn;

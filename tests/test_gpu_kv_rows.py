@@ -157,6 +157,30 @@ def test_the_cases_reach_both_ways_of_sharing():
     assert [s > 0 for s in size] == [False, False, False, True, True, False, True, True, True, False, False, True, False], size
 
 
+@pytest.mark.parametrize("case", [0, 1, 2, 3, 4, 6, 7, 10])
+@pytest.mark.parametrize("low", [None, -32, -18])
+def test_values_whose_pages_differ_in_scale(case, low):
+    """V pages of nothing but zeros (the least scale, 2^-32) or 2^11 .. 2^26 smaller than the others: their tokens still count in the softmax sum,
+    whatever their weight times their scale is to the largest's"""
+    B, kv, heads, hd, page, width, most, causal, window, scale, typ = MANY[case]
+    causal, window = 0, 0      # every row sees many pages
+    cache, vals, table, g = make_cache(B, width, kv, page, hd, 400 + case)
+    small = torch.rand((cache.pages, kv), generator=g, device=DEV) < 0.5
+    if low is None:
+        cache.v_pages[small] = 0
+        vals[1][small] = 0
+    e = -32 if low is None else low
+    was = cache.v_scale.double()
+    cache.v_scale[small] = 2.0 ** e
+    vals[1] *= torch.where(small, 2.0 ** e / was, torch.ones_like(was))[..., None, None]
+    lens, new = [width * page - b % 7 for b in range(B)], ragged(B, most, 500 + case, 1)
+    cu = offsets(new)
+    q = torch.randn((cu[-1], heads * hd), generator=g, device=DEV).to(DT[typ])
+    want, wv, amax = attention64(q, vals, table, lens, cu, heads, causal, window, scale)
+    got = ops.kv_attention(q, cache, table, ints(lens), ints(cu), heads=heads, causal=causal, window=window, scale=scale, max_new=most)
+    close(got, want.cpu(), attn_tol(typ, want, wv, amax, max(lens)).cpu(), "case %d" % case)
+
+
 def test_many_segments_of_few_rows():
     """more (sequence, column tile) pairs than a workgroup looks up at once, most of them empty; single tokens in pieces"""
     kv, heads, hd, page, width, B, most = 2, 8, 64, 16, 70, 300, 9
