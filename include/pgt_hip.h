@@ -352,8 +352,8 @@ int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const
  * h / (heads / kv_heads)).  lens: tokens INCLUDING the rows' own: row i of n of sequence b is at position p = lens[b] - n + i.
  *   causal == 0: sees tokens < lens[b].   causal = c >= 1: tokens < e = (p / c + 1) * c (and < lens[b]): c = 1 token by token, c = 1024 the whole
  *   frames of 1024 tokens up to its own.  window = w > 0 (with causal): of these the tokens >= e - w.
- * Weights carry 11 bits (fp32: 22), sums 32; a weight that times its page's V scale is under 2^-32 of the row's largest such product adds to
- * the softmax sum only.
+ * Weights carry 11 bits (fp32: 22) in the product with V, and an absolute error of 2^-32 of the row's largest product of a weight and its
+ * page's V scale - less than that adds to the softmax sum only, which is fp32 throughout.
  * A row that sees no token is zero.  Deterministic for one shape of call (B, max_new, width, window choose how the work is split, and with it
  * the order of the sums).  width * page <= 2^31 - 2^16.  workspace: pgt_kv_attention_workspace_bytes(...) bytes (0: may be NULL), scratch
  * of one call - calls that may run concurrently need their own. */

@@ -226,17 +226,17 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             float em = ev - m;
             float ls = 0.f;
             uint32_t pw[8], pl[F32 ? 8 : 1];      // weights in half; fp32: what is left of them, in half
-            const halfx2 ones = {(_Float16)1.f, (_Float16)1.f};
-            auto weight2 = [&](int i) {      // weights 2 i, 2 i + 1; their sum is that of the rounded ones
+            // weights 2 i, 2 i + 1; summed before they are rounded: in half, those of pages whose values are by far smaller than the others' - or
+            // nothing but zeros - vanish, for the product as they should, but not for the sum
+            auto weight2 = [&](int i) {
                 const float a = exp2_(__builtin_fmaf(x[2 * i], ck, em)), b = exp2_(__builtin_fmaf(x[2 * i + 1], ck, em));
                 pw[i] = f2h2_nosat(a, b);
                 if constexpr (F32) {
                     x3_opaque(pw[i]);
                     const halfx2 w = __builtin_bit_cast(halfx2, pw[i]);
                     pl[i] = f2h2_nosat(a - (float)w.x, b - (float)w.y);
-                    ls = __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, pl[i]), ones, ls, false);
                 }
-                ls = __builtin_amdgcn_fdot2(__builtin_bit_cast(halfx2, pw[i]), ones, ls, false);
+                ls += a + b;
             };
             const float2 scn = sscale[nst][nsb * 2 + h];
             SLICE();
@@ -268,14 +268,6 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 ls = 0.f;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) weight2(i);
-            }
-            // The sum of rounded weights is off by 16 x 2^-25 / vs at most, 2^-21 of l while 1 / vs <= l.  Where it is not - at first, and in pages whose
-            // values are by far smaller than those the reference comes from, down to nothing but zeros - the unrounded ones are added up.
-            if (__any(back > l)) {
-                float exact = 0.f;
-#pragma unroll
-                for (int k = 0; k < 16; ++k) exact += exp2_(__builtin_fmaf(x[k], ck, em));
-                ls = back > l ? exact : ls;
             }
             if (sb == 0) __syncthreads();      // the next tile's stage is written
             sc = scn;
