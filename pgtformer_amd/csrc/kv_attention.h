@@ -54,8 +54,9 @@ struct AttnP {
     float *po, *pml;                  // partial results: (slot, columns, hd), (slot, columns, {m, l})
     int2* ends;                       // per segment: the workgroups that hold its first and its last piece
     int64_t ldq, ldo;
-    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, cshift, nct, wgs, jrows, causal, window;      // column tiles of 2^cshift; wgs: workgroups that share the work, 0 = one per
-                                      // column tile; jrows: rows of a column tile that the join looks at
+    int pages, pshift, ldt, width, B, rows, max_new, heads, kv, group, causal, window;
+    int cshift, nct, wgs, jrows;      // column tiles of 2^cshift, nct per sequence and kv head; workgroups that share the work, 0 = one per
+                                      // column tile; rows of a column tile that the join looks at
     float c;                          // scale * log2 e
 };
 
@@ -136,9 +137,6 @@ __device__ __forceinline__ Segment segment_of(const AttnP& p, int order, int e) 
     return g;
 }
 __device__ __forceinline__ Segment uni(const Segment& g) { return {uni(g.b), uni(g.hk), uni(g.ct), uni(g.first), uni(g.tiles), uni(g.s)}; }
-struct Line {
-    int total, share;
-};
 // This workgroup's part [pos, end) of the line, the segment e that pos lies in and the line before that; false: nothing (all 64 * W threads;
 // red: W + 2 ints).  In order 1 the kv heads of a column tile are counted at once.
 template <int W, int ORDER>

@@ -527,11 +527,15 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     constexpr int JR = 4;
 #define ATTN_GO(TT, HD_)                                                                                              \
     do {                                                                                                              \
-        if (w.cshift != 4) {}                                                                                         \
-        else if (p.nct == 1) hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, true>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p); \
-        else hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, false>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);      \
-        if (p.wgs && w.cshift == 4) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), dim3((unsigned)(w.segs * p.jrows)), dim3(256), 0, st, p); \
-        else if (p.wgs) hipLaunchKernelGGL((kv_attn_join_rows_kernel<TT, HD_, JR>), dim3((unsigned)(w.segs * (HD_ / 4 / JR))), dim3(256), 0, st, p); \
+        if (w.cshift == 4) {                                                                                          \
+            if (p.nct == 1) hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, true>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);\
+            else hipLaunchKernelGGL((kv_attn_kernel<TT, HD_, false>), dim3((unsigned)wgs), dim3(64 * NW), 0, st, p);  \
+            const dim3 rows((unsigned)(w.segs * p.jrows));                                                            \
+            if (p.wgs) hipLaunchKernelGGL((kv_attn_join_kernel<TT, HD_>), rows, dim3(256), 0, st, p);                 \
+        } else if constexpr (!__is_same(TT, float) || HD_ == 64) {      /* the 256-column kernel has no other fp32 form */\
+            const dim3 rows((unsigned)(w.segs * (HD_ / 4 / JR)));                                                     \
+            if (p.wgs) hipLaunchKernelGGL((kv_attn_join_rows_kernel<TT, HD_, JR>), rows, dim3(256), 0, st, p);        \
+        }                                                                                                             \
     } while (0)
 #define ATTN_HD(TT)                                                                                                   \
     do {                                                                                                              \
