@@ -591,11 +591,9 @@ def test_graph_replay_after_the_allocator_returned_memory_to_the_driver(models):
 
 
 def test_captured_forward_has_no_fork(models):
-    """The root cause of the segfault inside hipGraphLaunch (DESIGN.md section 3.4): ROCm 7.0's hip::Graph::UpdateStreams searches, for every
-    root of a graph beyond the first, the executable graph's internal streams for one on another hardware queue than the launch stream - without
-    bounding the search (rocgdb: both internal streams on the launch stream's queue, index past the end, null dereference).  A graph with one root
-    never enters the loop, so a forward that is being captured must not fork its condition branch onto the side stream; eager forwards keep the
-    fork; frames are bit-identical either way."""
+    """A forward that is being captured does not fork its condition branch onto the side stream: in long processes hipGraphLaunch (ROCm 7.0)
+    has ended in a segmentation fault on graphs with more than one root, which a captured fork makes, and never on graphs with one root.  Eager
+    forwards keep the fork; frames are bit-identical either way."""
     from pgtformer_amd.driver import WindowRunner
     from pgtformer_amd.synth import make_clip
 
