@@ -167,6 +167,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             }
             if (BOTH || part == 1) {
                 uint4 w = BOTH ? rb : ra;
+                if (!have0) w = make_uint4(0, 0, 0, 0);      // no page: page 0 was read in its place, and its NaN times the weight 0 would be one
                 if (((t * 64 < all_lo) | (t * 64 + 64 > all_hi)) & (t < te)) {
                     // NaN times the weight 0 of a query that does not see the token: zeros here, see the end
                     const uint4 n = make_uint4(nan_bytes(w.x), nan_bytes(w.y), nan_bytes(w.z), nan_bytes(w.w));

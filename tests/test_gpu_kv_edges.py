@@ -1,0 +1,36 @@
+"""Cached-attention operators at the edges of their definitions (include/pgt_hip.h): pages that are not there in front of a page of NaN, sequences with
+more rows than the call processes, pages that nobody wrote, scores of any size, broken offsets, caches past 4 GiB at many rows, recorded calls."""
+import pytest
+import torch
+
+from pgtformer_amd import ops
+from tests import kv_ref
+from tests.test_gpu_kv import DEV, DT, HALF, TINY, attn_tol, close, filled, gpu_codes
+from tests.test_gpu_kv_rows import MANY, attention64, ints, make_cache, offsets, ragged
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("case", [0, 1, 3, 4, 7, 10, 12])
+@pytest.mark.parametrize("most", [0, 2])
+def test_missing_pages_while_page_0_holds_nan(case, most):
+    """a token without a page is not seen, whatever the page holds that is read in its place (the first one, another sequence's): here NaN, K and V"""
+    B, kv, heads, hd, page, width, n, causal, window, scale, typ = MANY[case]
+    n = most or n
+    cache, vals, table, g = make_cache(B, width, kv, page, hd, 700 + case)
+    table[table == 0] = (set(range(cache.pages)) - set(table.flatten().tolist())).pop() if 0 in table else 0
+    assert 0 not in table
+    cache.k_pages[0], cache.v_pages[0] = 0xff, 0x7f
+    for t in vals:
+        t[0] = float("nan")
+    for b in range(B):      # in the middle, at the beginning and at the end of what is seen
+        for i in {(width // 2 + b) % width, 0 if b % 3 == 0 else width // 2, width - 1 if b % 5 == 0 else width // 3}:
+            table[b, i] = (-1, cache.pages, 1 << 30)[(b + i) % 3]
+    lens, new = [width * page - b % 5 for b in range(B)], ragged(B, n, 710 + case, 1)
+    cu = offsets(new)
+    q = torch.randn((cu[-1], heads * hd), generator=g, device=DEV).to(DT[typ])
+    for order in ((causal, window), (0, 0)):
+        want, wv, amax = attention64(q, vals, table, lens, cu, heads, *order, scale)
+        got = ops.kv_attention(q, cache, table, ints(lens), ints(cu), heads=heads, causal=order[0], window=order[1], scale=scale, max_new=n)
+        assert not bool(want.isnan().any()) and not bool(got.isnan().any()), (order, int(got.isnan().sum()))
+        close(got, want.cpu(), attn_tol(typ, want, wv, amax, max(lens)).cpu(), order)
