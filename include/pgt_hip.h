@@ -341,15 +341,15 @@ int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const
  *   page and head is <= 448 * 2^e.  Larger values and infinities saturate, NaN stays NaN and does not count for the scale.
  * table (B, ld_table) int32: table[b][i] = page that holds tokens i * page .. of sequence b, `width` entries used; entries outside
  * [0, pages) and tokens past width * page are not there: nothing is written to them, they read as zeros, attention does not see them.
- * Sequence b owns rows cu[b] .. cu[b + 1] - 1 of the packed rows (cu: B + 1 int32 on the device, non-decreasing), at most max_new / max_rows
- * of them; cu == NULL: rows b * max_new .. .  Rows that no sequence owns are neither read nor written.  lens, start: int32 (B),
+ * Sequence b owns rows cu[b] .. cu[b + 1] - 1 of the packed rows (cu: B + 1 int32 on the device, non-decreasing), of which a call processes the first
+ * max_new / max_rows; cu == NULL: rows b * max_new .. .  Rows that no sequence owns or the call does not process are neither read nor written.  lens, start: int32 (B),
  * negative = 0.  All index tensors live on the device and are bounded there: no value of theirs reaches outside the buffers.
  * pgt_kv_append: writes the rows k, v (kv_heads * hd) of sequence b to its tokens lens[b] .. (lens: tokens BEFORE the call).  A page that
  * held tokens of the sequence keeps the larger of its scale and the new tokens' - its codes are re-expressed under it; a page that begins
  * here is written whole, zeros behind the last token.  A page that is written to must belong to one sequence.
  * pgt_kv_read: rows of sequence b <- its tokens start[b] .. , values rounded once to dtype.
  * pgt_kv_attention: out = softmax(scale * q K^T) V; q, out rows of heads * hd, `heads` a multiple of kv_heads (head h reads kv head
- * h / (heads / kv_heads)).  lens: tokens INCLUDING the rows' own: row i of n of sequence b is at position p = lens[b] - n + i.
+ * h / (heads / kv_heads)).  lens: tokens INCLUDING the rows' own: row i of the n rows that sequence b owns is at position p = lens[b] - n + i.
  *   causal == 0: sees tokens < lens[b].   causal = c >= 1: tokens < e = (p / c + 1) * c (and < lens[b]): c = 1 token by token, c = 1024 the whole
  *   frames of 1024 tokens up to its own.  window = w > 0 (with causal): of these the tokens >= e - w.
  * Weights carry 11 bits (fp32: 22) in the product with V, and an absolute error of 2^-32 of the row's largest product of a weight and its

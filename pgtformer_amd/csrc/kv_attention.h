@@ -60,20 +60,23 @@ struct AttnP {
     float c;                          // scale * log2 e
 };
 
-// sequence b: its packed rows and its tokens in the cache (which end with the rows' own)
+// sequence b: its packed rows (those that are processed: max_new at most), its tokens in the cache (which end with ALL its rows' own) and the position of
+// its first row
 struct Seq {
-    int r0, n, len;
+    int r0, n, len, p0;
 };
 __device__ __forceinline__ Seq seq_of(const AttnP& p, int b) {
     Seq s;
+    int n = p.max_new;
     if (p.cu) {
         s.r0 = min(max(p.cu[b], 0), p.rows);
-        s.n = min(min(max(p.cu[b + 1], s.r0), p.rows) - s.r0, p.max_new);
+        n = min(max(p.cu[b + 1], s.r0), p.rows) - s.r0;
     } else {
         s.r0 = b * p.max_new;
-        s.n = p.max_new;
     }
+    s.n = min(n, p.max_new);
     s.len = min(max(p.lens[b], 0), p.width << p.pshift);
+    s.p0 = s.len - n;
     return s;
 }
 // tokens [lo, hi) that the query at position pos (of a sequence of len tokens) sees
@@ -92,7 +95,7 @@ __device__ __forceinline__ void sees(const AttnP& p, int len, int pos, int& lo, 
 
 // values that every lane of a wave holds alike but that came from memory, into scalar registers
 __device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
-__device__ __forceinline__ Seq uni(const Seq& s) { return {uni(s.r0), uni(s.n), uni(s.len)}; }
+__device__ __forceinline__ Seq uni(const Seq& s) { return {uni(s.r0), uni(s.n), uni(s.len), uni(s.p0)}; }
 __device__ __forceinline__ void sees_uni(const AttnP& p, int len, int pos, int& lo, int& hi) {
     sees(p, len, pos, lo, hi);
     lo = uni(lo);
@@ -129,8 +132,8 @@ __device__ __forceinline__ Segment segment_of(const AttnP& p, int order, int e) 
     g.first = g.tiles = 0;
     if (c0 < cols) {
         int lo, hi, dummy;
-        sees(p, s.len, s.len - s.n + (c0 == 0 ? 0 : c0 / p.group), lo, dummy);
-        sees(p, s.len, s.len - s.n + (cz == cols - 1 ? s.n - 1 : cz / p.group), dummy, hi);
+        sees(p, s.len, s.p0 + (c0 == 0 ? 0 : c0 / p.group), lo, dummy);
+        sees(p, s.len, s.p0 + (cz == cols - 1 ? s.n - 1 : cz / p.group), dummy, hi);
         g.first = lo >> 6;
         g.tiles = max(((hi + 63) >> 6) - g.first, 0);
     }

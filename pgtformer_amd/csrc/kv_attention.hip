@@ -51,11 +51,11 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
     if (ct * 16 >= cols) return;
     const int qc = min(ct * 16 + col, cols - 1), qi = qc / p.group, qg = qc - qi * p.group;
     int lo, hi;
-    sees(p, s.len, s.len - s.n + qi, lo, hi);
+    sees(p, s.len, s.p0 + qi, lo, hi);
     // what every query of the tile sees: from the last one's first token to the first one's last
     int hi_a, lo_z, dummy;
-    sees_uni(p, s.len, s.len - s.n + ct * 16 / p.group, dummy, hi_a);
-    sees_uni(p, s.len, s.len - s.n + min(ct * 16 + 15, cols - 1) / p.group, lo_z, dummy);
+    sees_uni(p, s.len, s.p0 + ct * 16 / p.group, dummy, hi_a);
+    sees_uni(p, s.len, s.p0 + min(ct * 16 + 15, cols - 1) / p.group, lo_z, dummy);
     int hk = sg.hk;
     if (p.wgs) {      // (the look-up gives the first kv head)
         hk = (pos - before) / sg.tiles;

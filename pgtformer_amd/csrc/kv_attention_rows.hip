@@ -60,7 +60,7 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         if (p.wgs && sg.tiles == 0) { ++e; continue; }
         const int b = sg.b, hk = sg.hk, ct = sg.ct;
         const Seq& s = sg.s;
-        const int cols = s.n * p.group, shift = s.len - s.n;
+        const int cols = s.n * p.group, shift = s.p0;
         if (ct * CT >= cols) return;
         const int t0 = sg.first + (p.wgs ? pos - before : 0), te = p.wgs ? sg.first + min(pos_end - before, sg.tiles) : sg.first + sg.tiles;
         const bool whole = te - t0 == sg.tiles;

@@ -34,3 +34,21 @@ def test_missing_pages_while_page_0_holds_nan(case, most):
         got = ops.kv_attention(q, cache, table, ints(lens), ints(cu), heads=heads, causal=order[0], window=order[1], scale=scale, max_new=n)
         assert not bool(want.isnan().any()) and not bool(got.isnan().any()), (order, int(got.isnan().sum()))
         close(got, want.cpu(), attn_tol(typ, want, wv, amax, max(lens)).cpu(), order)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("B,n,most,heads", [(3, 9, 4, 4), (3, 9, 1, 8), (40, 90, 60, 16)])
+def test_more_rows_than_the_call_processes(typ, B, n, most, heads):
+    """max_new below a sequence's rows: its first max_new rows, each at the position it has among all of them; the others stay as they were"""
+    kv, hd, page, width = 4, 64, 16, 40
+    cache, vals, table, g = make_cache(B, width, kv, page, hd, 720)
+    lens, new = ragged(B, width * page, 721, n), ragged(B, n, 722, 1)
+    cu = offsets(new)
+    q = torch.randn((cu[-1], heads * hd), generator=g, device=DEV).to(DT[typ])
+    done = torch.cat([torch.arange(c) < most for c in new])
+    for causal, window in ((1, 0), (1, 40), (16, 0), (0, 0)):
+        want, wv, amax = attention64(q, vals, table, lens, cu, heads, causal, window, 0.125)
+        out = torch.full((cu[-1], heads * hd), 3.0, dtype=DT[typ], device=DEV)
+        got = ops.kv_attention(q, cache, table, ints(lens), ints(cu), heads=heads, causal=causal, window=window, max_new=most, out=out)
+        close(got[done.to(DEV)], want.cpu()[done], attn_tol(typ, want, wv, amax, max(lens)).cpu()[done], (causal, window))
+        assert bool((got[~done.to(DEV)] == 3).all())
