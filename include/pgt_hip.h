@@ -339,6 +339,7 @@ int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const
  *   k_pages (pages, kv_heads, hd / 16, page, 16), v_pages (pages, kv_heads, page / 16, hd, 16): e4m3 codes (OCP, no infinities);
  *   k_scale, v_scale (pages, kv_heads) fp32: value = code * scale, scale = 2^e with the least e in [-32, 32] for which the largest |x| of the
  *   page and head is <= 448 * 2^e.  Larger values and infinities saturate, NaN stays NaN and does not count for the scale.
+ *   Memory that was only cleared is a cache of zeros: a scale of 0 counts as 2^-32.
  * table (B, ld_table) int32: table[b][i] = page that holds tokens i * page .. of sequence b, `width` entries used; entries outside
  * [0, pages) and tokens past width * page are not there: nothing is written to them, they read as zeros, attention does not see them.
  * Sequence b owns rows cu[b] .. cu[b + 1] - 1 of the packed rows (cu: B + 1 int32 on the device, non-decreasing), of which a call processes the first

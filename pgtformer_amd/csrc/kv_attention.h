@@ -41,6 +41,8 @@ __device__ __forceinline__ void split3(const float* p, uint4& hi, uint4& mid, ui
         (pl == 0 ? hi : pl == 1 ? mid : lo) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
+// log2 of a page's scale, a power of two from 2^-32 on (0 - memory that was only cleared - as that: its tokens count as the zeros they are)
+__device__ __forceinline__ float log2_scale(float s) { return (float)max((int)((__float_as_uint(s) >> 23) & 255) - 127, -32); }
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 // does any of the four codes stand for NaN (0x7f, 0xff)?
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }

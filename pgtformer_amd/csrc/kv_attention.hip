@@ -161,7 +161,7 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
                 }
             }
         }
-        const float ev = (float)((int)((__float_as_uint(sv_t) >> 23) & 255) - 127), ck = p.c * sk_t;
+        const float ev = log2_scale(sv_t), ck = p.c * sk_t;
         const bool masked = (t * 64 < lo_z) | (t * 64 + 64 > hi_a) | (__any(!here) != 0);
         float y[16], mx = -INFINITY;
 #pragma unroll

@@ -1210,11 +1210,12 @@ class KvCache:
 
     @classmethod
     def alloc(cls, pages, kv_heads, page, hd, device="cuda"):
+        """a cache of zeros, as kv_append writes them: codes 0, scales 2^-32 (the least there is; a scale of 0 is none)"""
         _need(pages > 0 and kv_heads > 0 and page in (16, 32, 64, 128) and hd in (64, 128),
               "KvCache: pages=%d kv_heads=%d page=%d (16, 32, 64, 128) head_dim=%d (64, 128)", pages, kv_heads, page, hd)
-        z = lambda *shape, dt=torch.uint8: torch.zeros(shape, dtype=dt, device=device)      # noqa: E731
-        return cls(z(pages, kv_heads, hd // 16, page, 16), z(pages, kv_heads, page // 16, hd, 16),
-                   z(pages, kv_heads, dt=torch.float32), z(pages, kv_heads, dt=torch.float32))
+        codes = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=device)      # noqa: E731
+        scale = lambda: torch.full((pages, kv_heads), 2.0 ** -32, dtype=torch.float32, device=device)      # noqa: E731
+        return cls(codes(pages, kv_heads, hd // 16, page, 16), codes(pages, kv_heads, page // 16, hd, 16), scale(), scale())
 
 
 def _seq_args(table, lens, cu, rows, most, what):

@@ -52,3 +52,32 @@ def test_more_rows_than_the_call_processes(typ, B, n, most, heads):
         got = ops.kv_attention(q, cache, table, ints(lens), ints(cu), heads=heads, causal=causal, window=window, max_new=most, out=out)
         close(got[done.to(DEV)], want.cpu()[done], attn_tol(typ, want, wv, amax, max(lens)).cpu()[done], (causal, window))
         assert bool((got[~done.to(DEV)] == 3).all())
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("n", [1, 3, 64])
+def test_pages_that_nobody_wrote_hold_zeros(typ, n):
+    """tokens of a fresh cache's pages count in the softmax sum as tokens of zeros do"""
+    B, kv, heads, hd, page, width = 40, 2, 16, 64, 32, 12
+    g = torch.Generator().manual_seed(730)
+    table = torch.arange(B * width, dtype=torch.int32, device=DEV).reshape(B, width)
+    fresh, zeros = (ops.KvCache.alloc(B * width, kv, page, hd, DEV) for _ in range(2))
+    rows = torch.zeros((B * width * page, kv * hd), device=DEV)
+    ops.kv_append(zeros, rows, rows, table, ints([0] * B))
+    some = torch.randn((B * page, kv * hd), generator=g).to(DEV)
+    for c in (fresh, zeros):      # the second page of every sequence
+        ops.kv_append(c, some, some, table, ints([page] * B))
+    lens = [width * page - b for b in range(B)]
+    q = torch.randn((B * n, heads * hd), generator=g).to(DT[typ]).to(DEV)
+    k, v = (t.double().reshape(B, -1, kv, hd) for t in ops.kv_read(fresh, table, ints([0] * B), B * width * page, torch.float32))
+    vals = [t.reshape(B * width, page, kv, hd).transpose(1, 2) for t in (k, v)]
+    assert bool((vals[1][0] == 0).all()) and bool((vals[1][1] != 0).any())
+    cu = [n * b for b in range(B + 1)]
+    want, wv, amax = attention64(q, vals, table, lens, cu, heads, 1, 0, 0.3)
+    got = [ops.kv_attention(q, c, table, ints(lens), heads=heads, scale=0.3) for c in (fresh, zeros)]
+    assert torch.equal(*got)
+    close(got[0], want.cpu(), attn_tol(typ, want, wv, amax, max(lens)).cpu())
+    # memory that was only cleared: scales of 0
+    raw = ops.KvCache(*(torch.zeros_like(t) for t in (fresh.k_pages, fresh.v_pages, fresh.k_scale, fresh.v_scale)))
+    ops.kv_append(raw, some, some, table, ints([page] * B))
+    assert torch.equal(got[0], ops.kv_attention(q, raw, table, ints(lens), heads=heads, scale=0.3))
