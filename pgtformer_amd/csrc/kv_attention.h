@@ -104,7 +104,7 @@ __device__ __forceinline__ void sees_uni(const AttnP& p, int len, int pos, int& 
     hi = uni(hi);
 }
 
-constexpr float NEVER = -1e30f;      // reference of a query that has seen nothing (finite: differences and products stay numbers)
+constexpr float NEVER = -3.402823466e38f;      // reference of a query that has seen nothing: below every score, finite (so that NEVER - NEVER is 0)
 constexpr int MIN_SHARE = 4;         // tiles of a piece
 
 // Work sharing (wgs > 0).  The tiles of 64 tokens of all segments - (sequence, column tile, kv head), in an order of the kernel's - are one line

@@ -175,8 +175,8 @@ template <typename T, int HD, bool ONCE> __global__ __launch_bounds__(64 * NW, 2
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, y[e]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
         mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        if (__any(mx > m + 15.f)) {
-            const float mn = mx > m + 15.f ? mx - 7.f : m;      // each query by itself: its result does not depend on its neighbours
+        if (__any(mx - m > 15.f)) {      // (a difference: m + 15 would be rounded, to m + 16 from 2^25 on, and 2^16 is no half)
+            const float mn = mx - m > 15.f ? mx - 7.f : m;      // each query by itself: its result does not depend on its neighbours
             const float al = exp2_(m - mn);
             l *= al;
 #pragma unroll

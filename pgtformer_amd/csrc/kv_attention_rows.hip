@@ -143,6 +143,11 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
         };
         f32x16 o[ND];
         float m = NEVER, l = 0.f;
+        // most: what a lane's 16 weights may sum up to before the query's reference is looked at.  x ck + (ev - m) adds an unrounded product to a rounded
+        // difference, which cancel to within the rounding of m only: from some 2^27 on that is more exponents than half has.  The weights of such a
+        // query are always taken again, from the rounded score that m came from (most < 0; finite scores of any size: one weight of 1 is left)
+        float most = 32768.f;
+        auto far = [&]() { return fabsf(m) > 1048576.f && m != NEVER; };
 #pragma unroll
         for (int d = 0; d < ND; ++d) o[d] = zero16();
 
@@ -224,13 +229,15 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
 #pragma unroll
                 for (int k = 0; k < 16; ++k) x[k] = (uint32_t)(at + k) < span ? x[k] : -INFINITY;
             }
-            float em = ev - m;
             float ls = 0.f;
             uint32_t pw[8], pl[F32 ? 8 : 1];      // weights in half; fp32: what is left of them, in half
             // weights 2 i, 2 i + 1; summed before they are rounded: in half, those of pages whose values are by far smaller than the others' - or
             // nothing but zeros - vanish, for the product as they should, but not for the sum
-            auto weight2 = [&](int i) {
-                const float a = exp2_(__builtin_fmaf(x[2 * i], ck, em)), b = exp2_(__builtin_fmaf(x[2 * i + 1], ck, em));
+            float add = ev - m, less = 0.f;
+            auto weight2 = [&](int i, bool again = false) {
+                float a = __builtin_fmaf(x[2 * i], ck, add), b = __builtin_fmaf(x[2 * i + 1], ck, add);
+                if (again) a -= less, b -= less;
+                a = exp2_(a), b = exp2_(b);
                 pw[i] = f2h2_nosat(a, b);
                 if constexpr (F32) {
                     x3_opaque(pw[i]);
@@ -253,22 +260,24 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             // A query whose weights passed 2^15 in sum (each fits half until then) takes a new reference, 7 under its largest score, and its weights
             // again - each query by itself: its result does not depend on its neighbours.  A maximum ahead of the weights would cost 12
             // instructions more, and its way from the products to the exponentials stands between the steps.
-            if (__any(!(ls <= 32768.f))) {
+            if (__any(!(ls <= most))) {
                 float mx = x[0];
 #pragma unroll
                 for (int k = 1; k < 16; ++k) mx = fmaxf(mx, x[k]);
                 const float tm = max_of_halves(__builtin_fmaf(mx, ck, ev));
-                const bool over = max_of_halves(ls <= 32768.f ? 0.f : 1.f) > 0.f;
-                const float mn = over && tm > m + 10.f ? tm - 7.f : m;
+                const bool over = (max_of_halves(ls <= 32768.f ? 0.f : 1.f) > 0.f) | far();
+                const float mn = over && tm - m > 10.f ? tm - 7.f : m;
                 const float al = exp2_(m - mn);
                 l *= al;
 #pragma unroll
                 for (int d = 0; d < ND; ++d) o[d] *= al;
                 m = mn;
-                em = ev - m;
+                most = far() ? -1.f : 32768.f;
+                add = far() ? ev : ev - m;
+                less = far() ? m : 0.f;
                 ls = 0.f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) weight2(i);
+                for (int i = 0; i < 8; ++i) weight2(i, true);
             }
             if (sb == 0) __syncthreads();      // the next tile's stage is written
             sc = scn;

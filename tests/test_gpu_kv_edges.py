@@ -81,3 +81,43 @@ def test_pages_that_nobody_wrote_hold_zeros(typ, n):
     raw = ops.KvCache(*(torch.zeros_like(t) for t in (fresh.k_pages, fresh.v_pages, fresh.k_scale, fresh.v_scale)))
     ops.kv_append(raw, some, some, table, ints([page] * B))
     assert torch.equal(got[0], ops.kv_attention(q, raw, table, ints(lens), heads=heads, scale=0.3))
+
+
+@pytest.mark.parametrize("scale", [3e6, 5e7, 2e8, 7e9, 1e14, 3e31])
+@pytest.mark.parametrize("case,n", [(0, 0), (1, 0), (3, 0), (4, 0), (10, 0), (12, 0), (3, 1), (11, 2)])
+def test_scores_of_any_size(case, n, scale):
+    """finite scores, far apart: the row of the largest, whatever their size and sign.  Differences of distinct scores are beyond the exponential's range,
+    so the weights are 1 and 0: what is left is the rounding of the one weight in the product (half: 2^-11; fp32: two halves 2^-22, and the quotient's
+    two roundings) and of the output."""
+    B, kv, heads, hd, page, width, most, causal, window, _, typ = MANY[case]
+    most = n or most
+    causal, window = 0, 0
+    cache, vals, table, g = make_cache(B, width, kv, page, hd, 740 + case)
+    lens, new = [width * page - b % 7 for b in range(B)], ragged(B, most, 741, 1)
+    cu = offsets(new)
+    for sign in (1, -1):      # the second time: all products of one sign, so that every score is far below zero
+        q = torch.randn((cu[-1], heads * hd), generator=g, device=DEV).to(DT[typ])
+        if sign < 0:
+            q = q.abs()
+            cache.k_pages.bitwise_and_(0x7f)
+            vals[0].abs_()
+        # the largest and the second largest score of every row and head, in 64 bits
+        want, best = torch.zeros((cu[-1], heads, hd), dtype=torch.float64, device=DEV), torch.zeros((cu[-1], heads), dtype=torch.bool, device=DEV)
+        for b in range(B):
+            k, v = (t[table[b].long()].transpose(1, 2).reshape(-1, kv, hd)[:lens[b]] for t in vals)
+            for h in range(heads):
+                hk = h * kv // heads
+                qq = q[cu[b]:cu[b + 1], h * hd:(h + 1) * hd].double()
+                kt = k[:, hk].t().contiguous()
+                x = torch.matmul(qq, kt) * (sign * scale)
+                top, at = x.topk(2, -1)
+                bound = 2.0 ** -15 * torch.matmul(qq.abs(), kt.abs()).amax(-1) * scale      # far above the fp32 sums' rounding
+                best[cu[b]:cu[b + 1], h] = top[:, 0] - top[:, 1] > bound + 1000
+                want[cu[b]:cu[b + 1], h] = v[at[:, 0], hk]
+        got = ops.kv_attention(q, cache, table, ints(lens), ints(cu), heads=heads, causal=causal, window=window, scale=sign * scale, max_new=most)
+        assert bool(torch.isfinite(got).all()), (sign, int((~torch.isfinite(got)).sum()))
+        pick = best[..., None].expand_as(want).reshape(cu[-1], -1)
+        assert bool(best.any())
+        want = want.reshape(cu[-1], -1)
+        tol = (HALF[typ] + 2.0 ** (-21 if typ == "f32" else -11)) * (1 + 2.0 ** -7) * want.abs() + TINY[typ]
+        close(got[pick], want[pick].cpu(), tol[pick].cpu(), sign)
