@@ -1062,13 +1062,16 @@ def _pointers(*ts):
 
 
 def _apart(outs, ins, what):
-    """outputs a caller passed: each may be one of the inputs itself, but must not overlap one in another way, nor another output"""
+    """outputs a caller passed: output i may be one of its own inputs itself - ins[i], ins[i + len(outs)], ... - which are read where it is written, but must
+    not overlap an input in another way (nor be another's), nor another output"""
+    n = len(outs)
     for i, o in enumerate(outs):
-        for x in list(ins) + list(outs[:i]):
+        for j, x in enumerate(list(ins) + list(outs[:i])):
             if o.numel() == 0 or x.numel() == 0 or o.untyped_storage().data_ptr() != x.untyped_storage().data_ptr():
                 continue
             es, ld = o.element_size(), (o.stride(0) if o.shape[0] > 1 else x.stride(0))
-            if any(x is t for t in ins) and o.data_ptr() == x.data_ptr() and (o.stride(0) == x.stride(0) or o.shape[0] <= 1) and o.shape == x.shape:
+            own = j < len(ins) and j % n == i
+            if own and o.data_ptr() == x.data_ptr() and (o.stride(0) == x.stride(0) or o.shape[0] <= 1) and o.shape == x.shape:
                 continue
             end = lambda t: t.data_ptr() + es * ((t.shape[0] - 1) * t.stride(0) + t.shape[1])      # noqa: E731
             if end(o) <= x.data_ptr() or end(x) <= o.data_ptr():
@@ -1148,8 +1151,8 @@ def _rope_args(q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, out, wha
 
 def qk_norm_rope(q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_heads, eps=1e-6, interleaved=False, out=None):
     """Per-head RMS norm (gains fp32 (hd,) or None) of q (rows, heads * hd) and k (rows, kv_heads * hd) and the rotation by their positions
-    (int32 (rows,); freqs: rope_freqs(rot), None = no rotation) in one pass -> (q_out, k_out).  out: the two outputs, which may be q and
-    k themselves.  interleaved: pairs (2i, 2i + 1) instead of (i, i + rot / 2)."""
+    (int32 (rows,); freqs: rope_freqs(rot), None = no rotation) in one pass -> (q_out, k_out).  out: the two outputs; the first may be q
+    itself, the second k.  interleaved: pairs (2i, 2i + 1) instead of (i, i + rot / 2)."""
     if out is None and (nat := _native(q)) is not None:
         r = nat[0].qk_norm_rope(nat[1], nat[2], q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, eps, True if interleaved else False)
         if r is not None:
@@ -1165,7 +1168,7 @@ def qk_norm_rope(q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_
 
 def qk_norm_rope_backward(dq, dk, q, k, positions, freqs, q_gain=None, k_gain=None, *, heads, kv_heads, eps=1e-6, interleaved=False, out=None):
     """Gradients of qk_norm_rope: (dq, dk) of its outputs, its inputs q, k -> (gradient of q, of k, of q_gain, of k_gain; the gains' fp32
-    (hd,)).  out: where the first two go (dq, dk themselves are allowed)."""
+    (hd,)).  out: where the first two go (the first may be dq or q itself, the second dk or k)."""
     what = "qk_norm_rope_backward"
     if out is None and (nat := _native(q)) is not None:
         r = nat[0].qk_norm_rope_backward(nat[1], nat[2], q, k, positions, freqs, q_gain, k_gain, heads, kv_heads, eps, True if interleaved else False, dq, dk)
