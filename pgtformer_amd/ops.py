@@ -1033,14 +1033,18 @@ def _need(ok, what, *args):
         raise hip.PgtError(what % args if args else what)
 
 
+I32_MAX = 2 ** 31 - 1      # sizes, strides and the like are int32 in the C entry points: a larger one would arrive without its upper bits
+
+
 def _rows(t, cols, what, name):
     """row stride of a (rows, cols) matrix whose rows do not overlap"""
     shape, stride = t.shape, t.stride()
     if len(shape) == 2 and shape[1] == cols and stride[1] == 1:
-        if shape[0] <= 1:
-            return cols
-        if stride[0] >= cols:
-            return stride[0]
+        ld = cols if shape[0] <= 1 else stride[0]
+        if ld > I32_MAX or shape[0] > I32_MAX:
+            raise hip.PgtError("%s: %s has shape %s, strides %s: more than 31 bits" % (what, name, tuple(shape), stride))
+        if ld >= cols:
+            return ld
     raise hip.PgtError("%s: %s has shape %s, strides %s; (rows, %d) wanted, elements of a row adjacent, rows not overlapping" % (
         what, name, tuple(shape), stride, cols))
 
@@ -1227,6 +1231,8 @@ def _seq_args(table, lens, cu, rows, most, what):
     if len(shape) != 2 or table.dtype is not torch.int32 or (shape[1] > 1 and stride[1] != 1) or (shape[0] > 1 and stride[0] < shape[1]):
         raise hip.PgtError("%s: int32 table (B, width) wanted, got %s %s" % (what, table.dtype, tuple(shape)))
     B, width = shape
+    if max(B, width, stride[0] if B > 1 else 0, rows) > I32_MAX:
+        raise hip.PgtError("%s: table of shape %s, strides %s, %d rows: more than 31 bits" % (what, tuple(shape), stride, rows))
     _vec(lens, torch.int32, B, what, "lens")
     if cu is None:
         if B <= 0 or rows % B or (most is not None and most != rows // B):
@@ -1295,6 +1301,7 @@ def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=
         if r is not None:
             return _done(r, "pgt_kv_attention")
     rows, hd = q.shape[0], cache.hd
+    _need(0 <= causal <= I32_MAX and 0 <= window <= I32_MAX, "kv_attention: causal=%s window=%s", causal, window)
     B, width, ldt, most = _seq_args(table, lens, cu, rows, max_new, "kv_attention")
     ldq = _rows(q, heads * hd, "kv_attention", "q")
     if out is None:

@@ -1,4 +1,4 @@
-"""Cached-attention operators without a GPU: what a fresh cache holds, outputs that a caller may not pass"""
+"""Cached-attention operators without a GPU: what a fresh cache holds, outputs that a caller may not pass, sizes of more than 31 bits"""
 import pytest
 import torch
 
@@ -32,3 +32,25 @@ def test_an_output_is_no_other_outputs_input():
     for outs, ins in (((b, a), (a, b)), ((a, a), ()), ((b, d), (a, b, c, d)), ((wide[:, 8:520], d), (a, b))):
         with pytest.raises(hip.PgtError, match="overlaps"):
             ops._apart(outs, ins, "t")
+
+
+def test_sizes_past_31_bits_are_refused():
+    """the C entry points take int32: a stride of 2^32 + 512 would arrive there as 512, a window of 2^32 + 5 as 5"""
+    far = lambda *shape, ld, dt=torch.float32: torch.empty_strided(shape, (ld, 1), dtype=dt, device="meta")      # noqa: E731
+    c = ops.KvCache.alloc(4, 2, 16, 64, "cpu")
+    q, k, lens, table = torch.zeros(4, 512), torch.zeros(4, 128), torch.zeros(2, dtype=torch.int32), torch.zeros((2, 2), dtype=torch.int32)
+    for ld in (1 << 31, (1 << 32) + 512):
+        for call in (lambda: ops.kv_attention(far(4, 512, ld=ld), c, table, lens, heads=8), lambda: ops.kv_attention(q, c, table, lens, heads=8, out=far(4, 512, ld=ld)),
+                     lambda: ops.kv_attention(q, c, far(2, 2, ld=ld, dt=torch.int32), lens, heads=8), lambda: ops.kv_append(c, far(4, 128, ld=ld), k, table, lens),
+                     lambda: ops.kv_append(c, k, far(4, 128, ld=ld), table, lens),
+                     lambda: ops.kv_read(c, table, lens, 4, torch.float32, out=(far(4, 128, ld=ld), k)),
+                     lambda: ops.qk_norm_rope(far(4, 512, ld=ld), k, None, None, heads=8, kv_heads=2),
+                     lambda: ops.qk_norm_rope_backward(q, far(4, 128, ld=ld), q, k, None, None, heads=8, kv_heads=2)):
+            with pytest.raises(hip.PgtError, match="31 bits"):
+                call()
+    for rows in (1 << 31, 1 << 33):
+        with pytest.raises(hip.PgtError, match="31 bits"):
+            ops.kv_read(c, table, lens, rows, torch.float32)
+    for kw in (dict(window=1 << 32), dict(window=(1 << 32) + 5), dict(causal=(1 << 32) + 1), dict(causal=1 << 31), dict(causal=-1), dict(window=-1)):
+        with pytest.raises(hip.PgtError, match="causal="):
+            ops.kv_attention(q, c, table, lens, heads=8, **kw)
