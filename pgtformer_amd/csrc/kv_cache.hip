@@ -1,10 +1,11 @@
 // Key / value cache in 8 bits: quantise tokens as they are written, read them back.
 //
 // A page holds `page` tokens of every kv head.  Per (page, head) K and V each have one scale 2^e, e the least exponent in [-32, 32] with
-// max |x| <= 448 * 2^e, and codes e4m3(x * 2^-e): with a power of two the product is exact, so the code is the one rounding there is
+// max |x| <= 448 * 2^e over the finite x, and codes e4m3(x * 2^-e): with a power of two the product is exact, so the code is the one rounding there is
 // (half a step, 2^-4 of the value above 2^-6 * 2^e), and a page that later receives a larger token is re-expressed exactly but for what
 // falls under the new scale's smallest normal number.  A mantissa in the scale would gain nothing: the step of a floating-point
-// code is relative.  Values beyond 448 * 2^32 and infinities saturate; NaN stays NaN and does not count for the scale.
+// code is relative.  Infinities and NaN do not count for the scale (one infinity would take e to 32 and its page's other tokens to zero): infinities, as
+// values beyond 448 * 2^32, become +-448 * 2^e, NaN stays NaN.
 //
 // Layouts are the operand order of the attention that reads them (16 bytes = what one lane feeds to two matrix instructions):
 //   K (pages, kv, hd / 16, page, 16): 16 dims of one token          V (pages, kv, page / 16, hd, 16): 16 tokens of one dim

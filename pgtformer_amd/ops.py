@@ -1028,6 +1028,7 @@ def mha(q, k, v, B, L, heads, hd, scale, x3=None):
 
 
 # ---- attention over a cache of earlier tokens (include/pgt_hip.h has the definitions) ----------------------------------------
+# As everywhere in this module, results carry no autograd graph, whatever the inputs require: qk_norm_rope_backward is the gradient to call.
 def _need(ok, what, *args):
     if not ok:
         raise hip.PgtError(what % args if args else what)
@@ -1249,7 +1250,7 @@ def _seq_args(table, lens, cu, rows, most, what):
 def kv_append(cache, k, v, table, lens, cu=None, *, max_new=None):
     """Quantise the rows k, v (rows, kv_heads * hd) into the cache: sequence b's (rows cu[b] .. cu[b + 1] - 1; cu None: rows / B each) become
     its tokens lens[b] .. .  lens: int32 (B,), tokens BEFORE the call (the caller counts on).  max_new: most rows of one sequence - the
-    launch covers so many (default with cu: all rows, correct but a larger launch)."""
+    launch covers so many (default with cu: all rows, correct but a larger launch); rows of a sequence beyond them are left out."""
     if (nat := _native(k)) is not None:
         r = nat[0].kv_append(nat[1], nat[2], cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, cache.pages, cache.page, cache.kv_heads, cache.hd,
                              table, lens, cu, k, v, max_new)
@@ -1294,7 +1295,8 @@ def kv_attention(q, cache, table, lens, cu=None, *, heads, max_new=None, causal=
     """softmax(scale * q K^T) V over the cache: q (rows, heads * hd), row i of the n rows of sequence b at position lens[b] - n + i, lens[b]
     (int32) the tokens the cache holds INCLUDING these rows'.  causal: 0 = every token, c = those up to the end of the block of c tokens that
     the position lies in (1 = token by token, tokens per frame = whole frames); window > 0: only the last `window` of these.  A row that
-    sees nothing is zero; rows that no sequence owns stay as they are in `out`.  scale: default hd ** -0.5."""
+    sees nothing is zero, as is one at a position below 0; rows that no sequence owns, or beyond the first max_new of a sequence, stay as they are in
+    `out`.  lens beyond the table (width * page) counts as that.  scale: default hd ** -0.5."""
     if out is None and (nat := _native(q)) is not None:
         r = nat[0].kv_attention(nat[1], nat[2], cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale, cache.pages, cache.page, cache.kv_heads, cache.hd,
                                 table, lens, cu, q, heads, max_new, causal, window, scale)
