@@ -121,3 +121,106 @@ def test_scores_of_any_size(case, n, scale):
         want = want.reshape(cu[-1], -1)
         tol = (HALF[typ] + 2.0 ** (-21 if typ == "f32" else -11)) * (1 + 2.0 ** -7) * want.abs() + TINY[typ]
         close(got[pick], want[pick].cpu(), tol[pick].cpu(), sign)
+
+
+def test_broken_offsets_are_bounded_and_what_they_leave_is_processed():
+    """descending, negative, past the end: a sequence owns what is left of its range inside the rows"""
+    heads, kv, hd, page, pages = 4, 2, 64, 16, 12
+    cache, ref, table, g = filled(3, 4, pages, kv, page, hd, [64, 64, 64], 31)
+    tab = table.clone()
+    tab[2] = -7
+    q = torch.randn((13, heads * hd), generator=g)
+    out = torch.full((13, heads * hd), 2.0, device=DEV)
+    ops.kv_attention(q.to(DEV), cache, tab.to(DEV), ints([60, 60, 60]), ints([9, 3, -1, 500]), heads=heads, out=out)
+    assert bool((out == 0).all())      # all 13 rows are the last sequence's, which has no page
+    out.fill_(2.0)
+    ops.kv_attention(q.to(DEV), cache, table.to(DEV), ints([60, 60, 60]), ints([9, 3, -1, 500]), heads=heads, out=out)
+    want, wv, amax = kv_ref.attention(q, ref, table, [60, 60, 60], [0, 0, 0, 13], heads, 1, 0, 0.125)
+    close(out, want, attn_tol("f32", want, wv, amax, 60))
+    before = [t.clone() for t in (cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale)]
+    k = torch.randn((40, kv * hd), generator=g)
+    tab = torch.tensor([[2, -1, 1 << 30], [pages, -5, 4]], dtype=torch.int32)
+    ops.kv_append(cache, k.to(DEV), k.to(DEV), tab.to(DEV), ints([0, 0]), ints([30, -4, 1000]))
+    # the first sequence owns nothing, the second all 40 rows: its tokens 32 .. 39 are on page 4
+    for old, now in zip(before, (cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale)):
+        assert [i for i in range(pages) if not torch.equal(old[i], now[i])] == [4]
+    part = kv_ref.Cache(pages, kv, page, hd)
+    part.append(k[32:], k[32:], torch.tensor([[4]]), [0], [0, 8])
+    codes, scales = gpu_codes(cache)
+    for w in range(2):
+        assert torch.equal(codes[w][4], part.code[w][4]) and torch.equal(scales[w][4], torch.exp2(part.e[w][4].double()))
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+def test_many_rows_past_32_bits(typ):
+    """the 256-column kernel on pages behind 4 GiB, NaN values among them, against the same tokens in a small cache"""
+    kv, hd, page, heads, rows, length = 8, 128, 128, 256, 200, 300
+    pages = 33000      # x 128 KiB = 4.03 GiB
+    mk = lambda *s, dt=torch.uint8: torch.empty(s, dtype=dt, device=DEV)      # noqa: E731
+    cache = ops.KvCache(mk(pages, kv, hd // 16, page, 16), mk(pages, kv, page // 16, hd, 16), mk(pages, kv, dt=torch.float32), mk(pages, kv, dt=torch.float32))
+    small = ops.KvCache.alloc(4, kv, page, hd, DEV)
+    cache.v_pages[0], cache.k_pages[0] = 0x7f, 0x7f
+    g = torch.Generator().manual_seed(751)
+    k, v = (torch.randn((length, kv * hd), generator=g).to(DT[typ]).to(DEV) for _ in range(2))
+    zero = ints([0])
+    ta, tb = ints([[pages - 1, pages - 2, pages - 3]]), ints([[1, 3, 2]])
+    q = torch.randn((rows, heads * hd), generator=g).to(DT[typ]).to(DEV)
+    for nan in (False, True):
+        got = []
+        for c, t in ((cache, ta), (small, tb)):
+            ops.kv_append(c, k, v, t, zero)
+            if nan:
+                pid = int(t[0, 1])
+                c.v_pages[pid, 3, 5, 77, 9] = 0x7f      # token 128 + 5 * 16 + 9 = 217 of kv head 3
+            got.append(ops.kv_attention(q, c, t, zero + length, heads=heads))
+        assert torch.equal(got[0].isnan(), got[1].isnan()) and torch.equal(got[0].nan_to_num(), got[1].nan_to_num())
+        hit = torch.zeros_like(got[0], dtype=torch.bool).reshape(rows, heads, hd)
+        if nan:
+            hit[217 - (length - rows):, 3 * 32:4 * 32, 77] = True
+        assert torch.equal(got[0].isnan(), hit.reshape(rows, -1))
+    del cache
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("case", range(len(MANY)))
+def test_which_kernel_the_cases_of_many_rows_reach(case):
+    """the 256-column kernel runs in all of them but fp32 at 128 dims"""
+    B, kv, heads, hd, page, width, most, causal, window, scale, typ = MANY[case]
+    cache, _, table, g = make_cache(B, width, kv, page, hd, 760)
+    q = torch.zeros((B * most, heads * hd), dtype=DT[typ], device=DEV)
+    with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+        ops.kv_attention(q, cache, table, ints([width * page] * B), heads=heads, causal=causal, window=window, scale=scale)
+        torch.cuda.synchronize()
+    names = [e.name for e in prof.events() if "kv_attn" in e.name]
+    assert names
+    assert any("kv_attn_rows_kernel" in n for n in names) == (not (typ == "f32" and hd == 128)), names
+
+
+def test_recorded_calls_replay_from_the_file(tmp_path):
+    """norm + rotation, append and attention as a program: a replay gives what the recorded calls gave.  The cache and the lengths in the file are those of
+    the moment the file was written, so the file is written before the recorded calls' own effects (the tokens they append are the same)"""
+    from pgtformer_amd import export
+    B, heads, kv, hd, page, width = 2, 8, 2, 64, 16, 4
+    cache, _, table, g = filled(B, width, B * width, kv, page, hd, [30, 17], 771)
+    tab, before, after = table.to(DEV), ints([30, 17]), ints([31, 18])
+    freqs = ops.rope_freqs(hd, device=DEV)
+    qkv = torch.randn((B, (heads + 2 * kv) * hd), generator=g).to(torch.bfloat16).to(DEV)
+    raw, out = qkv.view(torch.uint8), torch.zeros((B, heads * hd), dtype=torch.bfloat16, device=DEV)
+
+    def step():
+        q, k = ops.qk_norm_rope(qkv[:, :heads * hd], qkv[:, heads * hd:(heads + kv) * hd], before, freqs, heads=heads, kv_heads=kv)
+        ops.kv_append(cache, k, qkv[:, (heads + kv) * hd:], tab, before)
+        return ops.kv_attention(q, cache, tab, after, heads=heads, out=out)
+    keep = (cache.k_pages, cache.v_pages, cache.k_scale, cache.v_scale)
+    state = [t.clone() for t in keep]
+    persistent = export._live_cuda_storages(DEV)
+    calls, _ = export.record(step, DEV)
+    want = out.clone()
+    for t, was in zip(keep, state):
+        t.copy_(was)
+    tape, layout, work = export.build_program(calls, persistent, raw, out.view(torch.uint8))
+    path = str(tmp_path / "step.prog")
+    export.write_program(path, tape, layout, work, raw.numel(), out.view(torch.uint8).numel(), storages=persistent)
+    assert len(tape) == 3
+    got = export.run_program(path, raw)
+    assert torch.equal(got.view(torch.bfloat16).reshape(out.shape), want)
