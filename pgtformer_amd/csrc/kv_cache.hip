@@ -94,7 +94,7 @@ struct KvP {
 // what the workgroup works on: sequence b, its packed rows, page `idx` of the sequence, or nothing
 struct Spot {
     bool any;
-    int row0, first, t_lo, t_hi, half, head;      // token t of the page is packed row row0 + (t - t_off)
+    int row0, t_lo, t_hi, half, head;      // token t of the page is packed row row0 + (t - t_off)
     int t_off;
     size_t id;
 };

@@ -225,3 +225,42 @@ def test_recorded_calls_replay_from_the_file(tmp_path):
     assert len(tape) == 3
     got = export.run_program(path, raw)
     assert torch.equal(got.view(torch.bfloat16).reshape(out.shape), want)
+
+
+def test_captured_gradient_and_read():
+    """a norm + rotation with its gradient, and the read of a cache, captured: every replay on new values gives what the eager calls give"""
+    rows, heads, kv, hd, page, width = 700, 8, 2, 64, 16, 4
+    g = torch.Generator().manual_seed(781)
+    cache, _, table, _ = filled(2, width, 2 * width, kv, page, hd, [60, 33], 782)
+    tab, start, freqs = table.to(DEV), ints([3, 0]), ops.rope_freqs(32, device=DEV)
+    x = torch.empty((rows, (heads + kv) * hd), dtype=torch.float16, device=DEV)
+    dy, pos, gain = torch.empty_like(x), torch.empty(rows, dtype=torch.int32, device=DEV), torch.ones(hd, device=DEV)
+
+    def step():
+        q, k, dq, dk = x[:, :heads * hd], x[:, heads * hd:], dy[:, :heads * hd], dy[:, heads * hd:]
+        kw = dict(heads=heads, kv_heads=kv)
+        return [*ops.qk_norm_rope(q, k, pos, freqs, gain, gain, **kw), *ops.qk_norm_rope_backward(dq, dk, q, k, pos, freqs, gain, gain, **kw),
+                *ops.kv_read(cache, tab, start, 60, torch.float16)]
+
+    def fill():
+        x.copy_(torch.randn(x.shape, generator=g))
+        dy.copy_(torch.randn(x.shape, generator=g))
+        pos.copy_(torch.randint(0, 1 << 20, (rows,), generator=g))
+        gain.copy_(torch.rand(hd, generator=g))
+        start.copy_(torch.randint(0, 30, (2,), generator=g))
+    fill()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for _ in range(4):
+        fill()
+        want = [t.clone() for t in step()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert len(outs) == 8 and all(torch.equal(a, b) for a, b in zip(outs, want))
