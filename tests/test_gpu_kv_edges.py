@@ -263,4 +263,6 @@ def test_captured_gradient_and_read():
         torch.cuda.synchronize()
         graph.replay()
         torch.cuda.synchronize()
-        assert len(outs) == 8 and all(torch.equal(a, b) for a, b in zip(outs, want))
+        assert len(outs) == 8
+        for i, (a, b) in enumerate(zip(outs, want)):      # (tokens behind the last one of `filled` read as NaN)
+            assert (i > 5 or not bool(b.isnan().any())) and torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num()), i
