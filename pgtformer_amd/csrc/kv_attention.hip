@@ -14,8 +14,8 @@
 // holds: P goes from the accumulators into the operand without an exchange.
 // The query columns are the group's heads times the tokens (column = token * group + head in group).
 //
-// Single tokens are bound by reading the cache once: 48 sequences of up to 8191 tokens, 32 / 8 heads of 128: 515 MB in 89 us, 5.8 TB/s (a plain
-// streaming read: 7.1); one of 131071, 40 / 8 heads: 268 MB in 46 us, of which some 8 are start and end.  Every wave has a tile in LDS and one
+// Single tokens are bound by reading the cache once: 48 sequences of up to 8191 tokens, 32 / 8 heads of 128: 515 MB in 88 us, 5.9 TB/s (a plain
+// streaming read: 7.1; fp32 queries, 48 of 8191: 6.0); one of 131071, 40 / 8 heads: 268 MB in 46 us, of which some 8 are start and end.  Every wave has a tile in LDS and one
 // in registers; the loads write LDS directly, since in registers the compiler waits for all of them wherever one is moved (113 us), and two
 // tiles per wave in LDS leave half the waves (96).
 #include "kv_attention.h"
@@ -421,16 +421,19 @@ template <typename T, int HD> __global__ __launch_bounds__(256) void kv_attn_joi
 // How a call is run: column tiles of 16 (this file) or 256 (kv_attention_rows.hip), and the workgroups that share the work (0: one per column
 // tile, no join).  Lengths are only known on the device; the table's width bounds them.
 //
-// 256 columns, in units of a tile's time (2.2 us at hd 128, 1.6 at 64): one workgroup per column tile takes ceil(segs / 256) * tiles + 4, of
-// ragged lengths some 1.25 times that; shared, segs * tiles / 256 + 16 for the look-up, second segments and the join.  Shared against not, us: 8
-// segments of 64 tiles 32 / 101 (hd 64), 40 / 126 (128); 64 of 8: 36 / 20, 48 / 26; 256 of 32: 80 / 59, 107 / 79; 256 of 160 and 512 of 128,
-// ragged: 172 / 230, 437 / 559.  From 1024 segments on the dispatch evens lengths out by itself: 16 tiles 139 / 125, 202 / 163, 128 tiles 798 /
-// 784, 1163 / 1110.
-// 16 columns: the whole chip does a tile of 1024 segments in about that unit.  16 columns against 256, us: 1 sequence of 65536, 64 columns 52 / 67
-// (hd 64), 49 / 77 (128), 128 columns 92 / 71, 79 / 81; 16 of 8192, 128 columns 160 / 94, 169 / 119; 64 of 1024, 64 columns 34 / 60, 54 / 79,
-// 128 columns 63 / 64, 100 / 86, 256 columns 116 / 80, 194 / 110; 4 of 700, 256 columns 10 / 30, 13 / 39.  fp32 (hd 64; at 128 its three planes
-// of q do not fit the registers of a wave of 32 columns): 2 of 8192, 8192 columns 764 / 552; 64 of 1024, 256 columns 170 / 96; 4 of 2048, 512
-// columns 38 / 47.
+// 256 columns, in units of a tile's time (2.2 us at hd 128, 1.5 at 64): one workgroup per column tile takes ceil(segs / 256) * tiles + 4, of
+// ragged lengths some 1.25 times that; shared, segs * tiles / 256 + 16 for the look-up, second segments and the join.  Shared against not, us, equal
+// lengths: 64 segments of 60 tiles 52 / 97 (hd 64), 66 / 119 (128), of 28 tiles 39 / 52, 53 / 65; 256 of 12: 54 / 32, 74 / 44; 256 of 60: 120 / 101,
+// 165 / 136; ragged, 256 of 160 and 512 of 128: 172 / 230, 437 / 559.  From 1024 segments on the dispatch evens lengths out by itself: 12 tiles 124 /
+// 118, 175 / 158, 124 tiles 748 / 740, 1105 / 1039.
+// 16 columns: the whole chip does a tile of 1024 segments in about that unit.  16 columns against 256, us: 1 sequence of 65536, 48 columns 35 / 60
+// (hd 64), 71 / 73 (128), 64 columns 52 / 60, 49 / 73, 96 columns 44 / 62, 129 / 76, 128 columns 92 / 63, 78 / 77; 16 of 8192, 48 columns 52 / 80,
+// 137 / 106, 64 columns 99 / 80, 86 / 106, 96 columns 85 / 85, 155 / 111, 128 columns 157 / 87, 163 / 115; 64 of 1024, 64 columns 33 / 44, 51 / 61,
+// 128 columns 59 / 50, 96 / 67, 256 columns 114 / 64, 185 / 94; 4 of 700, 256 columns 10 / 29, 13 / 41.  The model does not see that the column tiles
+// of a (sequence, kv head) read the same pages, which costs one reading where their pieces of the line run in step and several where they do not: of
+// these it takes the slower kernel for 48 columns of 16 x 8192 and 96 of 65536 at hd 128, and for 64 of 16 x 8192 at hd 64.
+// fp32 (hd 64; at 128 its three planes of q do not fit the registers of a wave of 32 columns): 2 of 8192, 8192 columns 764 / 552; 64 of 1024, 256
+// columns 170 / 96; 4 of 2048, 512 columns 38 / 47.  At hd 128 the 16 columns take 1170 for 2 of 8192, 8192 columns, 1.13 times its five products.
 struct Way {
     int cshift, wgs;
     size_t segs, slots;      // column tiles of the launch; slots of partial results

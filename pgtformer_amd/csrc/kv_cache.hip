@@ -12,9 +12,9 @@
 //
 // One workgroup per (page, head, K | V), 32 elements per thread: a maximum over the new tokens, then the codes.  K: two runs of 16 dims
 // of a token; V: 16 tokens x 2 dims, transposed in registers.
-// Memory bound only where much is written at once: 16396 tokens of 8 heads of 64 in half, 50 MB each way: append 19 us (2.6 TB/s; 7392 workgroups that
-// live some 6 us each, with K and V in one workgroup the same), read 14.5 (3.5).  A token for each of 48 sequences: 5.7 and 4.8 us, the chain of
-// index, scale and data loads.
+// Much at once - 16396 tokens of 8 heads of 64 in half, 50 MB each way - is bound by the start and end of 7392 short workgroups: append 18 us (2.8
+// TB/s; they live some 6 us each, with K and V in one workgroup the same), read 14 (3.5; a copy: 5.1).  A token for each of 48 sequences: 5.8 and
+// 4.6 us, the chain of index, scale and data loads.
 #include <cfloat>
 
 #include "kv_common.h"

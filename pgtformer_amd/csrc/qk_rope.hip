@@ -8,8 +8,8 @@
 // Memory bound: x is read once and y written once.  hd / 8 (or hd / 16) lanes hold a head row, two runs of 4 (8) elements each, picked so that
 // both halves of every pair sit in one lane (a rotation needs no exchange; the mean is a few lane exchanges).  The angle is taken in fp64 and
 // reduced to a fraction of a turn before it is rounded to fp32 - exact for any int32 position - once per token and pair, into
-// LDS, for all heads of the token.  16411 tokens of 32 + 8 heads of 128 in bf16: 65 us, 5.2 TB/s (a copy: 5.1); the gradient of 8190: 49 us, 5.1
-// TB/s, and 4.6 for the sums of the gain gradients.  Issue counts: a division per row, selects between q and k and an exact root cost 10 us.
+// LDS, for all heads of the token.  16411 tokens of 32 + 8 heads of 128 in bf16: 63 to 69 us, 5.3 to 4.8 TB/s (a copy: 5.1); the gradient of
+// 8190: 49 to 52 us, 5.1 to 4.8 TB/s, and 4.7 for the sums of the gain gradients.  Issue counts: a division per row, selects between q and k and an exact root cost 10 us.
 #include "kv_common.h"
 #include "pgt_internal.h"
 
