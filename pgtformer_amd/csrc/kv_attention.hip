@@ -513,7 +513,8 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
     p.wgs = w.wgs;
     p.jrows = w.cshift == 4 && max_new * p.group < 16 ? max_new * p.group : 1 << w.cshift;
     const size_t wgs = w.wgs ? w.wgs : w.segs;
-    PGT_CHECK(w.segs < (1ULL << 31), "kv_attention: %d sequences of up to %d tokens exceed one launch", B, max_new);
+    PGT_CHECK(w.segs < (1ULL << 31) && wgs * (w.cshift == 4 ? 256 : 512) < (1ULL << 32),      // (a grid's threads are counted in 32 bits)
+              "kv_attention: %d sequences of up to %d tokens each exceed one launch", B, max_new);
     if (w.wgs) {
         PGT_CHECK((double)w.segs * (((int64_t)width << p.pshift) / 64 + 1) < 1073741824.0,
                   "kv_attention: %d sequences of up to %d pages of %d tokens exceed one launch", B, width, page);

@@ -311,12 +311,13 @@ int check(const char* what, int dtype, const KvP& p, int page, const void* a, co
     PGT_CHECK((((uintptr_t)a | (uintptr_t)b) & 15) == 0, "%s: misaligned pointer", what);
     return 0;
 }
-// workgroups of a launch: every page that `per_seq` tokens can touch, each kv head, K and V; 0 = does not fit a grid
+// workgroups of a launch: every page that `per_seq` tokens can touch, each kv head, K and V; 0 = does not fit a grid, whose threads are counted in 32 bits
+unsigned threads(const KvP& p) { return max((p.hd << p.pshift) / 32, 64); }
 unsigned groups(KvP& p) {
     const int64_t page = 1 << p.pshift;
     p.npg = (int)((p.per_seq + 2 * page - 2) / page);
     const int64_t g = (int64_t)p.B * p.npg * p.kv * 2;
-    return g < (1LL << 31) ? (unsigned)g : 0;
+    return g < (1LL << 31) && g * threads(p) < (1LL << 32) ? (unsigned)g : 0;
 }
 
 }  // namespace
@@ -332,8 +333,8 @@ extern "C" int pgt_kv_append(int32_t dtype, const void* k, int32_t ldk, const vo
     if (const int rc = check("kv_append", dtype, p, page, k, v, ldk, ldv)) return rc;
     if (B == 0 || rows == 0 || max_new == 0 || width == 0) return 0;
     const unsigned g = groups(p);
-    PGT_CHECK(g, "kv_append: %d sequences of up to %d tokens exceed one launch", B, max_new);
-    const dim3 blk(page * hd < 2048 ? 64 : page * hd / 32);
+    PGT_CHECK(g, "kv_append: %d sequences of up to %d tokens each exceed one launch", B, max_new);
+    const dim3 blk(threads(p));
     hipStream_t st = (hipStream_t)stream;
     if (dtype == PGT_F32) hipLaunchKernelGGL(kv_append_kernel<float>, dim3(g), blk, 0, st, p);
     else if (dtype == PGT_BF16) hipLaunchKernelGGL(kv_append_kernel<bf16_t>, dim3(g), blk, 0, st, p);
@@ -353,8 +354,8 @@ extern "C" int pgt_kv_read(int32_t dtype, void* k_out, int32_t ldk, void* v_out,
     if (const int rc = check("kv_read", dtype, p, page, k_out, v_out, ldk, ldv)) return rc;
     if (B == 0 || rows == 0 || max_rows == 0) return 0;
     const unsigned g = groups(p);
-    PGT_CHECK(g, "kv_read: %d sequences of up to %d tokens exceed one launch", B, max_rows);
-    const dim3 blk(page * hd < 2048 ? 64 : page * hd / 32);
+    PGT_CHECK(g, "kv_read: %d sequences of up to %d tokens each exceed one launch", B, max_rows);
+    const dim3 blk(threads(p));
     hipStream_t st = (hipStream_t)stream;
     if (dtype == PGT_F32) hipLaunchKernelGGL(kv_read_kernel<float>, dim3(g), blk, 0, st, p);
     else if (dtype == PGT_BF16) hipLaunchKernelGGL(kv_read_kernel<bf16_t>, dim3(g), blk, 0, st, p);

@@ -300,7 +300,8 @@ extern "C" int pgt_qk_norm_rope(int32_t dtype, const void* q, int32_t ldq, const
     // lane costs more (4 tokens: 4.7 instead of 3.9)
     p.run = dtype != PGT_F32 && rot % 16 == 0 && p.tok > 1 ? 8 : 4;
     const int ng = 256 / (hd / (2 * p.run)), nh = heads + kv_heads;
-    const dim3 grid((rows + p.tok - 1) / p.tok, p.tok == 1 ? (nh + ng - 1) / ng : 1);
+    const int nblk = (rows + p.tok - 1) / p.tok;      // (a grid's threads are counted in 32 bits: a workgroup takes every 2^22-th block of tokens)
+    const dim3 grid(nblk < (1 << 22) ? nblk : 1 << 22, p.tok == 1 ? (nh + ng - 1) / ng : 1);
     PGT_CHECK(grid.y <= 65535, "qk_norm_rope: %d heads", nh);
     launch<false>(dtype, hd, p, grid, (hipStream_t)stream);
     PGT_LAUNCH_CHECK();

@@ -266,3 +266,21 @@ def test_captured_gradient_and_read():
         assert len(outs) == 8
         for i, (a, b) in enumerate(zip(outs, want)):      # (tokens behind the last one of `filled` read as NaN)
             assert (i > 5 or not bool(b.isnan().any())) and torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num()), i
+
+
+def test_norm_and_rotation_of_more_rows_than_a_grid_has_blocks():
+    """2^26 rows and some: workgroups take several blocks of tokens; the last rows against a call of their own, the rows between by a sample"""
+    rows, hd, n = (1 << 26) + 4099, 32, 5000
+    x = torch.empty((rows, 2 * hd), dtype=torch.bfloat16, device=DEV)
+    g = torch.Generator(DEV).manual_seed(791)
+    for at in range(0, rows, 1 << 24):
+        x[at:at + (1 << 24)].normal_(generator=g)
+    pos = torch.arange(rows, dtype=torch.int32, device=DEV)
+    kw = dict(heads=1, kv_heads=1)
+    freqs = ops.rope_freqs(hd, device=DEV)
+    q, k = ops.qk_norm_rope(x[:, :hd], x[:, hd:], pos, freqs, **kw)
+    for part in (slice(rows - n, rows), slice(0, n), slice((1 << 24) - 7, (1 << 24) + n), slice((1 << 26) - 2500, (1 << 26) + 2500)):
+        a, b = ops.qk_norm_rope(x[part, :hd], x[part, hd:], pos[part], freqs, **kw)
+        assert torch.equal(a, q[part]) and torch.equal(b, k[part])
+    del x, q, k, pos
+    torch.cuda.empty_cache()

@@ -1,8 +1,10 @@
-"""Cached-attention operators without a GPU: what a fresh cache holds, outputs that a caller may not pass, sizes of more than 31 bits"""
+"""Cached-attention operators without a GPU: what a fresh cache holds, outputs that a caller may not pass, sizes of more than 31 bits, grids of more threads than a
+launch can have"""
 import pytest
 import torch
 
 from pgtformer_amd import hip, ops
+from tests.test_kv_host import P, refused
 
 
 def test_a_fresh_cache_holds_zeros_under_a_valid_scale():
@@ -54,3 +56,14 @@ def test_sizes_past_31_bits_are_refused():
     for kw in (dict(window=1 << 32), dict(window=(1 << 32) + 5), dict(causal=(1 << 32) + 1), dict(causal=1 << 31), dict(causal=-1), dict(window=-1)):
         with pytest.raises(hip.PgtError, match="causal="):
             ops.kv_attention(q, c, table, lens, heads=8, **kw)
+
+
+def test_launches_of_2_to_the_32_threads_are_refused():
+    """ragged rows without max_new ask for a launch that covers all rows of every sequence"""
+    kv = dict(dtype=0, k=P, ldk=512, v=P, ldv=512, kp=P, vp=P, ks=P, vs=P, pages=4, page=16, kv=8, hd=64, table=P, ldt=8, width=8, lens=P, cu=P, B=64,
+              rows=1 << 20, n=1 << 20, stream=None)      # 2^26 workgroups of 64 threads
+    for name in ("pgt_kv_append", "pgt_kv_read"):
+        refused(name, kv, [dict(), dict(page=128, hd=128, ldk=1024, ldv=1024, B=512)])      # 2^26 of 512
+    att = dict(dtype=0, q=P, ldq=512, kp=P, vp=P, ks=P, vs=P, pages=4, page=16, kv=8, hd=64, table=P, ldt=3, width=3, lens=P, cu=P, B=2048, rows=1 << 16, n=1 << 16,
+               heads=8, scale=0.1, causal=1, window=0, out=P, ldo=512, ws=P, nb=1 << 30, stream=None)      # 2^22 workgroups of 512 threads, or 2^26 of 256
+    refused("pgt_kv_attention", att, [dict(B=4096), dict(dtype=1, B=4096), dict(dtype=0, B=1 << 14, rows=1 << 18, n=1 << 14, hd=128, ldq=1024, ldo=1024)])
