@@ -182,8 +182,8 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
                 *reinterpret_cast<uint4*>(d + v_to) = half8(w.x, w.y);
                 *reinterpret_cast<uint4*>(d + v_to + HD * 16) = half8(w.z, w.w);
             }
-            if (lane < 2 && part == 0) {      // (a factor of 0 would turn masked scores into NaN: 1e-30 is as flat)
-                const float factor = have0 ? fmaxf(fabsf(p.c) * rscale, 1e-30f) : -1.f, ev = log2_scale(rscale);
+            if (lane < 2 && part == 0) {      // (a factor of 0 would turn masked scores into NaN: the least normal number is as flat)
+                const float factor = have0 ? fmaxf(fabsf(p.c) * rscale, 1.17549435e-38f) : -1.f, ev = log2_scale(rscale);
                 reinterpret_cast<float*>(&sscale[st][blk])[lane] = lane ? ev : factor;
             }
             // pages of the tiles ahead, and whether they are there

@@ -284,3 +284,19 @@ def test_norm_and_rotation_of_more_rows_than_a_grid_has_blocks():
         assert torch.equal(a, q[part]) and torch.equal(b, k[part])
     del x, q, k, pos
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("case", [0, 3, 10, 12])
+@pytest.mark.parametrize("size", [2.0 ** 100, 2.0 ** -90])
+def test_queries_of_any_size(case, size):
+    """queries and scale that only together give ordinary scores (size a power of two: the same roundings as without it)"""
+    B, kv, heads, hd, page, width, most, causal, window, scale, typ = MANY[case]
+    typ = "bf16" if typ == "f16" else typ
+    cache, vals, table, g = make_cache(B, width, kv, page, hd, 800 + case)
+    lens, new = [width * page - b % 7 for b in range(B)], ragged(B, most, 801, 1)
+    cu = offsets(new)
+    q = torch.randn((cu[-1], heads * hd), generator=g, device=DEV).to(DT[typ])
+    kw = dict(heads=heads, causal=causal, window=window, max_new=most)
+    want, wv, amax = attention64(q, vals, table, lens, cu, heads, causal, window, scale)
+    got = ops.kv_attention(q * size, cache, table, ints(lens), ints(cu), scale=scale / size, **kw)
+    close(got, want.cpu(), attn_tol(typ, want, wv, amax, max(lens)).cpu())
