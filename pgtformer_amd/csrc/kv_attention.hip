@@ -495,7 +495,7 @@ extern "C" int pgt_kv_attention(int32_t dtype, const void* q, int32_t ldq, const
               "kv_attention: pages=%d B=%d rows=%d tokens per sequence=%d table width=%d", pages, B, rows, max_new, width);
     PGT_CHECK(causal >= 0 && window >= 0 && (causal > 0 || window == 0), "kv_attention: causal=%d window=%d", causal, window);
     PGT_CHECK(((int64_t)width << p.pshift) <= 0x7fff0000, "kv_attention: %d pages of %d tokens: positions exceed 32 bits", width, page);      // (tiles are fetched ahead)
-    PGT_CHECK(scale - scale == 0.f, "kv_attention: scale must be finite");
+    PGT_CHECK(p.c - p.c == 0.f, "kv_attention: scale=%g must be finite, in units of log 2 too", scale);
     PGT_CHECK(k_pages && v_pages && k_scale && v_scale, "kv_attention: null cache");
     PGT_CHECK((((uintptr_t)k_pages | (uintptr_t)v_pages) & 15) == 0, "kv_attention: misaligned cache");
     if (B == 0 || rows == 0 || max_new == 0) return 0;

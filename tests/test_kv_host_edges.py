@@ -67,3 +67,9 @@ def test_launches_of_2_to_the_32_threads_are_refused():
     att = dict(dtype=0, q=P, ldq=512, kp=P, vp=P, ks=P, vs=P, pages=4, page=16, kv=8, hd=64, table=P, ldt=3, width=3, lens=P, cu=P, B=2048, rows=1 << 16, n=1 << 16,
                heads=8, scale=0.1, causal=1, window=0, out=P, ldo=512, ws=P, nb=1 << 30, stream=None)      # 2^22 workgroups of 512 threads, or 2^26 of 256
     refused("pgt_kv_attention", att, [dict(B=4096), dict(dtype=1, B=4096), dict(dtype=0, B=1 << 14, rows=1 << 18, n=1 << 14, hd=128, ldq=1024, ldo=1024)])
+
+
+def test_a_scale_that_leaves_fp32_is_refused():
+    att = dict(dtype=0, q=P, ldq=512, kp=P, vp=P, ks=P, vs=P, pages=4, page=16, kv=2, hd=64, table=P, ldt=3, width=3, lens=P, cu=None, B=2, rows=8, n=4,
+               heads=8, scale=0.1, causal=1, window=0, out=P, ldo=512, ws=P, nb=1 << 30, stream=None)
+    refused("pgt_kv_attention", att, [dict(scale=2.5e38), dict(scale=-3.4e38)])      # times log2 e: infinite
