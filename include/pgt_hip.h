@@ -348,7 +348,7 @@ int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const
  * negative = 0; pgt_kv_attention takes a lens beyond the table, width * page, as that, for the rows' positions too.  All index tensors live on the device and are bounded there: no value of theirs reaches outside the buffers.
  * pgt_kv_append: writes the rows k, v (kv_heads * hd) of sequence b to its tokens lens[b] .. (lens: tokens BEFORE the call).  A page that
  * held tokens of the sequence keeps the larger of its scale and the new tokens' - its codes are re-expressed under it; a page that begins
- * here is written whole, zeros behind the last token.  A page that is written to must belong to one sequence.
+ * here is written whole, zeros behind the last token.  A page that is written to must belong to one sequence, once.
  * pgt_kv_read: rows of sequence b <- its tokens start[b] .. , values rounded once to dtype.
  * pgt_kv_attention: out = softmax(scale * q K^T) V; q, out rows of heads * hd, `heads` a multiple of kv_heads (head h reads kv head
  * h / (heads / kv_heads)).  lens: tokens INCLUDING the rows' own: row i of the n rows that sequence b owns is at position p = lens[b] - n + i.
