@@ -338,14 +338,15 @@ int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const
 /* The cache holds keys and values in 8 bits, in pages of `page` tokens (16, 32, 64 or 128) of all kv heads; hd 64 or 128:
  *   k_pages (pages, kv_heads, hd / 16, page, 16), v_pages (pages, kv_heads, page / 16, hd, 16): e4m3 codes (OCP, no infinities);
  *   k_scale, v_scale (pages, kv_heads) fp32: value = code * scale, scale = 2^e with the least e in [-32, 32] for which the largest finite |x|
- *   of the page and head is <= 448 * 2^e.  Infinities and NaN do not count for the scale - one of them does not flush its page's other tokens to zero;
- *   infinities, and values beyond 448 * 2^32, become +-448 * 2^e, NaN stays NaN.
+ *   of the page and head is <= 448 * 2^e.  Infinities and NaN do not count for the scale (one infinity would flush
+ *   its page's other tokens to zero): infinities, and values beyond 448 * 2^32, become +-448 * 2^e, NaN stays NaN.
  *   Memory that was only cleared is a cache of zeros: a scale of 0 counts as 2^-32.
  * table (B, ld_table) int32: table[b][i] = page that holds tokens i * page .. of sequence b, `width` entries used; entries outside
  * [0, pages) and tokens past width * page are not there: nothing is written to them, they read as zeros, attention does not see them.
  * Sequence b owns rows cu[b] .. cu[b + 1] - 1 of the packed rows (cu: B + 1 int32 on the device, non-decreasing), of which a call processes the first
- * max_new / max_rows; cu == NULL: rows b * max_new .. .  Rows that no sequence owns or the call does not process are neither read nor written.  lens, start: int32 (B),
- * negative = 0; pgt_kv_attention takes a lens beyond the table, width * page, as that, for the rows' positions too.  All index tensors live on the device and are bounded there: no value of theirs reaches outside the buffers.
+ * max_new / max_rows; cu == NULL: rows b * max_new .. .  Rows that no sequence owns or the call does not process are neither read nor written.
+ * lens, start: int32 (B), negative = 0; pgt_kv_attention takes a lens beyond the table, width * page, as that, for the rows' positions too.
+ * All index tensors live on the device and are bounded there: no value of theirs reaches outside the buffers.
  * pgt_kv_append: writes the rows k, v (kv_heads * hd) of sequence b to its tokens lens[b] .. (lens: tokens BEFORE the call).  A page that
  * held tokens of the sequence keeps the larger of its scale and the new tokens' - its codes are re-expressed under it; a page that begins
  * here is written whole, zeros behind the last token.  A page that is written to must belong to one sequence, once.
@@ -356,7 +357,8 @@ int pgt_qk_norm_rope_backward(int32_t dtype, const void* dq, int32_t lddq, const
  *   frames of 1024 tokens up to its own.  window = w > 0 (with causal): of these the tokens >= e - w.
  * Weights carry 11 bits (fp32: 22) in the product with V, and an absolute error of 2^-32 of the row's largest product of a weight and its
  * page's V scale - less than that adds to the softmax sum only, which is fp32 throughout.
- * A row that sees no token is zero; a row at a position below 0 - a sequence of more rows than tokens - sees none, with causal == 0 either.  Deterministic for one shape of call (B, max_new, width, window choose how the work is split, and with it
+ * A row that sees no token is zero; a row at a position below 0 - a sequence of more rows than tokens - sees none, nor with causal == 0.
+ * Deterministic for one shape of call (B, max_new, width, window choose how the work is split, and with it
  * the order of the sums).  width * page <= 2^31 - 2^16.  workspace: pgt_kv_attention_workspace_bytes(...) bytes (0: may be NULL), scratch
  * of one call - calls that may run concurrently need their own. */
 int pgt_kv_append(int32_t dtype, const void* k, int32_t ldk, const void* v, int32_t ldv, void* k_pages, void* v_pages,

@@ -15,9 +15,9 @@
 // The query columns are the group's heads times the tokens (column = token * group + head in group).
 //
 // Single tokens are bound by reading the cache once: 48 sequences of up to 8191 tokens, 32 / 8 heads of 128: 515 MB in 88 us, 5.9 TB/s (a plain
-// streaming read: 7.1; fp32 queries, 48 of 8191: 6.0); one of 131071, 40 / 8 heads: 268 MB in 46 us, of which some 8 are start and end.  Every wave has a tile in LDS and one
-// in registers; the loads write LDS directly, since in registers the compiler waits for all of them wherever one is moved (113 us), and two
-// tiles per wave in LDS leave half the waves (96).
+// streaming read: 7.1; fp32 queries, 48 of 8191: 6.0); one of 131071, 40 / 8 heads: 268 MB in 46 us, of which some 8 are start and end.
+// Every wave has a tile in LDS and one in registers; the loads write LDS directly, since in registers the compiler waits for all of them
+// wherever one is moved (113 us), and two tiles per wave in LDS leave half the waves (96).
 #include "kv_attention.h"
 #include "pgt_internal.h"
 

@@ -94,7 +94,8 @@ template <typename T, int HD> __global__ __launch_bounds__(TH, 2) void kv_attn_r
             const uint32_t i = lane == 2 ? (uint32_t)min(page_index(t + 3, blk), p.width - 1) : pg;
             lds_load4(word + (uint64_t)i * word_step, to + SET - 256);
         };
-        bool have0 = false, have1 = false, have2 = false;      // whether the next three tiles have a page (scalars: 150 instead of 153 us for the frames, 354 / 360 the chunks)
+        // whether the next three tiles have a page (kept in scalars: 150 instead of 153 us for the frames, 354 / 360 for the chunks)
+        bool have0 = false, have1 = false, have2 = false;
         if (t0 < te) {      // the first three tiles are on their way while the columns are set up
             int pg[3];
 #pragma unroll

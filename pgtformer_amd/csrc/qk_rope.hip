@@ -9,7 +9,8 @@
 // both halves of every pair sit in one lane (a rotation needs no exchange; the mean is a few lane exchanges).  The angle is taken in fp64 and
 // reduced to a fraction of a turn before it is rounded to fp32 - exact for any int32 position - once per token and pair, into
 // LDS, for all heads of the token.  16411 tokens of 32 + 8 heads of 128 in bf16: 63 to 69 us, 5.3 to 4.8 TB/s (a copy: 5.1); the gradient of
-// 8190: 49 to 52 us, 5.1 to 4.8 TB/s, and 4.7 for the sums of the gain gradients.  Issue counts: a division per row, selects between q and k and an exact root cost 10 us.
+// 8190: 49 to 52 us, 5.1 to 4.8 TB/s, and 4.7 for the sums of the gain gradients.  Issue counts: a division per row, selects between q and k and an
+// exact root cost 10 us.
 #include "kv_common.h"
 #include "pgt_internal.h"
 
